@@ -48,6 +48,17 @@ EXPORTS = {
     "wf_linear_gguf_workspace": (_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
     "wf_linear_gguf_ws": (_int, [_p, _i64, _i64, _p, _i64, _int, _i64, _p, _p, _int, _p, _i64, _p]),
     "wf_linear_gguf_noalloc": (_int, [_p, _i64, _i64, _p, _i64, _int, _i64, _p, _p, _int, _p]),
+    "wf_layer_norm": (_int, [_p, _i64, _int, _p, _p, _int, _int, _i64, ctypes.c_float, _p, _p, _i64, _i64, _p]),
+    "wf_layer_norm_bwd_workspace": (_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "wf_layer_norm_bwd": (_int, [_p, _i64, _p, _i64, _int, _p, _int, _int, _i64, _p, _p, _p, _p, _i64, _i64, _p, _i64,
+                                 _p]),
+    "wf_dense_workspace": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "wf_dense": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _p, _int, _int, _p, _int, _i64, _p, _i64,
+                        _p, _p, _p, _i64, _p]),
+    "wf_dense_grad_workspace": (_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "wf_dense_grad": (_int, [_p, _i64, _p, _int, _int, _p, _int, _i64, _p, _p, _int, _p, _i64, _i64, _p, _i64, _p]),
+    "wf_adamw": (_int, [_p, _i64, _int, _int, _p, _p, _p, _p, _i64, _i64] + [ctypes.c_double] * 5 + [_p]),
+    "wf_adamw_values": (_int, [_p, _p, _p, _p, _i64, _p, _p, _p]),
     "wf_host_alloc": (_int, [_sz, ctypes.POINTER(ctypes.c_void_p)]),
     "wf_host_free": (_int, [_p]),
     "wf_h2d_async": (_int, [_p, _p, _sz, _p]),

@@ -171,6 +171,62 @@ int wf_linear_gguf_noalloc(const void* x_bf16, int64_t M, int64_t K, const void*
 int wf_linear_bf16(const void* x_bf16, const void* w_bf16, const void* bias_bf16, void* out_bf16, int64_t M, int64_t N,
                    int64_t K, void* stream);
 
+/* -------------------------------------------------------------------------------- a training step's operators
+ * No reference counterpart: the reference runs its models only; these fine-tune a block next to the inference path.
+ *
+ * LayerNorm over rows of K <= 32768 values of type dt: y = (x - mean) rstd s + b, s = w (plus_one 0) or 1 + w, each sum in
+ * float32. w and b (either may be NULL) are [M / rows_per_group, K] of type param_dt (dt or WF_F32), row r using row r /
+ * rows_per_group: rows_per_group = M for affine weights, the rows of one batch entry for a DiT block's modulation. x: M
+ * rows ldx values apart; y: [M, K]; stats (may be NULL): float32 [M, 2], mean and rstd, what the backward pass reads.
+ * Pointers need only their values' alignment. At most 65535 groups. */
+int wf_layer_norm(const void* x, int64_t ldx, int dt, const void* w, const void* b, int param_dt, int plus_one,
+                  int64_t rows_per_group, float eps, void* y, float* stats, int64_t M, int64_t K, void* stream);
+
+/* Its gradients: dx [M, K] of type dt, dw and db [M / rows_per_group, K] of type param_dt; any of the three may be NULL.
+ * dy: M rows ldd values apart. The workspace (needed for dw and db: the bytes that wf_layer_norm_bwd_workspace gives, 4-byte
+ * aligned) holds partial sums; they are added in a fixed order, so the results are the same on every run. */
+int wf_layer_norm_bwd_workspace(int64_t M, int64_t K, int64_t rows_per_group, int64_t* bytes);
+int wf_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldd, int dt, const void* w, int param_dt,
+                      int plus_one, int64_t rows_per_group, const float* stats, void* dx, void* dw, void* db, int64_t M,
+                      int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* y[m, n] = resid[m, n] + gate[m / rows_per_group, n] * act(sum_k x[m, k] * w[n, k] + bias[n]) in dt (WF_BF16 or WF_F16),
+ * float32 accumulation, one rounding. act: 0 none, 1 GELU (erf), 2 GELU (tanh), 3 SiLU, 4 ReLU. bias, gate, resid may be
+ * NULL; bias and gate have type dt or WF_F32 (bias_dt, gate_dt). An operand's value (r, k) is at r * row + k * col, so
+ * transposed views need no copy by the caller; resid's rows are resid_row values apart; y is [M, N]. h (may be NULL): the
+ * sums with the bias, [M, N] of type dt, what wf_dense_grad reads (float16: kept finite). M, N <= 2^24, K <= 2^20.
+ * The workspace (256-byte aligned, at least the bytes that wf_dense_workspace gives for the same operands) holds copies of
+ * operands that cannot be loaded as they are, and the partial sums of products that run in slices of K; it need not be
+ * cleared and is free again when the call's work on the stream is done. The products of the backward pass are this call
+ * too: dx = dh . w is (dh, w with row and col exchanged), dw = dh^T . x both exchanged. */
+int wf_dense_workspace(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt,
+                       int64_t M, int64_t N, int64_t K, int64_t* bytes);
+int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt, int64_t M,
+             int64_t N, int64_t K, const void* bias, int bias_dt, int act, const void* gate, int gate_dt,
+             int64_t rows_per_group, const void* resid, int64_t resid_row, void* y, void* h, void* workspace,
+             int64_t workspace_bytes, void* stream);
+
+/* The element-wise part of its backward pass: dh = dy gate act'(h) [M, N], dbias = the sum over rows of dh (bias_dt), dgate =
+ * the sum over each group's rows of dy act(h) (gate_dt); any of the three may be NULL. dy: rows dy_row values apart; h
+ * may be NULL when act is 0 and dgate NULL. Workspace as above, 4-byte aligned, only for dbias and dgate. */
+int wf_dense_grad_workspace(int64_t M, int64_t N, int64_t rows_per_group, int64_t* bytes);
+int wf_dense_grad(const void* dy, int64_t dy_row, const void* h, int dt, int act, const void* gate, int gate_dt,
+                  int64_t rows_per_group, void* dh, void* dbias, int bias_dt, void* dgate, int64_t M, int64_t N,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One AdamW step (step >= 1) of `count` tensors of type dt, in place: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ * p = (1 - lr decay) p - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps). table: host memory, read before the
+ * call returns: address of the parameter, address of its gradient, values, for each tensor. The moments are flat over all
+ * tensors, each starting on a whole block of 256 values, `blocks` in all: bits 32: float32 [blocks * 256], scales unused;
+ * bits 8: exp_avg int8, exp_avg_sq uint8 [blocks * 256] with float32 scales [blocks], m = sign(q) (q / 127)^2 s, v = ((q /
+ * 255)^2 s)^2, s a block's largest |m| or sqrt(v); a v > 0 keeps a code > 0. wf_adamw_values: the float32 values that 8-bit
+ * moments stand for. */
+int wf_adamw(const int64_t* table, int64_t count, int dt, int bits, void* exp_avg, void* exp_avg_sq, float* avg_scale,
+             float* sq_scale, int64_t blocks, int64_t step, double lr, double beta1, double beta2, double eps,
+             double weight_decay, void* stream);
+int wf_adamw_values(const int8_t* exp_avg, const uint8_t* exp_avg_sq, const float* avg_scale, const float* sq_scale,
+                    int64_t blocks, float* avg, float* sq, void* stream);
+
 /* ---------------------------------------------------------------------------------------- block streaming
  * Exact-size page-locked host memory: replaces PinnedHost's cudaHostRegister / cudaHostUnregister
  * (core/tiers/pinned.py:84-129); allocated page-locked (hipHostMalloc) instead of registered after the fact. */
