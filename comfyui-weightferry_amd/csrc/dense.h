@@ -7,71 +7,91 @@
 
 namespace wf {
 
-// Activations. All but the erf form of GELU are h times a factor that is the logistic of z = h (a + b h^2): GELU's tanh
-// form, since (1 + tanh z) / 2 is the logistic of 2 z, has a = 2 sqrt(2 / pi), b = 0.044715 a; SiLU a = 1, b = 0.
 enum { ACT_NONE = 0, ACT_GELU = 1, ACT_GELU_TANH = 2, ACT_SILU = 3, ACT_RELU = 4 };
-
-struct Act {
-    int kind;
-    float a, b;
-};
-inline Act act_of(int kind) {
-    const float c = 1.5957691216057308f;                                   // 2 sqrt(2 / pi)
-    return kind == ACT_GELU_TANH ? Act{kind, c, 0.044715f * c} : Act{kind, 1.0f, 0.0f};
-}
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float rcp_of(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// 1 / (1 + exp(-z)), one ulp of exp2 and of the reciprocal: far below the 16-bit outputs' rounding
-__device__ __forceinline__ float logistic(float z) { return rcp_of(1.0f + exp2_of(z * -1.4426950408889634f)); }
-
-// the normal distribution function by formula 7.1.26 of Abramowitz and Stegun (|error| < 1e-7), on the side where it is
-// small, and exp(-h^2 / 2) that it needs on the way
+// The normal distribution function by formula 7.1.26 of Abramowitz and Stegun (|error| < 1e-7), on the side where it is
+// small, and e = exp(-h^2 / 2) that it needs on the way. exp2 and the reciprocal are the hardware's, one ulp: far below the
+// 16-bit outputs' rounding.
 __device__ __forceinline__ float normal_cdf(float h, float& e) {
-    const float x = fabsf(h) * 0.7071067811865476f;
-    const float t = rcp_of(fmaf(0.3275911f, x, 1.0f));
+    const float t = rcp_of(fmaf(0.23164189f, fabsf(h), 1.0f));                           // 0.3275911 |h| / sqrt(2)
     e = exp2_of(h * h * -0.7213475204444817f);
-    const float q = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t,
-                         0.254829592f) * t * e * 0.5f;
+    const float q = fmaf(fmaf(fmaf(fmaf(0.5307027145f, t, -0.7265760135f), t, 0.7107068705f), t, -0.142248368f), t,
+                         0.127414796f) * t * e;                                          // the coefficients' halves
     return h < 0.0f ? q : 1.0f - q;
 }
+// GELU's tanh form is h times the logistic of 2 z, z = sqrt(2 / pi) (h + 0.044715 h^3), since (1 + tanh z) / 2 is that
+__device__ __forceinline__ float tanh_factor(float h) {
+    return rcp_of(1.0f + exp2_of(h * fmaf(-0.10294324f, h * h, -2.3022082f)));           // - 2 sqrt(2 / pi) log2(e) (...)
+}
+__device__ __forceinline__ float logistic(float h) { return rcp_of(1.0f + exp2_of(h * -1.4426950408889634f)); }
 
-// (h^2 is kept finite, so that b = 0 times it stays 0)
-__device__ __forceinline__ float act_z(const Act& f, float h) { return h * fmaf(f.b, fminf(h * h, 1e30f), f.a); }
-
-__device__ __forceinline__ float act_value(const Act& f, float h) {
-    if (f.kind == ACT_NONE) return h;
-    if (f.kind == ACT_RELU) return h < 0.0f ? 0.0f : h;
+// v = act(v) on a run of values; one decision a run
+__device__ __forceinline__ void act_run(int kind, float (&v)[8]) {
     float e;
-    return h * (f.kind == ACT_GELU ? normal_cdf(h, e) : logistic(act_z(f, h)));
-}
-
-__device__ __forceinline__ float act_slope(const Act& f, float h) {
-    if (f.kind == ACT_NONE) return 1.0f;
-    if (f.kind == ACT_RELU) return h > 0.0f ? 1.0f : 0.0f;
-    if (f.kind == ACT_GELU) {
-        float e;
-        const float phi = normal_cdf(h, e);
-        return fmaf(h * 0.3989422804014327f, e, phi);                      // 1 / sqrt(2 pi)
+    if (kind == ACT_GELU_TANH) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= tanh_factor(v[i]);
+    } else if (kind == ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= normal_cdf(v[i], e);
+    } else if (kind == ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= logistic(v[i]);
+    } else if (kind == ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];
     }
-    const float s = logistic(act_z(f, h));
-    const float dz = fmaf(3.0f * f.b, fminf(h * h, 1e30f), f.a);
-    return fmaf(h * s * (1.0f - s), dz, s);
 }
 
-// the pre-activation as it is kept for the backward pass: float16's infinity would make the slope 0 * infinity where the
-// float32 value gives a limit, so it stays finite
+// a = act(h) and its slope, from finite h (keep_finite)
+__device__ __forceinline__ void act_slope_run(int kind, const float (&h)[8], float (&a)[8], float (&slope)[8]) {
+    if (kind == ACT_GELU_TANH) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float s = tanh_factor(h[i]), dz = fmaf(0.21406614f, fminf(h[i] * h[i], 1e30f), 1.5957691f);
+            a[i] = h[i] * s;
+            slope[i] = fmaf(a[i] * (1.0f - s), dz, s);
+        }
+    } else if (kind == ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float e;
+            const float phi = normal_cdf(h[i], e);
+            a[i] = h[i] * phi;
+            slope[i] = fmaf(h[i] * 0.3989422804014327f, e, phi);                         // 1 / sqrt(2 pi)
+        }
+    } else if (kind == ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float s = logistic(h[i]);
+            a[i] = h[i] * s;
+            slope[i] = fmaf(a[i], 1.0f - s, s);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const bool on = kind == ACT_NONE || h[i] > 0.0f;
+            a[i] = on ? h[i] : h[i] < 0.0f ? 0.0f : h[i];
+            slope[i] = on ? 1.0f : 0.0f;
+        }
+    }
+}
+
+// the pre-activation as it is kept for the backward pass: an infinity (float16's, past 65504) would make the slope 0 *
+// infinity where its limit is 0 or 1, so it stays finite
 template <int D>
 __device__ __forceinline__ float keep_finite(float h) {
-    if constexpr (D == WF_F16) return h > 65504.0f ? 65504.0f : h < -65504.0f ? -65504.0f : h;
-    else return h;
+    constexpr float most = D == WF_F16 ? 65504.0f : 3.38953139e38f;
+    return h > most ? most : h < -most ? -most : h;
 }
 
 struct DenseEpilogue {
     const void *bias, *gate, *resid;       // any may be NULL
     int bias_dt, gate_dt;                  // the outputs' type or float32
-    Act act;
+    int act;
     int64_t rows_per_group, ldr;           // row m's gate is row m / rows_per_group of gate; resid's row stride
     void *y, *h;                           // [M, N]; h (may be NULL): the pre-activations
 };
@@ -85,11 +105,12 @@ __device__ __forceinline__ Pack<D> epilogue_prefetch(const DenseEpilogue& e, int
     return r;
 }
 
-template <int D>
+// v: a run's sums, without the bias when BIAS is set
+template <int D, bool BIAS>
 __device__ __forceinline__ void epilogue_run(const DenseEpilogue& e, float (&v)[8], const Pack<D>& r, int64_t m, int n,
                                              int N, int cnt) {
     float u[8];
-    if (e.bias) {
+    if (BIAS && e.bias) {
         load_params<8>(u, e.bias, n, cnt, e.bias_dt);
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] += u[i];
@@ -101,9 +122,7 @@ __device__ __forceinline__ void epilogue_run(const DenseEpilogue& e, float (&v)[
         o.put(u);
         o.store(static_cast<value_t<D>*>(e.h) + m * N + n, cnt);
     }
-    if (e.act.kind != ACT_NONE)
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = act_value(e.act, v[i]);
+    act_run(e.act, v);
     if (e.gate) {
         load_params<8>(u, e.gate, (int64_t)((uint32_t)m / (uint32_t)e.rows_per_group) * N + n, cnt, e.gate_dt);
 #pragma unroll

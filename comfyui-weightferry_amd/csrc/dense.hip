@@ -13,100 +13,9 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "dense.h"
-#include "dense_ring.h"
+#include "dense_gemm.h"
 
 namespace wf {
-
-typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
-
-template <int D>
-__device__ __forceinline__ f32x16v mma16(const f32x16v& c, const wl_frag& a, const wl_frag& b) {
-    if constexpr (D == WF_BF16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8v, a), __builtin_bit_cast(bf16x8v, b), c, 0,
-                                                       0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8v, a), __builtin_bit_cast(f16x8v, b), c, 0, 0,
-                                                      0);
-}
-
-struct DenseOperand {
-    const uint16_t* p;
-    int64_t row;                                      // values between rows
-    int k;                                            // values to load of a row (a copied row's zeros among them)
-};
-
-// workgroup (tile, slice); parts: [slices, M, N] float32 partial sums, or NULL: one slice and the epilogue
-template <int D, typename S>
-__global__ __launch_bounds__(S::NT) void dense_gemm(DenseOperand a, DenseOperand b, int M, int N, int K, int slice_stages,
-                                                    float* __restrict__ parts, DenseEpilogue e) {
-    constexpr int WM = S::WM, WN = S::WN, TC = WN * 32;
-    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS];
-    const int ntm = (M + S::BM - 1) / S::BM, ntn = (N + S::BN - 1) / S::BN;
-    int tm, tn;
-    tile_order(blockIdx.x, ntm * ntn, ntm, ntn, tm, tn);
-    const int m0 = __builtin_amdgcn_readfirstlane(tm * S::BM), n0 = __builtin_amdgcn_readfirstlane(tn * S::BN);
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int stages = (K + 63) / 64, s0 = blockIdx.y * slice_stages, nk = min(slice_stages, stages - s0);
-    // (a buffer ends with the last row's values: whole 16-byte runs, as dense_direct asks)
-    const DenseTile ta = {tile_rsrc(a.p + m0 * a.row, ((M - 1 - m0) * a.row + a.k) * 2), (uint32_t)a.row * 2u,
-                          (uint32_t)a.k * 2u};
-    const DenseTile tb = {tile_rsrc(b.p + n0 * b.row, ((N - 1 - n0) * b.row + b.k) * 2), (uint32_t)b.row * 2u,
-                          (uint32_t)b.k * 2u};
-    f32x16v acc[WM][WN];
-#pragma unroll
-    for (int i = 0; i < WM; i++)
-#pragma unroll
-        for (int j = 0; j < WN; j++)
-#pragma unroll
-            for (int x = 0; x < 16; x++) acc[i][j][x] = 0.0f;
-    dense_mainloop<S>(ta, tb, s0, nk, wave, lane, sb0, sb1, acc,
-                      [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<D>(c, x, y); });
-    const int mw = m0 + wave / S::VN * WM * 32, nw = n0 + wave % S::VN * TC;
-    const int lr = lane & 31, lk = lane >> 5;
-    // the wave's region: 16 rows x TC float32
-    constexpr int PER_BUF = S::SLOTS * 16 / (16 * TC * 4);
-    static_assert(2 * PER_BUF >= S::NW, "the output rows fit in the stage buffers");
-    float* ot = reinterpret_cast<float*>(wave < PER_BUF ? sb0 : sb1) + (wave % PER_BUF) * 16 * TC;
-    constexpr int RUNS = TC / 8;
-#pragma unroll
-    for (int half = 0; half < 2 * WM; half++) {
-        const int mi = mw + half * 16;
-        if (mi >= M) break;
-        Pack<D> res[WN];
-        if (!parts) {
-#pragma unroll
-            for (int it = 0; it < WN; it++) {
-                const int q = it * 64 + lane, m = mi + q / RUNS, n = nw + 8 * (q % RUNS);
-                res[it] = epilogue_prefetch<D>(e, m, n, m < M ? N - n : 0);
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < 8; x++)
-#pragma unroll
-            for (int j = 0; j < WN; j++)
-                ot[(8 * (x >> 2) + 4 * lk + (x & 3)) * TC + j * 32 + lr] = acc[half / 2][j][8 * (half & 1) + x];
-#pragma unroll
-        for (int it = 0; it < WN; it++) {
-            const int q = it * 64 + lane, m = mi + q / RUNS, n = nw + 8 * (q % RUNS);
-            const float4 lo = reinterpret_cast<const float4*>(ot)[2 * q], hi = reinterpret_cast<const float4*>(ot)[2 * q + 1];
-            if (m >= M || n >= N) continue;
-            float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-            if (parts) {
-                float* o = parts + ((int64_t)blockIdx.y * M + m) * N + n;
-                if (n + 8 <= N) __builtin_memcpy(o, v, 32);
-                else
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (n + i < N) o[i] = v[i];
-            } else {
-                epilogue_run<D>(e, v, res[it], m, n, N, N - n);
-            }
-        }
-    }
-}
 
 // the slices' sums in slice order, then the epilogue: one run of 8 outputs a thread
 template <int D>
@@ -130,7 +39,7 @@ __global__ __launch_bounds__(256) void dense_sum(const float* __restrict__ parts
 #pragma unroll
         for (int x = 0; x < 8; x++) v[x] += u[x];
     }
-    epilogue_run<D>(e, v, r, m, n, N, cnt);
+    epilogue_run<D, true>(e, v, r, m, n, N, cnt);
 }
 
 // rows of a strided operand (values row apart along its rows, col apart along K) as [R, KP] rows of whole stages, zeros
@@ -153,10 +62,6 @@ __global__ __launch_bounds__(256) void dense_pack(const uint16_t* __restrict__ p
 }
 
 // ------------------------------------------------------------------------------------------------- host side
-struct DensePlan {
-    int tiling, slices, slice_stages;
-};
-
 // the tilings, each with its outputs per modelled time (per mille of the largest's)
 struct DenseTiling {
     int bm, bn, eff;
@@ -184,54 +89,42 @@ static DensePlan dense_plan(int64_t M, int64_t N, int64_t K) {
     return best;
 }
 
-template <int D, int VM, int VN, int WM, int WN>
-static void dense_launch(const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p,
-                         float* parts, const DenseEpilogue& e, hipStream_t s) {
-    using S = DenseShape<VM, VN, WM, WN>;
-    const int tiles = ((M + S::BM - 1) / S::BM) * ((N + S::BN - 1) / S::BN);
-    dense_gemm<D, S><<<dim3(tiles, p.slices), S::NT, 0, s>>>(a, b, M, N, K, p.slice_stages, p.slices > 1 ? parts : nullptr,
-                                                             e);
-}
-
-template <int D>
-static void dense_run(const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p, float* parts,
-                      const DenseEpilogue& e, hipStream_t s) {
-    switch (p.tiling) {
-    case 0: dense_launch<D, 4, 2, 2, 5>(a, b, M, N, K, p, parts, e, s); break;
-    case 1: dense_launch<D, 2, 4, 4, 2>(a, b, M, N, K, p, parts, e, s); break;
-    case 2: dense_launch<D, 4, 2, 2, 3>(a, b, M, N, K, p, parts, e, s); break;
-    case 3: dense_launch<D, 2, 2, 4, 2>(a, b, M, N, K, p, parts, e, s); break;
-    case 4: dense_launch<D, 4, 1, 1, 5>(a, b, M, N, K, p, parts, e, s); break;
-    case 5: dense_launch<D, 2, 2, 2, 2>(a, b, M, N, K, p, parts, e, s); break;
-    case 6: dense_launch<D, 1, 4, 2, 1>(a, b, M, N, K, p, parts, e, s); break;
-    default: dense_launch<D, 1, 4, 1, 1>(a, b, M, N, K, p, parts, e, s); break;
-    }
+static void dense_run(int dt, const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p,
+                      float* parts, const DenseEpilogue& e, hipStream_t s) {
+    (a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : dense_gemm_along)(dt, a, b, M, N, K, p, parts, e, s);
     if (p.slices > 1) {
         const int64_t runs = (int64_t)M * ((N + 7) / 8);
-        dense_sum<D><<<dim3((uint32_t)((runs + 255) / 256)), 256, 0, s>>>(parts, p.slices, M, N, e);
+        const dim3 grid((uint32_t)((runs + 255) / 256));
+        if (dt == WF_BF16) dense_sum<WF_BF16><<<grid, 256, 0, s>>>(parts, p.slices, M, N, e);
+        else dense_sum<WF_F16><<<grid, 256, 0, s>>>(parts, p.slices, M, N, e);
     }
 }
 
-// whether rows along K can be loaded as they are: 16-byte runs, a row's bytes and a tile's rows inside 32-bit offsets
-static bool dense_direct(const void* p, int64_t row, int64_t col, int64_t K) {
+// whether an operand can be loaded as it is, along K or across it: 16-byte runs, offsets inside 31 bits
+static bool dense_along(const void* p, int64_t row, int64_t col, int64_t K) {
     return col == 1 && row % 8 == 0 && K % 8 == 0 && row >= K && row <= (1 << 20) && aligned(p, 16);
+}
+static bool dense_across(const void* p, int64_t row, int64_t col, int64_t R, int64_t K) {
+    return row == 1 && col % 8 == 0 && col >= R && aligned(p, 16) && (K + 128) * col * 2 < (1LL << 31);
 }
 
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 struct DenseNeeds {
-    bool pack_x, pack_w;
-    int64_t kp, x_at, w_at, parts_at, bytes;          // offsets into the workspace
+    bool across_x, across_w, copy_x, copy_w;
+    int64_t kp, w_at, parts_at, bytes;                // a copy's row; offsets into the workspace, x's copy first
 };
 static DenseNeeds dense_needs(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col,
                               int64_t M, int64_t N, int64_t K, const DensePlan& p) {
     DenseNeeds d;
-    d.pack_x = !dense_direct(x, x_row, x_col, K);
-    d.pack_w = !dense_direct(w, w_row, w_col, K);
+    const bool along_x = dense_along(x, x_row, x_col, K), along_w = dense_along(w, w_row, w_col, K);
+    d.across_w = !along_w && dense_across(w, w_row, w_col, N, K);
+    d.across_x = !along_x && d.across_w && dense_across(x, x_row, x_col, M, K);   // (x across and w along: x is copied)
+    d.copy_x = !along_x && !d.across_x;
+    d.copy_w = !along_w && !d.across_w;
     d.kp = up(K, 64);
-    d.x_at = 0;
-    d.w_at = d.pack_x ? up(M * d.kp * 2, 256) : 0;
-    d.parts_at = d.w_at + (d.pack_w ? up(N * d.kp * 2, 256) : 0);
+    d.w_at = d.copy_x ? up(M * d.kp * 2, 256) : 0;
+    d.parts_at = d.w_at + (d.copy_w ? up(N * d.kp * 2, 256) : 0);
     d.bytes = d.parts_at + (p.slices > 1 ? (int64_t)p.slices * M * N * 4 : 0);
     return d;
 }
@@ -291,22 +184,22 @@ extern "C" int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void*
     }
     const hipStream_t s = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
-    DenseOperand a = {static_cast<const uint16_t*>(x), x_row, (int)K}, b = {static_cast<const uint16_t*>(w), w_row, (int)K};
-    auto pack = [&](DenseOperand& o, int64_t row, int64_t col, int64_t R, int64_t at) {
+    auto operand = [&](const void* v, int64_t row, int64_t col, int64_t R, bool across, bool copy, int64_t at) {
+        const uint16_t* q = static_cast<const uint16_t*>(v);
+        if (!copy) return DenseOperand{q, across ? col : row, (int)K, (int)R, across};
         uint16_t* out = reinterpret_cast<uint16_t*>(ws + at);
         for (int64_t r = 0; r < R; r += 65535 * 64) {                        // (a grid's second dimension ends there)
             const int64_t n = std::min<int64_t>(R - r, 65535 * 64);
             dense_pack<<<dim3((uint32_t)(d.kp / 64), (uint32_t)((n + 63) / 64)), 256, 0, s>>>(
-                o.p + r * row, row, col, (int)n, (int)K, (int)d.kp, out + r * d.kp);
+                q + r * row, row, col, (int)n, (int)K, (int)d.kp, out + r * d.kp);
         }
-        o = {out, d.kp, (int)d.kp};
+        return DenseOperand{out, d.kp, (int)d.kp, (int)R, false};
     };
-    if (d.pack_x) pack(a, x_row, x_col, M, d.x_at);
-    if (d.pack_w) pack(b, w_row, w_col, N, d.w_at);
-    const DenseEpilogue e = {bias, gate, resid, bias_dt, gate_dt, act_of(act), gate ? rows_per_group : 1, resid_row, y, h};
+    const DenseOperand a = operand(x, x_row, x_col, M, d.across_x, d.copy_x, 0);
+    const DenseOperand b = operand(w, w_row, w_col, N, d.across_w, d.copy_w, d.w_at);
+    const DenseEpilogue e = {bias, gate, resid, bias_dt, gate_dt, act, gate ? rows_per_group : 1, resid_row, y, h};
     float* parts = reinterpret_cast<float*>(ws + d.parts_at);
-    if (dt == WF_BF16) dense_run<WF_BF16>(a, b, (int)M, (int)N, (int)K, p, parts, e, s);
-    else dense_run<WF_F16>(a, b, (int)M, (int)N, (int)K, p, parts, e, s);
+    dense_run(dt, a, b, (int)M, (int)N, (int)K, p, parts, e, s);
     WF_LAUNCH_CHECK("wf_dense launch");
     return WF_OK;
 }

@@ -16,7 +16,7 @@ namespace wf {
 // workgroup (512 columns, i, g) walks rows 4 i + wave, + 4 gridDim.y, ... of group g
 template <int D>
 __global__ __launch_bounds__(256) void dense_dact(const value_t<D>* __restrict__ dy, int64_t ldd,
-                                                  const value_t<D>* __restrict__ h, Act act, const void* gate, int gate_dt,
+                                                  const value_t<D>* __restrict__ h, int act, const void* gate, int gate_dt,
                                                   int64_t rows_per_group, value_t<D>* __restrict__ dh,
                                                   float* __restrict__ bparts, float* __restrict__ gparts, int N) {
     __shared__ float red[4][2][512];
@@ -33,14 +33,16 @@ __global__ __launch_bounds__(256) void dense_dact(const value_t<D>* __restrict__
         pd.load(dy + m * ldd + n, cnt);
         ph.zero();
         if (h) ph.load(h + m * N + n, cnt);
-        float v[8];
+        float v[8], x[8], a[8], slope[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = ph.get(i);
+        act_slope_run(act, x, a, slope);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float d = pd.get(i), x = ph.get(i);
-            v[i] = d * gv[i];
-            if (act.kind != ACT_NONE) v[i] *= act_slope(act, x);
+            const float d = pd.get(i);
+            v[i] = d * gv[i] * slope[i];
             sb[i] += v[i];
-            if (gparts) sg[i] += d * act_value(act, x);
+            sg[i] += d * a[i];
         }
         if (dh) {
             Pack<D> o;
@@ -120,7 +122,7 @@ extern "C" int wf_dense_grad(const void* dy, int64_t dy_row, const void* h, int 
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
         dense_dact<D><<<grid, 256, 0, s>>>(static_cast<const value_t<D>*>(dy), dy_row, static_cast<const value_t<D>*>(h),
-                                           act_of(act), gate, gate_dt, rows_per_group, static_cast<value_t<D>*>(dh), bparts,
+                                           act, gate, gate_dt, rows_per_group, static_cast<value_t<D>*>(dh), bparts,
                                            gparts, (int)N);
     };
     if (dt == WF_BF16) go(std::integral_constant<int, WF_BF16>{});

@@ -1,9 +1,15 @@
-// Main loop of the 16-bit linear's GEMM (dense.hip): C[BM x BN] += A[BM rows, K] . B[BN rows, K]^T through the two LDS
+// Main loop of the 16-bit linear's GEMM (dense_gemm.h): C[BM x BN] += A[BM rows, K] . B[BN rows, K]^T through the two LDS
 // stage buffers and the barrier discipline of wl_ring.h -- a stage is 64 values of K of every row, loaded global -> LDS;
 // stage p + 1 flies while stage p is computed; one barrier a stage, before its last K step's MFMAs, behind which the
 // loads of stage p + 2 and the first fragment reads of stage p + 1 go out between those MFMAs. What differs: each operand
-// has a row length of its own and the last stage may be short (its chunks past K load zeros), so strided rows and every
-// K that is a multiple of 8 need no copy; and each operand's loads are divided over the waves by themselves.
+// lies in memory one of two ways, with a row length of its own, and K need not be whole stages.
+//
+// Along K (DenseAlong): a row's K values are consecutive. A 1 KiB load covers 8 rows of a stage's 128 bytes; the chunks of
+// the last stage that lie past K load zeros. Across K (DenseAcross): value (r, k) is at k * row + r -- the operands of a
+// linear's backward products, which would otherwise have to be transposed through memory first. A stage is then 64 rows of
+// memory of B values each, and ds_read_b64_tr_b16 turns 4 (of K) x 16 (rows) blocks into the MFMA's fragments on the way
+// out of LDS. Rows of memory past K lie past the buffer's end and load zeros; chunks past the operand's last row hold
+// other values, which only reach outputs that are not stored.
 #pragma once
 
 #include "wl_ring.h"
@@ -11,6 +17,7 @@
 namespace wf {
 
 typedef float f32x16v __attribute__((ext_vector_type(16)));
+typedef short s16x4v __attribute__((ext_vector_type(4)));
 
 template <int VM_, int VN_, int WM_, int WN_>
 struct DenseShape {
@@ -23,42 +30,122 @@ struct DenseShape {
     static_assert(2 * SLOTS * 16 <= 160 * 1024, "two stage buffers fit the LDS");
 };
 
-// an operand's tile: a buffer over its rows from the tile's first, row bytes, and K in bytes
+// an operand's tile: the buffer from its first value on, bytes between rows (of the operand, or of memory where it lies
+// across K), and the bytes of K to load of a row (along K)
 struct DenseTile {
     __amdgpu_buffer_rsrc_t r;
     uint32_t row, k;
 };
 
-// acc[i][j] over the nk stages from stage s0. mma(acc, a, b) returns acc + a . b.
-template <typename S, typename Mma>
+// B rows of an operand, LW loads a wave and stage for NW waves, W fragments of 32 rows a wave from fragment t0 on
+template <int B, int NW, int LW, int W>
+struct DenseAlong {
+    __amdgpu_buffer_rsrc_t r;
+    uint32_t lane_at, tail, step;
+    int base, last;
+
+    // load q is number g = q NW + wave of the stage and covers rows 8 g .. 8 g + 7: lane l takes row 8 g + l / 8, chunk
+    // swz8(row, l % 8). NW is even, so g's parity, all that the swizzle sees of it, is the wave's.
+    __device__ __forceinline__ void init(const DenseTile& t, int lane, int wave, int t0) {
+        static_assert(NW % 2 == 0, "the swizzle goes by the wave's parity");
+        const int row = 8 * wave + lane / 8;
+        const uint32_t c = 16u * (uint32_t)swz8(row, lane % 8);
+        r = t.r;
+        lane_at = (uint32_t)row * t.row + c;
+        step = (uint32_t)(8 * NW) * t.row;
+        last = (int)((t.k - 1) / 128);
+        tail = (uint32_t)last * 128u + c < t.k ? lane_at : 0x80000000u;      // past every buffer's end: zeros
+        const int lr = lane & 31;
+        base = (t0 * 32 + lr) * 8 + swz8(lr, lane >> 5);          // (the swizzle depends on the row mod 16)
+    }
+    // before the loads of stage kt; the stages past the last are not read, whatever they hold
+    __device__ __forceinline__ void begin(int kt) {
+        if (kt >= last) lane_at = tail;
+    }
+    template <int Q>
+    __device__ __forceinline__ void load(wl_frag* st, int wave, int kt) const {
+        lds_dma16(r, st + 64 * (Q * NW + wave), lane_at + (Q * step + (uint32_t)kt * 128u));
+    }
+    template <int I>
+    __device__ __forceinline__ wl_frag read(const wl_frag* st, int ks) const {
+        return (st + (base ^ (2 * ks)))[I * 256];
+    }
+};
+
+template <int B, int NW, int LW, int W>
+struct DenseAcross {
+    // chunk c of memory row k of the stage sits at slot k CPR + (c ^ swz(k)): the four memory rows that a transposing read
+    // takes 32 bytes of each then lie in different quarters of the banks
+    static constexpr int CPR = B / 8;
+    static constexpr int FOLD = CPR % 16 == 0 ? 3 : CPR % 8 == 0 ? 2 : 0;
+    __device__ static constexpr int swz(int k) { return FOLD == 3 ? 2 * (k & 3) : FOLD == 2 ? k & 2 : 0; }
+    // loads in strides of NW keep one lane pattern where that is whole rows of memory; else each wave takes LW in a row
+    static constexpr bool STRIDED = 64 * NW % CPR == 0;
+    static constexpr int PATTERNS = STRIDED ? 1 : LW;
+    static_assert(STRIDED || 64 * LW % CPR == 0, "a wave's loads are whole rows of memory");
+
+    __amdgpu_buffer_rsrc_t r;
+    uint32_t lane_at[PATTERNS], step, stage;
+    int base[2];
+
+    __device__ __forceinline__ void init(const DenseTile& t, int lane, int wave, int t0) {
+        r = t.r;
+#pragma unroll
+        for (int q = 0; q < PATTERNS; q++) {
+            const int slot = 64 * (STRIDED ? wave : wave * LW + q) + lane, k = slot / CPR, c = slot % CPR;
+            lane_at[q] = (uint32_t)k * t.row + 16u * (uint32_t)(c ^ swz(k));
+        }
+        step = (uint32_t)(64 * NW / CPR) * t.row;
+        stage = 64u * t.row;
+        const int kr = 8 * (lane >> 5) + ((lane >> 2) & 3), c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        const int f = swz(kr), across = f & 4 ? 64 : 0;           // the swizzle's third bit exchanges neighbour fragments
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            base[i] = kr * CPR * 16 + (c ^ (f & 2)) * 16 + (lane & 1) * 8 + t0 * 64 + ((t0 + i) & 1 ? -across : across);
+    }
+    __device__ __forceinline__ void begin(int) {}
+    template <int Q>
+    __device__ __forceinline__ void load(wl_frag* st, int wave, int kt) const {
+        if constexpr (STRIDED) lds_dma16(r, st + 64 * (Q * NW + wave), lane_at[0] + (Q * step + (uint32_t)kt * stage));
+        else lds_dma16(r, st + 64 * (wave * LW + Q), lane_at[Q] + (uint32_t)kt * stage);
+    }
+    template <int I>
+    __device__ __forceinline__ wl_frag read(const wl_frag* st, int ks) const {
+        wl_frag v = {};
+#if defined(__HIP_DEVICE_COMPILE__)
+        typedef __attribute__((address_space(3))) const char* lds_bytes;
+        typedef __attribute__((address_space(3))) s16x4v* lds_quad;
+        lds_bytes p = (lds_bytes)(const char*)st + base[I & 1];
+        const s16x4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(p + (ks * 16) * CPR * 16 + I * 64));
+        const s16x4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(p + (ks * 16 + 4) * CPR * 16 + I * 64));
+        v = __builtin_bit_cast(wl_frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#endif
+        return v;
+    }
+};
+
+// acc[i][j] over the nk stages from stage s0. AX, BX: whether A and B lie across K. mma(acc, a, b) returns acc + a . b.
+template <typename S, bool AX, bool BX, typename Mma>
 __device__ __forceinline__ void dense_mainloop(const DenseTile& ta, const DenseTile& tb, int s0, int nk, int wave,
                                                int lane, wl_frag* sb0, wl_frag* sb1, f32x16v (&acc)[S::WM][S::WN],
                                                Mma&& mma) {
     constexpr int WM = S::WM, WN = S::WN, AW = S::AW, BW = S::BW, IPW = AW + BW;
     constexpr int READS = WM + WN, MFMAS = WM * WN;
-    const int wm = wave / S::VN, wn = wave % S::VN;
-    // load g of an operand covers its rows 8 g .. 8 g + 7; lane l takes row 8 g + l / 8, chunk swz8(row, l % 8), which is
-    // swz8(l / 8, l % 8) for even g and that ^ 4 for odd g
-    const uint32_t chunk = (uint32_t)swz8(lane / 8, lane % 8) * 16u;
-    const uint32_t la = (uint32_t)(lane / 8) * ta.row, lb = (uint32_t)(lane / 8) * tb.row;
+    std::conditional_t<AX, DenseAcross<S::BM, S::NW, AW, WM>, DenseAlong<S::BM, S::NW, AW, WM>> a;
+    std::conditional_t<BX, DenseAcross<S::BN, S::NW, BW, WN>, DenseAlong<S::BN, S::NW, BW, WN>> b;
+    a.init(ta, lane, wave, wave / S::VN * WM);
+    b.init(tb, lane, wave, wave % S::VN * WN);
     auto issue = [&](wl_frag* st, int kt, auto qc) {               // load q of this wave's IPW of stage kt
         constexpr int q = decltype(qc)::value;
-        constexpr bool A = q < AW;
-        const int g = A ? wave * AW + q : wave * BW + (q - AW);
-        const uint32_t c = chunk ^ ((g & 1) ? 64u : 0u), k0 = (uint32_t)kt * 128u, k = A ? ta.k : tb.k;
-        // (a chunk past K goes past every buffer's end: zeros; stages past the last load zeros too)
-        const uint32_t at = k0 + c < k ? (A ? la : lb) + (uint32_t)(8 * g) * (A ? ta.row : tb.row) + k0 + c : 0x80000000u;
-        lds_dma16(A ? ta.r : tb.r, st + (A ? 0 : S::ASLOTS) + 64 * g, at);
+        if constexpr (q < AW) a.template load<q>(st, wave, kt);
+        else b.template load<q - AW>(st + S::ASLOTS, wave, kt);
     };
-    const int lr = lane & 31, lk = lane >> 5;
-    const int arow = wm * WM * 32 + lr, brow = wn * WN * 32 + lr;
-    const int abase = arow * 8 + swz8(arow, lk), bbase = S::ASLOTS + brow * 8 + swz8(brow, lk);
     wl_frag fa[2][WM], fb[2][WN];
     auto fread = [&](const wl_frag* st, int ks, int set, auto rc) {    // read rc of a K step: a0, the b's, the other a's
         constexpr int r = decltype(rc)::value;
-        if constexpr (r == 0) fa[set][0] = st[abase ^ (2 * ks)];
-        else if constexpr (r <= WN) fb[set][r - 1] = (st + (bbase ^ (2 * ks)))[(r - 1) * 256];
-        else fa[set][r - WN] = (st + (abase ^ (2 * ks)))[(r - WN) * 256];
+        if constexpr (r == 0) fa[set][0] = a.template read<0>(st, ks);
+        else if constexpr (r <= WN) fb[set][r - 1] = b.template read<r - 1>(st + S::ASLOTS, ks);
+        else fa[set][r - WN] = a.template read<r - WN>(st, ks);
     };
     auto kstep = [&](auto load, int set, const wl_frag* st, int ks, wl_frag* free_, int kt) {
         static_for<MFMAS>([&](auto mc) {
@@ -77,7 +164,13 @@ __device__ __forceinline__ void dense_mainloop(const DenseTile& ta, const DenseT
             __builtin_amdgcn_sched_barrier(0);
         });
     };
+    auto begin = [&](int kt) {
+        a.begin(kt);
+        b.begin(kt);
+    };
+    begin(s0);
     static_for<IPW>([&](auto q) { issue(sb0, s0, q); });
+    begin(s0 + 1);
     static_for<IPW>([&](auto q) { issue(sb1, s0 + 1, q); });
     wait_vm<IPW>();                                      // the first stage landed; the second may be in flight
     wave_barrier_sync();
@@ -86,6 +179,7 @@ __device__ __forceinline__ void dense_mainloop(const DenseTile& ta, const DenseT
         kstep(std::false_type{}, 0, cur, 1, nullptr, 0);
         kstep(std::false_type{}, 1, cur, 2, nullptr, 0);
         kstep(std::false_type{}, 0, cur, 3, nullptr, 0);
+        begin(p + 2);
         wait_vm<0>();                                    // stage p + 1 landed (this wave's loads)
         __builtin_amdgcn_s_waitcnt(0xc07f);              // lgkmcnt(0): this wave's reads of cur are done
         wave_barrier_sync();                             // ... and every wave's: cur is free, p + 1 is whole
