@@ -96,19 +96,28 @@ struct DenseEpilogue {
     void *y, *h;                           // [M, N]; h (may be NULL): the pre-activations
 };
 
-// the residual's run at (m, n), its first `cnt` values
+// what a run at (m, n) of `cnt` values (8, or fewer at a row's end) needs from memory
 template <int D>
-__device__ __forceinline__ Pack<D> epilogue_prefetch(const DenseEpilogue& e, int64_t m, int n, int cnt) {
-    Pack<D> r;
-    r.zero();
-    if (e.resid && cnt > 0) r.load(static_cast<const value_t<D>*>(e.resid) + m * e.ldr + n, cnt);
-    return r;
+struct EpilogueAhead {
+    Pack<D> resid;
+    float gate[8];
+};
+template <int D>
+__device__ __forceinline__ EpilogueAhead<D> epilogue_ahead(const DenseEpilogue& e, int64_t m, int n, int N, int cnt) {
+    EpilogueAhead<D> a;
+    a.resid.zero();
+    if (e.resid && cnt > 0) a.resid.load(static_cast<const value_t<D>*>(e.resid) + m * e.ldr + n, cnt);
+    if (e.gate && cnt > 0) {
+        const int64_t at = (int64_t)((uint32_t)m / (uint32_t)e.rows_per_group) * N + n;
+        load_params<8>(a.gate, e.gate, at, cnt, e.gate_dt);
+    }
+    return a;
 }
 
 // v: a run's sums, without the bias when BIAS is set
 template <int D, bool BIAS>
-__device__ __forceinline__ void epilogue_run(const DenseEpilogue& e, float (&v)[8], const Pack<D>& r, int64_t m, int n,
-                                             int N, int cnt) {
+__device__ __forceinline__ void epilogue_run(const DenseEpilogue& e, float (&v)[8], const EpilogueAhead<D>& a, int64_t m,
+                                             int n, int N, int cnt) {
     float u[8];
     if (BIAS && e.bias) {
         load_params<8>(u, e.bias, n, cnt, e.bias_dt);
@@ -123,14 +132,12 @@ __device__ __forceinline__ void epilogue_run(const DenseEpilogue& e, float (&v)[
         o.store(static_cast<value_t<D>*>(e.h) + m * N + n, cnt);
     }
     act_run(e.act, v);
-    if (e.gate) {
-        load_params<8>(u, e.gate, (int64_t)((uint32_t)m / (uint32_t)e.rows_per_group) * N + n, cnt, e.gate_dt);
+    if (e.gate)
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= u[i];
-    }
+        for (int i = 0; i < 8; i++) v[i] *= a.gate[i];
     if (e.resid)
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] += r.get(i);
+        for (int i = 0; i < 8; i++) v[i] += a.resid.get(i);
     Pack<D> o;
     o.put(v);
     o.store(static_cast<value_t<D>*>(e.y) + m * N + n, cnt);

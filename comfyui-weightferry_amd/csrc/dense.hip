@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void dense_sum(const float* __restrict__ parts
     if (i >= (int64_t)M * runs) return;
     const int64_t m = i / runs;
     const int n = (int)(i - m * runs) * 8, cnt = N - n;
-    const Pack<D> r = epilogue_prefetch<D>(e, m, n, cnt);
+    const EpilogueAhead<D> r = epilogue_ahead<D>(e, m, n, N, cnt);
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int s = 0; s < slices; s++) {
         const float* p = parts + ((int64_t)s * M + m) * N + n;

@@ -70,39 +70,45 @@ __global__ __launch_bounds__(S::NT) void dense_gemm(DenseOperand a, DenseOperand
     static_assert(2 * PER_BUF >= S::NW, "the output rows fit in the stage buffers");
     float* ot = reinterpret_cast<float*>(wave < PER_BUF ? sb0 : sb1) + (wave % PER_BUF) * 16 * TC;
     constexpr int RUNS = TC / 8;
+    // (the loop over runs stays a loop: unrolled, the epilogue's code took longer to fetch than to run. What a run needs
+    // from memory is loaded one run ahead.)
+    auto at_run = [&](int mi, int it, auto&& f) {
+        const int q = it * 64 + lane, m = mi + q / RUNS, n = nw + 8 * (q % RUNS);
+        return f(q, m, n, m < M ? N - n : 0);
+    };
 #pragma unroll
     for (int half = 0; half < 2 * WM; half++) {
         const int mi = mw + half * 16;
         if (mi >= M) break;
-        Pack<D> res[WN];
-        if (!parts) {
-#pragma unroll
-            for (int it = 0; it < WN; it++) {
-                const int q = it * 64 + lane, m = mi + q / RUNS, n = nw + 8 * (q % RUNS);
-                res[it] = epilogue_prefetch<D>(e, m, n, m < M ? N - n : 0);
-            }
-        }
+        auto ahead = [&](int it) {
+            return at_run(mi, it, [&](int, int m, int n, int cnt) { return epilogue_ahead<D>(e, m, n, N, cnt); });
+        };
+        EpilogueAhead<D> next;
+        if (!parts) next = ahead(0);
 #pragma unroll
         for (int x = 0; x < 8; x++)
 #pragma unroll
             for (int j = 0; j < WN; j++)
                 ot[(8 * (x >> 2) + 4 * lk + (x & 3)) * TC + j * 32 + lr] = acc[half / 2][j][8 * (half & 1) + x];
-#pragma unroll
+#pragma unroll 1
         for (int it = 0; it < WN; it++) {
-            const int q = it * 64 + lane, m = mi + q / RUNS, n = nw + 8 * (q % RUNS);
-            const float4 lo = reinterpret_cast<const float4*>(ot)[2 * q], hi = reinterpret_cast<const float4*>(ot)[2 * q + 1];
-            if (m >= M || n >= N) continue;
-            float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-            if (parts) {
+            const EpilogueAhead<D> now = next;
+            if (!parts && it + 1 < WN) next = ahead(it + 1);
+            at_run(mi, it, [&](int q, int m, int n, int cnt) {
+                const float4 lo = reinterpret_cast<const float4*>(ot)[2 * q], hi = reinterpret_cast<const float4*>(ot)[2 * q + 1];
+                float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                if (cnt <= 0) return;
+                if (!parts) {
+                    epilogue_run<D, false>(e, v, now, m, n, N, cnt);
+                    return;
+                }
                 float* o = parts + ((int64_t)blockIdx.y * M + m) * N + n;
-                if (n + 8 <= N) __builtin_memcpy(o, v, 32);
+                if (cnt >= 8) __builtin_memcpy(o, v, 32);
                 else
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        if (n + i < N) o[i] = v[i];
-            } else {
-                epilogue_run<D, false>(e, v, res[it], m, n, N, N - n);
-            }
+                        if (i < cnt) o[i] = v[i];
+            });
         }
     }
 }
