@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "dense_gemm.h"
+#include "dense_rows.h"
 
 namespace wf {
 
@@ -28,22 +29,43 @@ __global__ __launch_bounds__(256) void dense_sum(const float* __restrict__ parts
     const int n = (int)(i - m * runs) * 8, cnt = N - n;
     const EpilogueAhead<D> r = epilogue_ahead<D>(e, m, n, N, cnt);
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int s = 0; s < slices; s++) {
-        const float* p = parts + ((int64_t)s * M + m) * N + n;
-        float u[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (cnt >= 8) __builtin_memcpy(u, p, 32);
-        else
+    const float* p = parts + m * N + n;
+    const int64_t plane = (int64_t)M * N;
+    for (int s = 0; s < slices; s += 4) {                          // four slices' loads in flight, added in order
+        float u[4][8];
 #pragma unroll
-            for (int x = 0; x < 8; x++)
-                if (x < cnt) u[x] = p[x];
+        for (int i = 0; i < 4; i++) {
+            const int64_t at = min(s + i, slices - 1) * plane;
+            if (cnt >= 8) __builtin_memcpy(u[i], p + at, 32);
+            else
 #pragma unroll
-        for (int x = 0; x < 8; x++) v[x] += u[x];
+                for (int x = 0; x < 8; x++) u[i][x] = x < cnt ? p[at + x] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (s + i < slices)
+#pragma unroll
+                for (int x = 0; x < 8; x++) v[x] += u[i][x];
     }
     epilogue_run<D, true>(e, v, r, m, n, N, cnt);
 }
 
-// rows of a strided operand (values row apart along its rows, col apart along K) as [R, KP] rows of whole stages, zeros
-// past K: 64 x 64 tiles through LDS, read along whichever of the two is the shorter step
+// rows of an operand whose values lie one after another along K, as [R, KP] rows of whole stages, zeros past K: a run of 8
+// values a thread, loaded at any alignment
+__global__ __launch_bounds__(256) void dense_pack_rows(const uint16_t* __restrict__ p, int64_t row, int R, int K, int KP,
+                                                       uint16_t* __restrict__ out) {
+    const int runs = KP / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / runs;
+    if (r >= R) return;
+    const int k = (int)(i - r * runs) * 8;
+    Pack<WF_BF16> v;                                               // (16 bits are moved, whatever they stand for)
+    v.zero();
+    if (k < K) v.load(p + r * row + k, K - k);
+    v.store(out + r * KP + k, 8);
+}
+
+// the same for any strides (values row apart along its rows, col apart along K): 64 x 64 tiles through LDS, read along
+// whichever of the two is the shorter step
 __global__ __launch_bounds__(256) void dense_pack(const uint16_t* __restrict__ p, int64_t row, int64_t col, int R, int K,
                                                   int KP, uint16_t* __restrict__ out) {
     __shared__ uint16_t t[64][66];
@@ -62,71 +84,152 @@ __global__ __launch_bounds__(256) void dense_pack(const uint16_t* __restrict__ p
 }
 
 // ------------------------------------------------------------------------------------------------- host side
-// the tilings, each with its outputs per modelled time (per mille of the largest's)
+// The modelled time of a product in us, fitted to 2,240 measurements (30 shapes of 20-16384 rows, 64-13824 columns and K
+// 256-16384, every tiling, 1-16 slices, both orders of the operands; typically 5-10 % off): a workgroup takes `fixed` and
+// `stage` for each 64 values of K on a CU of its own, `shared` where `per_cu` of them share one; operands stream at 5 TB/s,
+// less with few workgroups; a second kernel adds the slices. Choosing by it stays within 5 % of the best measured way on
+// 21 of the shapes and within 13 % on all but one (600 x 800 x 13000: 61 against 46 us).
 struct DenseTiling {
-    int bm, bn, eff;
+    int bm, bn, per_cu;
+    float fixed, stage, shared;
 };
-constexpr DenseTiling kDense[] = {{256, 320, 1000}, {256, 256, 900}, {256, 192, 820}, {256, 128, 700},
-                                  {128, 160, 650},  {128, 128, 560}, {64, 128, 380},  {32, 128, 220}};
-constexpr int kDenseTilings = sizeof(kDense) / sizeof(kDense[0]);
+constexpr DenseTiling kDense[] = {{256, 320, 1, 6.36f, 1.443f, 1.443f}, {256, 256, 1, 3.72f, 1.281f, 1.281f},
+                                  {256, 192, 1, 3.12f, 1.124f, 1.124f}, {128, 160, 2, 4.02f, 0.722f, 0.582f},
+                                  {128, 128, 2, 2.66f, 0.647f, 0.511f}, {64, 128, 3, 1.77f, 0.499f, 0.376f},
+                                  {32, 128, 3, 2.06f, 0.428f, 0.326f}};
+constexpr float kDenseLaunch = 4.7f;
 
-static DensePlan dense_plan(int64_t M, int64_t N, int64_t K) {
+static DensePlan dense_plan_tiles(int64_t M, int64_t N, int64_t K, float& us) {
     const int64_t stages = (K + 63) / 64;
     DensePlan best = {0, 1, (int)stages};
-    double least = 1e300;
-    for (int t = 0; t < kDenseTilings; t++) {
-        const int64_t tiles = ((M + kDense[t].bm - 1) / kDense[t].bm) * ((N + kDense[t].bn - 1) / kDense[t].bn);
-        const double stage = (double)kDense[t].bm * kDense[t].bn / kDense[t].eff;
-        for (int64_t s = 1; s <= 16 && s <= stages; s++) {
-            const int64_t per = (stages + s - 1) / s, slices = (stages + per - 1) / per;
-            if (slices != s || (s > 1 && (per < 8 || tiles * s > 1024))) continue;
-            const int64_t rounds = (tiles * s + 255) / 256;
-            double c = (double)rounds * stage * (per + 8);
-            if (s > 1) c += 1200 + (double)M * N * (s + 1) * 0.0006;
-            if (c < least) least = c, best = {t, (int)s, (int)per};
+    us = 1e30f;
+    const float bytes = (float)(M * K + N * K) * 2.0f;
+    for (int t = 0; t < (int)(sizeof(kDense) / sizeof(kDense[0])); t++) {
+        const DenseTiling& q = kDense[t];
+        const int64_t tiles = ((M + q.bm - 1) / q.bm) * ((N + q.bn - 1) / q.bn);
+        for (int want : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            const int64_t per = (stages + want - 1) / want, slices = (stages + per - 1) / per;
+            if (want > 1 && (slices != want || per < 3 || tiles * slices > 1600)) continue;
+            // workgroups of the busiest CU: full rounds of per_cu together, then a rest
+            const int64_t wgs = tiles * slices, on = (wgs + 255) / 256, full = on / q.per_cu;
+            const int rest = (int)(on % q.per_cu);
+            auto together = [&](int n) {
+                if (n == 0) return 0.0f;
+                const float more = q.per_cu > 1 ? (q.shared * q.per_cu - q.stage) * (n - 1) / (q.per_cu - 1) : 0.0f;
+                return q.fixed + (float)per * (q.stage + more);
+            };
+            const float busy = (float)full * together(q.per_cu) + together(rest);
+            const float mem = bytes / 5.0e6f * (1.0f + 0.232f * 256.0f / (float)wgs);
+            const float hi = std::max(busy, mem), r = std::min(busy, mem) / hi;
+            float c = kDenseLaunch + hi * (1.0f + 0.26f * r * r * r);
+            if (want > 1) c += 1.64e-6f * (float)(M * N) * (float)(slices + 1);
+            if (c < us) us = c, best = {t, (int)slices, (int)per};
         }
     }
     return best;
 }
 
-static void dense_run(int dt, const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p,
-                      float* parts, const DenseEpilogue& e, hipStream_t s) {
-    (a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : dense_gemm_along)(dt, a, b, M, N, K, p, parts, e, s);
-    if (p.slices > 1) {
-        const int64_t runs = (int64_t)M * ((N + 7) / 8);
-        const dim3 grid((uint32_t)((runs + 255) / 256));
-        if (dt == WF_BF16) dense_sum<WF_BF16><<<grid, 256, 0, s>>>(parts, p.slices, M, N, e);
-        else dense_sum<WF_F16><<<grid, 256, 0, s>>>(parts, p.slices, M, N, e);
-    }
+// The few-rows form: weight bytes at 5.2 TB/s, up to 1.4 times that time as 16 rows fill up, more with every 16 rows.
+// 1 x 13824 x 5120 30 us, 16 x 13824 x 5120 42 (the tiles 35), 16 x 2048 x 8192 12 (19), 32 x 2048 x 2048 5.9 (8.9).
+static float dense_rows_time(int64_t M, int64_t N, int64_t K) {
+    const float fill = 1.0f + 0.4f * (float)std::min<int64_t>(M - 1, 15) / 15.0f;
+    const int64_t groups = (M + 15) / 16;
+    return 4.0f + (float)(N * K) * 2.0f / 5.2e6f * fill * (groups > 1 ? 0.87f * (float)groups : 1.0f);
 }
-
-// whether an operand can be loaded as it is, along K or across it: 16-byte runs, offsets inside 31 bits
-static bool dense_along(const void* p, int64_t row, int64_t col, int64_t K) {
-    return col == 1 && row % 8 == 0 && K % 8 == 0 && row >= K && row <= (1 << 20) && aligned(p, 16);
-}
-static bool dense_across(const void* p, int64_t row, int64_t col, int64_t R, int64_t K) {
-    return row == 1 && col % 8 == 0 && col >= R && aligned(p, 16) && (K + 128) * col * 2 < (1LL << 31);
+// Two weight tiles a workgroup share x's loads (16 x 5120 x 5120 20 against 25 us) where that leaves 128 workgroups; a
+// single or double row of a wide weight has little of x to share (1 x 13824 x 5120 30.5 against 32.3). A long K of a narrow
+// weight is split over four workgroups (16 x 2048 x 8192 12 against 17).
+static DenseRowsPlan dense_plan_rows(int64_t M, int64_t N, int64_t K) {
+    const int64_t pairs = (N + 31) / 32 * ((M + 15) / 16);
+    if (pairs >= 128) return {M <= 2 && pairs >= 256 ? 1 : 2, 1};
+    return K >= 4096 ? DenseRowsPlan{2, 4} : DenseRowsPlan{1, 1};
 }
 
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-struct DenseNeeds {
+struct DenseView {                                    // value (r, k) at r * row + k * col
+    const void* p;
+    int64_t row, col;
+};
+
+constexpr int64_t kRowsMost = 64;
+
+// How a call runs: in the few-rows form, or in tiles with its operands loaded along K, across it, or from a copy.
+struct DenseCall {
+    bool few;
+    DenseRowsPlan rows;
+    DensePlan tiles;
     bool across_x, across_w, copy_x, copy_w;
     int64_t kp, w_at, parts_at, bytes;                // a copy's row; offsets into the workspace, x's copy first
+    int slices() const { return few ? rows.slices : tiles.slices; }
 };
-static DenseNeeds dense_needs(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col,
-                              int64_t M, int64_t N, int64_t K, const DensePlan& p) {
-    DenseNeeds d;
-    const bool along_x = dense_along(x, x_row, x_col, K), along_w = dense_along(w, w_row, w_col, K);
-    d.across_w = !along_w && dense_across(w, w_row, w_col, N, K);
-    d.across_x = !along_x && d.across_w && dense_across(x, x_row, x_col, M, K);   // (x across and w along: x is copied)
+
+// whether an operand can be loaded as it is, along K or across it: 16-byte runs, offsets inside 31 bits
+static bool dense_along(const DenseView& v, int64_t K) {
+    return v.col == 1 && v.row % 8 == 0 && K % 8 == 0 && v.row >= K && v.row <= (1 << 20) && aligned(v.p, 16);
+}
+static bool dense_across(const DenseView& v, int64_t R, int64_t K) {
+    return v.row == 1 && v.col % 8 == 0 && v.col >= R && aligned(v.p, 16) && (K + 128) * v.col * 2 < (1LL << 31);
+}
+
+static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, int64_t N, int64_t K) {
+    DenseCall d = {};
+    float us;
+    d.tiles = dense_plan_tiles(M, N, K, us);
+    const bool along_x = dense_along(x, K), along_w = dense_along(w, K);
+    d.across_w = !along_w && dense_across(w, N, K);
+    d.across_x = !along_x && d.across_w && dense_across(x, M, K);                 // (x across and w along: x is copied)
     d.copy_x = !along_x && !d.across_x;
     d.copy_w = !along_w && !d.across_w;
+    if (d.copy_x) us += 3.0f + (float)(M * K) * 1e-6f;                            // (a copy: 4 bytes a value at 4 TB/s)
+    if (d.copy_w) us += 3.0f + (float)(N * K) * 1e-6f;
+    if (M <= kRowsMost && x.col == 1 && w.col == 1 && dense_rows_time(M, N, K) < us) {
+        d.few = true;
+        d.copy_x = d.copy_w = false;
+        d.rows = dense_plan_rows(M, N, K);
+    }
     d.kp = up(K, 64);
     d.w_at = d.copy_x ? up(M * d.kp * 2, 256) : 0;
     d.parts_at = d.w_at + (d.copy_w ? up(N * d.kp * 2, 256) : 0);
-    d.bytes = d.parts_at + (p.slices > 1 ? (int64_t)p.slices * M * N * 4 : 0);
+    d.bytes = d.parts_at + (d.slices() > 1 ? (int64_t)d.slices() * M * N * 4 : 0);
     return d;
+}
+
+static void dense_copy(const DenseView& v, int64_t R, int64_t K, int64_t kp, uint16_t* out, hipStream_t s) {
+    const uint16_t* p = static_cast<const uint16_t*>(v.p);
+    if (v.col == 1) {
+        dense_pack_rows<<<dim3((uint32_t)((R * (kp / 8) + 255) / 256)), 256, 0, s>>>(p, v.row, (int)R, (int)K, (int)kp, out);
+        return;
+    }
+    for (int64_t r = 0; r < R; r += 65535 * 64) {                                 // (a grid's second dimension ends there)
+        const int64_t n = std::min<int64_t>(R - r, 65535 * 64);
+        dense_pack<<<dim3((uint32_t)(kp / 64), (uint32_t)((n + 63) / 64)), 256, 0, s>>>(p + r * v.row, v.row, v.col, (int)n,
+                                                                                       (int)K, (int)kp, out + r * kp);
+    }
+}
+
+static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w, int dt, int64_t M, int64_t N, int64_t K,
+                      char* ws, const DenseEpilogue& e, hipStream_t s) {
+    float* parts = reinterpret_cast<float*>(ws + d.parts_at);
+    if (d.few) {
+        dense_rows_run(dt, d.rows, static_cast<const uint16_t*>(x.p), x.row, static_cast<const uint16_t*>(w.p), w.row, (int)M,
+                       (int)N, (int)K, parts, e, s);
+    } else {
+        auto operand = [&](const DenseView& v, int64_t R, bool across, bool copy, int64_t at) {
+            if (!copy) return DenseOperand{static_cast<const uint16_t*>(v.p), across ? v.col : v.row, (int)K, (int)R, across};
+            uint16_t* out = reinterpret_cast<uint16_t*>(ws + at);
+            dense_copy(v, R, K, d.kp, out, s);
+            return DenseOperand{out, d.kp, (int)d.kp, (int)R, false};
+        };
+        const DenseOperand a = operand(x, M, d.across_x, d.copy_x, 0), b = operand(w, N, d.across_w, d.copy_w, d.w_at);
+        (a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : dense_gemm_along)(dt, a, b, (int)M, (int)N, (int)K, d.tiles,
+                                                                                parts, e, s);
+    }
+    if (d.slices() > 1) {
+        const dim3 grid((uint32_t)((M * ((N + 7) / 8) + 255) / 256));
+        if (dt == WF_BF16) dense_sum<WF_BF16><<<grid, 256, 0, s>>>(parts, d.slices(), (int)M, (int)N, e);
+        else dense_sum<WF_F16><<<grid, 256, 0, s>>>(parts, d.slices(), (int)M, (int)N, e);
+    }
 }
 
 static int dense_check(const char* who, int dt, int64_t M, int64_t N, int64_t K, int64_t x_row, int64_t x_col,
@@ -153,7 +256,7 @@ extern "C" int wf_dense_workspace(const void* x, int64_t x_row, int64_t x_col, c
     using namespace wf;
     if (!bytes) { set_error("wf_dense_workspace: null pointer"); return WF_EINVAL; }
     if (const int rc = dense_check("wf_dense_workspace", dt, M, N, K, x_row, x_col, w_row, w_col)) return rc;
-    *bytes = M && N ? dense_needs(x, x_row, x_col, w, w_row, w_col, M, N, K, dense_plan(M, N, K)).bytes : 0;
+    *bytes = M && N ? dense_call({x, x_row, x_col}, {w, w_row, w_col}, M, N, K).bytes : 0;
     return WF_OK;
 }
 
@@ -176,30 +279,14 @@ extern "C" int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void*
         set_error("wf_dense: a pointer is not aligned to its values");
         return WF_EINVAL;
     }
-    const DensePlan p = dense_plan(M, N, K);
-    const DenseNeeds d = dense_needs(x, x_row, x_col, w, w_row, w_col, M, N, K, p);
+    const DenseView xv = {x, x_row, x_col}, wv = {w, w_row, w_col};
+    const DenseCall d = dense_call(xv, wv, M, N, K);
     if (d.bytes && (!workspace || workspace_bytes < d.bytes || !aligned(workspace, 256))) {
         set_error("wf_dense: a workspace of %lld bytes is required", (long long)d.bytes);
         return WF_EINVAL;
     }
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    char* ws = static_cast<char*>(workspace);
-    auto operand = [&](const void* v, int64_t row, int64_t col, int64_t R, bool across, bool copy, int64_t at) {
-        const uint16_t* q = static_cast<const uint16_t*>(v);
-        if (!copy) return DenseOperand{q, across ? col : row, (int)K, (int)R, across};
-        uint16_t* out = reinterpret_cast<uint16_t*>(ws + at);
-        for (int64_t r = 0; r < R; r += 65535 * 64) {                        // (a grid's second dimension ends there)
-            const int64_t n = std::min<int64_t>(R - r, 65535 * 64);
-            dense_pack<<<dim3((uint32_t)(d.kp / 64), (uint32_t)((n + 63) / 64)), 256, 0, s>>>(
-                q + r * row, row, col, (int)n, (int)K, (int)d.kp, out + r * d.kp);
-        }
-        return DenseOperand{out, d.kp, (int)d.kp, (int)R, false};
-    };
-    const DenseOperand a = operand(x, x_row, x_col, M, d.across_x, d.copy_x, 0);
-    const DenseOperand b = operand(w, w_row, w_col, N, d.across_w, d.copy_w, d.w_at);
     const DenseEpilogue e = {bias, gate, resid, bias_dt, gate_dt, act, gate ? rows_per_group : 1, resid_row, y, h};
-    float* parts = reinterpret_cast<float*>(ws + d.parts_at);
-    dense_run(dt, a, b, (int)M, (int)N, (int)K, p, parts, e, s);
+    dense_run(d, xv, wv, dt, M, N, K, static_cast<char*>(workspace), e, static_cast<hipStream_t>(stream));
     WF_LAUNCH_CHECK("wf_dense launch");
     return WF_OK;
 }

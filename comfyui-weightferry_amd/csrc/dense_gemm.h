@@ -134,10 +134,9 @@ static void dense_tiling(const DenseOperand& a, const DenseOperand& b, int M, in
     case 0: dense_launch<D, AX, BX, 4, 2, 2, 5>(a, b, M, N, K, p, parts, e, s); break;
     case 1: dense_launch<D, AX, BX, 2, 4, 4, 2>(a, b, M, N, K, p, parts, e, s); break;
     case 2: dense_launch<D, AX, BX, 4, 2, 2, 3>(a, b, M, N, K, p, parts, e, s); break;
-    case 3: dense_launch<D, AX, BX, 2, 2, 4, 2>(a, b, M, N, K, p, parts, e, s); break;
-    case 4: dense_launch<D, AX, BX, 4, 1, 1, 5>(a, b, M, N, K, p, parts, e, s); break;
-    case 5: dense_launch<D, AX, BX, 2, 2, 2, 2>(a, b, M, N, K, p, parts, e, s); break;
-    case 6: dense_launch<D, AX, BX, 1, 4, 2, 1>(a, b, M, N, K, p, parts, e, s); break;
+    case 3: dense_launch<D, AX, BX, 4, 1, 1, 5>(a, b, M, N, K, p, parts, e, s); break;
+    case 4: dense_launch<D, AX, BX, 2, 2, 2, 2>(a, b, M, N, K, p, parts, e, s); break;
+    case 5: dense_launch<D, AX, BX, 1, 4, 2, 1>(a, b, M, N, K, p, parts, e, s); break;
     default: dense_launch<D, AX, BX, 1, 4, 1, 1>(a, b, M, N, K, p, parts, e, s); break;
     }
 }
