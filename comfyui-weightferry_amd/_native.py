@@ -49,7 +49,7 @@ EXPORTS = {
     "wf_linear_gguf_ws": (_int, [_p, _i64, _i64, _p, _i64, _int, _i64, _p, _p, _int, _p, _i64, _p]),
     "wf_linear_gguf_noalloc": (_int, [_p, _i64, _i64, _p, _i64, _int, _i64, _p, _p, _int, _p]),
     "wf_layer_norm": (_int, [_p, _i64, _int, _p, _p, _int, _int, _i64, ctypes.c_float, _p, _p, _i64, _i64, _p]),
-    "wf_layer_norm_bwd_workspace": (_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "wf_layer_norm_bwd_workspace": (_int, [_i64, _i64, _i64, _int, ctypes.POINTER(_i64)]),
     "wf_layer_norm_bwd": (_int, [_p, _i64, _p, _i64, _int, _p, _int, _int, _i64, _p, _p, _p, _p, _i64, _i64, _p, _i64,
                                  _p]),
     "wf_dense_workspace": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, ctypes.POINTER(_i64)]),

@@ -21,6 +21,7 @@ static __global__ __launch_bounds__(1024) void column_sums(ColumnSums a, ColumnS
     const int64_t g = blockIdx.y;
     float s = 0.0f;
     if (col < K)
+#pragma unroll 8                                              // (the loads go out together; the order of the sum stays)
         for (int i = wave; i < q.n; i += 16) s += q.parts[(g * q.n + i) * K + col];
     red[wave][lane] = s;
     __syncthreads();

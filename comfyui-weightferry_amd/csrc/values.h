@@ -75,6 +75,12 @@ struct Pack {
             }
         }
     }
+    // the same past the caches' ordinary replacement, for outputs that no launch reads back at once
+    __device__ __forceinline__ void store_streamed(value_t<D>* p, int n) const {
+        typedef uint32_t quad __attribute__((ext_vector_type(4), aligned(2)));
+        if (n >= VEC) __builtin_nontemporal_store((quad){w[0], w[1], w[2], w[3]}, reinterpret_cast<quad*>(p));
+        else store(p, n);
+    }
     __device__ __forceinline__ void store(value_t<D>* p, int n) const {
         if (n >= VEC) {
             __builtin_memcpy(p, w, 16);

@@ -62,7 +62,7 @@ class _LayerNorm(torch.autograd.Function):
             ws = None
             if need_w or need_b:
                 need = ctypes.c_int64()
-                _native.call("wf_layer_norm_bwd_workspace", rows, width, rows // ctx.groups, ctypes.byref(need))
+                _native.call("wf_layer_norm_bwd_workspace", rows, width, rows // ctx.groups, ctx.code, ctypes.byref(need))
                 ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
             with _native.on_device(dev):
                 _native.call("wf_layer_norm_bwd", x2.data_ptr(), x2.stride(0), d2.data_ptr(), d2.stride(0), ctx.code,

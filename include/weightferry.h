@@ -185,7 +185,7 @@ int wf_layer_norm(const void* x, int64_t ldx, int dt, const void* w, const void*
 /* Its gradients: dx [M, K] of type dt, dw and db [M / rows_per_group, K] of type param_dt; any of the three may be NULL.
  * dy: M rows ldd values apart. The workspace (needed for dw and db: the bytes that wf_layer_norm_bwd_workspace gives, 4-byte
  * aligned) holds partial sums; they are added in a fixed order, so the results are the same on every run. */
-int wf_layer_norm_bwd_workspace(int64_t M, int64_t K, int64_t rows_per_group, int64_t* bytes);
+int wf_layer_norm_bwd_workspace(int64_t M, int64_t K, int64_t rows_per_group, int dt, int64_t* bytes);
 int wf_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldd, int dt, const void* w, int param_dt,
                       int plus_one, int64_t rows_per_group, const float* stats, void* dx, void* dw, void* db, int64_t M,
                       int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
