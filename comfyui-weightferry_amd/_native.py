@@ -55,8 +55,10 @@ EXPORTS = {
     "wf_dense_workspace": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, ctypes.POINTER(_i64)]),
     "wf_dense": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _p, _int, _int, _p, _int, _i64, _p, _i64,
                         _p, _p, _p, _i64, _p]),
-    "wf_dense_grad_workspace": (_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
-    "wf_dense_grad": (_int, [_p, _i64, _p, _int, _int, _p, _int, _i64, _p, _p, _int, _p, _i64, _i64, _p, _i64, _p]),
+    "wf_dense_bwd_workspace": (_int, [_p, _i64, _p, _i64, _i64, _p, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _int,
+                                      _int, _int, ctypes.POINTER(_i64)]),
+    "wf_dense_bwd": (_int, [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _int, _int, _p, _int, _i64, _i64, _i64, _i64, _p, _p,
+                            _p, _int, _p, _p, _i64, _p]),
     "wf_adamw": (_int, [_p, _i64, _int, _int, _p, _p, _p, _p, _i64, _i64] + [ctypes.c_double] * 5 + [_p]),
     "wf_adamw_values": (_int, [_p, _p, _p, _p, _i64, _p, _p, _p]),
     "wf_host_alloc": (_int, [_sz, ctypes.POINTER(ctypes.c_void_p)]),
@@ -150,11 +152,16 @@ def check(rc, what):
     raise NativeError(f"{what} failed ({rc}): {last_error()}")
 
 
+def must(rc, what):
+    """Raises NativeError for a return code that is not WF_OK."""
+    if rc != OK:
+        raise NativeError(f"{what} failed ({rc}): {last_error()}")
+
+
 def call(fn_name, *args):
     """lib().<fn_name>(*args), raising NativeError on any non-zero return."""
     rc = getattr(lib(), fn_name)(*args)
-    if rc != OK:
-        raise NativeError(f"{fn_name} failed ({rc}): {last_error()}")
+    must(rc, fn_name)
     return rc
 
 

@@ -4,7 +4,7 @@
 // 2 M N K operations: v_mfma_f32_32x32x16 tiles fed through the two-buffer LDS ring of dense_ring.h. A product with too
 // few tiles to fill the 256 CUs runs as slices of K that write float32 partial sums; a second kernel adds them in slice
 // order and runs the epilogue. Operands whose rows are not 16-byte runs along K (odd widths, transposed views) are first
-// copied into rows of whole 128-byte stages.
+// copied into rows that are.
 //
 // The epilogue works on runs of 8 outputs of a row: the accumulators (16 rows x 1 column a lane) pass through the idle
 // stage buffers in float32, so bias, activation, gate and residual are computed on the unrounded sums and every global
@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "dense_gemm.h"
+#include "dense_grad.h"
 #include "dense_rows.h"
 
 namespace wf {
@@ -50,8 +51,8 @@ __global__ __launch_bounds__(256) void dense_sum(const float* __restrict__ parts
     epilogue_run<D, true>(e, v, r, m, n, N, cnt);
 }
 
-// rows of an operand whose values lie one after another along K, as [R, KP] rows of whole stages, zeros past K: a run of 8
-// values a thread, loaded at any alignment
+// rows of K consecutive values (of an operand, or of memory where it lies across K) as [R, KP], KP a multiple of 8, zeros
+// past K: a run of 8 values a thread, loaded at any alignment
 __global__ __launch_bounds__(256) void dense_pack_rows(const uint16_t* __restrict__ p, int64_t row, int R, int K, int KP,
                                                        uint16_t* __restrict__ out) {
     const int runs = KP / 8;
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(256) void dense_pack_rows(const uint16_t* __restric
     v.store(out + r * KP + k, 8);
 }
 
-// the same for any strides (values row apart along its rows, col apart along K): 64 x 64 tiles through LDS, read along
+// an operand of any strides (value (r, k) at r row + k col) as such rows, KP a multiple of 64: 64 x 64 tiles through LDS, read along
 // whichever of the two is the shorter step
 __global__ __launch_bounds__(256) void dense_pack(const uint16_t* __restrict__ p, int64_t row, int64_t col, int R, int K,
                                                   int KP, uint16_t* __restrict__ out) {
@@ -150,62 +151,84 @@ static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 struct DenseView {                                    // value (r, k) at r * row + k * col
     const void* p;
     int64_t row, col;
+    bool zeros;                                       // along K: rows hold zeros from K up to the next multiple of 8
 };
 
 constexpr int64_t kRowsMost = 64;
 
-// How a call runs: in the few-rows form, or in tiles with its operands loaded along K, across it, or from a copy.
+// How an operand gets to the tiles: as it lies along K or across it, or copied into rows that can be loaded, which keeps
+// that order (along, across) or turns it (any strides, to rows along K).
+enum { LIES_ALONG, LIES_ACROSS, COPY_ALONG, COPY_ACROSS, COPY_TURNED };
+static bool is_across(int how) { return how == LIES_ACROSS || how == COPY_ACROSS; }
+
+// may_cross: whether the operand may lie across K
+static int dense_how(const DenseView& v, int64_t R, int64_t K, bool may_cross) {
+    const bool a16 = aligned(v.p, 16);
+    if (v.col == 1 && (R == 1 || v.row >= K)) {
+        return v.row % 8 == 0 && (K % 8 == 0 || v.zeros) && v.row <= (1 << 20) && a16 ? LIES_ALONG : COPY_ALONG;
+    }
+    if (!may_cross || v.row != 1) return COPY_TURNED;
+    if (v.col % 8 == 0 && v.col >= R && a16 && (K + 128) * v.col * 2 < (1LL << 31)) return LIES_ACROSS;
+    return (K + 128) * up(R, 8) * 2 < (1LL << 31) ? COPY_ACROSS : COPY_TURNED;
+}
+static int64_t dense_copy_row(int how, int64_t R, int64_t K) {
+    return how == COPY_ALONG ? up(K, 8) : how == COPY_ACROSS ? up(R, 8) : up(K, 64);
+}
+static int64_t dense_copy_bytes(int how, int64_t R, int64_t K) {
+    if (how == LIES_ALONG || how == LIES_ACROSS) return 0;
+    return up((how == COPY_ACROSS ? K : R) * dense_copy_row(how, R, K) * 2, 256);
+}
+
+// How a product runs: in the few-rows form, or in tiles.
 struct DenseCall {
     bool few;
     DenseRowsPlan rows;
     DensePlan tiles;
-    bool across_x, across_w, copy_x, copy_w;
-    int64_t kp, w_at, parts_at, bytes;                // a copy's row; offsets into the workspace, x's copy first
+    int how_x, how_w;
+    int64_t w_at, parts_at, bytes;                    // offsets into the workspace, x's copy first
     int slices() const { return few ? rows.slices : tiles.slices; }
 };
-
-// whether an operand can be loaded as it is, along K or across it: 16-byte runs, offsets inside 31 bits
-static bool dense_along(const DenseView& v, int64_t K) {
-    return v.col == 1 && v.row % 8 == 0 && K % 8 == 0 && v.row >= K && v.row <= (1 << 20) && aligned(v.p, 16);
-}
-static bool dense_across(const DenseView& v, int64_t R, int64_t K) {
-    return v.row == 1 && v.col % 8 == 0 && v.col >= R && aligned(v.p, 16) && (K + 128) * v.col * 2 < (1LL << 31);
-}
 
 static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, int64_t N, int64_t K) {
     DenseCall d = {};
     float us;
     d.tiles = dense_plan_tiles(M, N, K, us);
-    const bool along_x = dense_along(x, K), along_w = dense_along(w, K);
-    d.across_w = !along_w && dense_across(w, N, K);
-    d.across_x = !along_x && d.across_w && dense_across(x, M, K);                 // (x across and w along: x is copied)
-    d.copy_x = !along_x && !d.across_x;
-    d.copy_w = !along_w && !d.across_w;
-    if (d.copy_x) us += 3.0f + (float)(M * K) * 1e-6f;                            // (a copy: 4 bytes a value at 4 TB/s)
-    if (d.copy_w) us += 3.0f + (float)(N * K) * 1e-6f;
+    d.how_w = dense_how(w, N, K, true);
+    d.how_x = dense_how(x, M, K, is_across(d.how_w));
+    int64_t copies = dense_copy_bytes(d.how_x, M, K);
+    if (copies) us += 3.0f + (float)copies * 0.5e-6f;                             // (read and written at 4 TB/s)
+    if (const int64_t c = dense_copy_bytes(d.how_w, N, K)) us += 3.0f + (float)c * 0.5e-6f, copies += c;
     if (M <= kRowsMost && x.col == 1 && w.col == 1 && dense_rows_time(M, N, K) < us) {
         d.few = true;
-        d.copy_x = d.copy_w = false;
         d.rows = dense_plan_rows(M, N, K);
+        copies = 0;
+    } else {
+        d.w_at = dense_copy_bytes(d.how_x, M, K);
     }
-    d.kp = up(K, 64);
-    d.w_at = d.copy_x ? up(M * d.kp * 2, 256) : 0;
-    d.parts_at = d.w_at + (d.copy_w ? up(N * d.kp * 2, 256) : 0);
+    d.parts_at = copies;
     d.bytes = d.parts_at + (d.slices() > 1 ? (int64_t)d.slices() * M * N * 4 : 0);
     return d;
 }
 
-static void dense_copy(const DenseView& v, int64_t R, int64_t K, int64_t kp, uint16_t* out, hipStream_t s) {
+// the operand as the tiles load it, copied to `out` where it has to be
+static DenseOperand dense_operand(const DenseView& v, int how, int64_t R, int64_t K, uint16_t* out, hipStream_t s) {
     const uint16_t* p = static_cast<const uint16_t*>(v.p);
-    if (v.col == 1) {
-        dense_pack_rows<<<dim3((uint32_t)((R * (kp / 8) + 255) / 256)), 256, 0, s>>>(p, v.row, (int)R, (int)K, (int)kp, out);
-        return;
+    const int64_t to = dense_copy_row(how, R, K);
+    auto pack_rows = [&](int64_t row, int64_t n, int64_t values) {
+        dense_pack_rows<<<dim3((uint32_t)((n * (to / 8) + 255) / 256)), 256, 0, s>>>(p, row, (int)n, (int)values, (int)to, out);
+    };
+    switch (how) {
+    case LIES_ALONG: return {p, v.row, (int)(v.zeros ? up(K, 8) : K), (int)R, false};
+    case LIES_ACROSS: return {p, v.col, (int)K, (int)R, true};
+    case COPY_ALONG: pack_rows(v.row, R, K); return {out, to, (int)to, (int)R, false};
+    case COPY_ACROSS: pack_rows(v.col, K, R); return {out, to, (int)K, (int)R, true};
     }
     for (int64_t r = 0; r < R; r += 65535 * 64) {                                 // (a grid's second dimension ends there)
         const int64_t n = std::min<int64_t>(R - r, 65535 * 64);
-        dense_pack<<<dim3((uint32_t)(kp / 64), (uint32_t)((n + 63) / 64)), 256, 0, s>>>(p + r * v.row, v.row, v.col, (int)n,
-                                                                                       (int)K, (int)kp, out + r * kp);
+        dense_pack<<<dim3((uint32_t)(to / 64), (uint32_t)((n + 63) / 64)), 256, 0, s>>>(p + r * v.row, v.row, v.col, (int)n,
+                                                                                       (int)K, (int)to, out + r * to);
     }
+    return {out, to, (int)to, (int)R, false};
 }
 
 static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w, int dt, int64_t M, int64_t N, int64_t K,
@@ -215,13 +238,8 @@ static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w
         dense_rows_run(dt, d.rows, static_cast<const uint16_t*>(x.p), x.row, static_cast<const uint16_t*>(w.p), w.row, (int)M,
                        (int)N, (int)K, parts, e, s);
     } else {
-        auto operand = [&](const DenseView& v, int64_t R, bool across, bool copy, int64_t at) {
-            if (!copy) return DenseOperand{static_cast<const uint16_t*>(v.p), across ? v.col : v.row, (int)K, (int)R, across};
-            uint16_t* out = reinterpret_cast<uint16_t*>(ws + at);
-            dense_copy(v, R, K, d.kp, out, s);
-            return DenseOperand{out, d.kp, (int)d.kp, (int)R, false};
-        };
-        const DenseOperand a = operand(x, M, d.across_x, d.copy_x, 0), b = operand(w, N, d.across_w, d.copy_w, d.w_at);
+        const DenseOperand a = dense_operand(x, d.how_x, M, K, reinterpret_cast<uint16_t*>(ws), s);
+        const DenseOperand b = dense_operand(w, d.how_w, N, K, reinterpret_cast<uint16_t*>(ws + d.w_at), s);
         (a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : dense_gemm_along)(dt, a, b, (int)M, (int)N, (int)K, d.tiles,
                                                                                 parts, e, s);
     }
@@ -230,6 +248,33 @@ static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w
         if (dt == WF_BF16) dense_sum<WF_BF16><<<grid, 256, 0, s>>>(parts, d.slices(), (int)M, (int)N, e);
         else dense_sum<WF_F16><<<grid, 256, 0, s>>>(parts, d.slices(), (int)M, (int)N, e);
     }
+}
+
+// The backward pass: its two products, and where its parts lie in the workspace (dh, the column sums, then the products',
+// one after the other in the same place).
+struct DenseBackward {
+    bool changed;                                     // dh is not dy
+    int64_t dh_row, sums_at, product_at, bytes;
+    DenseView dh_along, w_turned, dh_turned, x_turned;
+    DenseCall dx, dw;
+};
+static DenseBackward dense_backward(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, const void* dy,
+                                    int64_t dy_row, int act, bool gate, int64_t rows_per_group, int64_t M, int64_t N,
+                                    int64_t K, bool dx, bool dw, bool sums, char* ws) {
+    DenseBackward b = {};
+    b.changed = (act != ACT_NONE || gate) && (dx || dw);
+    b.dh_row = b.changed ? up(N, 8) : dy_row;
+    b.sums_at = b.changed ? up(M * b.dh_row * 2, 256) : 0;
+    b.product_at = b.sums_at + (sums ? up(dense_grad_bytes(M, N, rows_per_group), 256) : 0);
+    const void* dh = b.changed ? ws : dy;             // (a workspace not yet there is as aligned as it will be)
+    b.dh_along = {dh, b.dh_row, 1, b.changed};
+    b.w_turned = {w, w_col, w_row, false};
+    b.dh_turned = {dh, 1, b.dh_row, false};
+    b.x_turned = {x, 1, x_row, false};
+    if (dx) b.dx = dense_call(b.dh_along, b.w_turned, M, K, N);
+    if (dw) b.dw = dense_call(b.dh_turned, b.x_turned, N, K, M);
+    b.bytes = b.product_at + std::max(b.dx.bytes, b.dw.bytes);
+    return b;
 }
 
 static int dense_check(const char* who, int dt, int64_t M, int64_t N, int64_t K, int64_t x_row, int64_t x_col,
@@ -256,7 +301,7 @@ extern "C" int wf_dense_workspace(const void* x, int64_t x_row, int64_t x_col, c
     using namespace wf;
     if (!bytes) { set_error("wf_dense_workspace: null pointer"); return WF_EINVAL; }
     if (const int rc = dense_check("wf_dense_workspace", dt, M, N, K, x_row, x_col, w_row, w_col)) return rc;
-    *bytes = M && N ? dense_call({x, x_row, x_col}, {w, w_row, w_col}, M, N, K).bytes : 0;
+    *bytes = M && N ? dense_call({x, x_row, x_col, false}, {w, w_row, w_col, false}, M, N, K).bytes : 0;
     return WF_OK;
 }
 
@@ -279,7 +324,7 @@ extern "C" int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void*
         set_error("wf_dense: a pointer is not aligned to its values");
         return WF_EINVAL;
     }
-    const DenseView xv = {x, x_row, x_col}, wv = {w, w_row, w_col};
+    const DenseView xv = {x, x_row, x_col, false}, wv = {w, w_row, w_col, false};
     const DenseCall d = dense_call(xv, wv, M, N, K);
     if (d.bytes && (!workspace || workspace_bytes < d.bytes || !aligned(workspace, 256))) {
         set_error("wf_dense: a workspace of %lld bytes is required", (long long)d.bytes);
@@ -288,5 +333,80 @@ extern "C" int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void*
     const DenseEpilogue e = {bias, gate, resid, bias_dt, gate_dt, act, gate ? rows_per_group : 1, resid_row, y, h};
     dense_run(d, xv, wv, dt, M, N, K, static_cast<char*>(workspace), e, static_cast<hipStream_t>(stream));
     WF_LAUNCH_CHECK("wf_dense launch");
+    return WF_OK;
+}
+
+static int dense_bwd_check(const char* who, int dt, int64_t M, int64_t N, int64_t K, int64_t x_row, int64_t w_row,
+                           int64_t w_col, int64_t dy_row, int act, int64_t rows_per_group) {
+    using namespace wf;
+    if (const int rc = dense_check(who, dt, M, N, K, x_row, dy_row, w_row, w_col)) return rc;
+    if (rows_per_group <= 0 || M % rows_per_group || act < ACT_NONE || act > ACT_RELU) {
+        set_error("%s: M, rows_per_group = %lld, %lld, activation %d", who, (long long)M, (long long)rows_per_group, act);
+        return WF_EINVAL;
+    }
+    if (M / rows_per_group > 65535 || M > (1 << 20) || N > (1 << 20)) {
+        set_error("%s: more than 65535 groups, or M or N above 2^20", who);
+        return WF_EUNSUPPORTED;
+    }
+    return WF_OK;
+}
+
+extern "C" int wf_dense_bwd_workspace(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col,
+                                      const void* dy, int64_t dy_row, int dt, int act, int gated, int64_t rows_per_group,
+                                      int64_t M, int64_t N, int64_t K, int dx, int dw, int sums, int64_t* bytes) {
+    using namespace wf;
+    if (!bytes) { set_error("wf_dense_bwd_workspace: null pointer"); return WF_EINVAL; }
+    if (const int rc = dense_bwd_check("wf_dense_bwd_workspace", dt, M, N, K, x_row, w_row, w_col, dy_row, act,
+                                       rows_per_group))
+        return rc;
+    *bytes = M && N ? dense_backward(x, x_row, w, w_row, w_col, dy, dy_row, act, gated, rows_per_group, M, N, K, dx, dw, sums,
+                                     nullptr).bytes
+                    : 0;
+    return WF_OK;
+}
+
+extern "C" int wf_dense_bwd(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, const void* dy,
+                            int64_t dy_row, const void* h, int dt, int act, const void* gate, int gate_dt,
+                            int64_t rows_per_group, int64_t M, int64_t N, int64_t K, void* dx, void* dw, void* dbias,
+                            int bias_dt, void* dgate, void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace wf;
+    if (const int rc = dense_bwd_check("wf_dense_bwd", dt, M, N, K, x_row, w_row, w_col, dy_row, act, rows_per_group))
+        return rc;
+    if ((gate && gate_dt != dt && gate_dt != WF_F32) || (dbias && bias_dt != dt && bias_dt != WF_F32)) {
+        set_error("wf_dense_bwd: dtype codes %d, %d", gate_dt, bias_dt);
+        return WF_EINVAL;
+    }
+    if (M == 0 || N == 0) return WF_OK;
+    if (!dy || (dx && !w) || (dw && !x) || ((act != ACT_NONE || dgate) && !h) || (dgate && !gate)) {
+        set_error("wf_dense_bwd: null pointer");
+        return WF_EINVAL;
+    }
+    if (!aligned(x, 2) || !aligned(w, 2) || !aligned(dy, 2) || !aligned(h, 2) || !aligned(dx, 2) || !aligned(dw, 2) ||
+        !aligned(gate, gate_dt == WF_F32 ? 4 : 2) || !aligned(dgate, gate_dt == WF_F32 ? 4 : 2) ||
+        !aligned(dbias, bias_dt == WF_F32 ? 4 : 2)) {
+        set_error("wf_dense_bwd: a pointer is not aligned to its values");
+        return WF_EINVAL;
+    }
+    char* ws = static_cast<char*>(workspace);
+    const bool sums = dbias || dgate;
+    const DenseBackward b = dense_backward(x, x_row, w, w_row, w_col, dy, dy_row, act, gate, rows_per_group, M, N, K, dx, dw,
+                                           sums, ws);
+    if (b.bytes && (!ws || workspace_bytes < b.bytes || !aligned(ws, 256))) {
+        set_error("wf_dense_bwd: a workspace of %lld bytes is required", (long long)b.bytes);
+        return WF_EINVAL;
+    }
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (b.changed || sums) {
+        const DenseGrad q = {dy, h, gate, dy_row, act, gate_dt, rows_per_group, b.changed ? ws : nullptr, b.dh_row,
+                             dbias, bias_dt, dgate};
+        dense_grad_run(q, dt, M, N, reinterpret_cast<float*>(ws + b.sums_at), s);
+    }
+    DenseEpilogue e = {};
+    e.rows_per_group = 1;
+    e.y = dx;
+    if (dx) dense_run(b.dx, b.dh_along, b.w_turned, dt, M, K, N, ws + b.product_at, e, s);
+    e.y = dw;
+    if (dw) dense_run(b.dw, b.dh_turned, b.x_turned, dt, N, K, M, ws + b.product_at, e, s);
+    WF_LAUNCH_CHECK("wf_dense_bwd launch");
     return WF_OK;
 }

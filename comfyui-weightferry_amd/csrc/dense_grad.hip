@@ -2,14 +2,14 @@
 // bias (dense.hip), and the gradient dy of y:
 //   dh = dy gate act'(h),  dbias = sum over all rows of dh,  dgate = sum over a group's rows of dy a
 // (dx = dh w and dw = dh^T x are products of dense.hip). One pass over dy and h that writes dh, rounded to the operands'
-// type because it is the next products' operand: bound by memory. A lane keeps the sums of its 8 columns in registers
+// type because it is the next products' operand (rows padded with zeros to 16-byte runs): bound by memory. A lane keeps the sums of its 8 columns in registers
 // over the rows its workgroup walks; column_sums.h adds the workgroups' rows in a fixed order.
 
 #include <algorithm>
 #include <type_traits>
 
 #include "column_sums.h"
-#include "dense.h"
+#include "dense_grad.h"
 
 namespace wf {
 
@@ -17,7 +17,7 @@ namespace wf {
 template <int D>
 __global__ __launch_bounds__(256) void dense_dact(const value_t<D>* __restrict__ dy, int64_t ldd,
                                                   const value_t<D>* __restrict__ h, int act, const void* gate, int gate_dt,
-                                                  int64_t rows_per_group, value_t<D>* __restrict__ dh,
+                                                  int64_t rows_per_group, value_t<D>* __restrict__ dh, int64_t ldh,
                                                   float* __restrict__ bparts, float* __restrict__ gparts, int N) {
     __shared__ float red[4][2][512];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void dense_dact(const value_t<D>* __restrict__
         if (dh) {
             Pack<D> o;
             o.put(v);
-            o.store(dh + m * N + n, cnt);
+            o.store(dh + m * ldh + n, 8);                          // (ldh is a multiple of 8: the row's padding, zeros)
         }
     }
     if (!bparts && !gparts) return;
@@ -67,76 +67,37 @@ __global__ __launch_bounds__(256) void dense_dact(const value_t<D>* __restrict__
 }
 
 // workgroups over a group's rows: about 2048 in all, no fewer than 4 rows each
-static int dact_parts(int64_t N, int64_t groups, int64_t rows_per_group) {
-    const int64_t across = (N + 511) / 512 * groups;
+static int dact_parts(int64_t M, int64_t N, int64_t rows_per_group) {
+    const int64_t across = (N + 511) / 512 * (M / rows_per_group);
     return (int)std::min<int64_t>((rows_per_group + 3) / 4, std::max<int64_t>(1, 2048 / across));
 }
 
-}  // namespace wf
-
-extern "C" int wf_dense_grad_workspace(int64_t M, int64_t N, int64_t rows_per_group, int64_t* bytes) {
-    using namespace wf;
-    if (!bytes || M < 0 || N < 0 || rows_per_group <= 0 || M % rows_per_group) {
-        set_error("wf_dense_grad_workspace: bad arguments");
-        return WF_EINVAL;
-    }
-    const int64_t groups = M / rows_per_group;
-    *bytes = M && N ? 2 * groups * dact_parts(N, groups, rows_per_group) * N * 4 : 0;
-    return WF_OK;
+int64_t dense_grad_bytes(int64_t M, int64_t N, int64_t rows_per_group) {
+    return 2 * (M / rows_per_group) * dact_parts(M, N, rows_per_group) * N * 4;
 }
 
-extern "C" int wf_dense_grad(const void* dy, int64_t dy_row, const void* h, int dt, int act, const void* gate, int gate_dt,
-                             int64_t rows_per_group, void* dh, void* dbias, int bias_dt, void* dgate, int64_t M, int64_t N,
-                             void* workspace, int64_t workspace_bytes, void* stream) {
-    using namespace wf;
-    if (M < 0 || N < 0 || dy_row < 0 || rows_per_group <= 0 || M % rows_per_group || act < ACT_NONE || act > ACT_RELU) {
-        set_error("wf_dense_grad: M, N, rows_per_group = %lld, %lld, %lld, activation %d", (long long)M, (long long)N,
-                  (long long)rows_per_group, act);
-        return WF_EINVAL;
-    }
-    if ((dt != WF_BF16 && dt != WF_F16) || (gate && gate_dt != dt && gate_dt != WF_F32) ||
-        (dbias && bias_dt != dt && bias_dt != WF_F32)) {
-        set_error("wf_dense_grad: dtype codes %d, %d, %d", dt, gate_dt, bias_dt);
-        return WF_EUNSUPPORTED;
-    }
-    const int64_t groups = M / rows_per_group;
-    if (groups > 65535 || M > (1 << 24) || N > (1 << 24)) {
-        set_error("wf_dense_grad: more than 65535 groups, or M or N above 2^24");
-        return WF_EUNSUPPORTED;
-    }
-    if (M == 0 || N == 0) return WF_OK;
-    if (!dy || ((act != ACT_NONE || dgate) && !h) || (dgate && !gate)) {
-        set_error("wf_dense_grad: null pointer");
-        return WF_EINVAL;
-    }
-    const int n = dact_parts(N, groups, rows_per_group);
-    const int64_t plane = groups * n * N;
-    float* parts = static_cast<float*>(workspace);
-    if ((dbias || dgate) && (!workspace || workspace_bytes < 2 * plane * 4 || !aligned(workspace, 4))) {
-        set_error("wf_dense_grad: a workspace of %lld bytes is required", (long long)(2 * plane * 4));
-        return WF_EINVAL;
-    }
-    float *bparts = dbias ? parts : nullptr, *gparts = dgate ? parts + plane : nullptr;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
+void dense_grad_run(const DenseGrad& q, int dt, int64_t M, int64_t N, float* parts, hipStream_t s) {
+    const int64_t groups = M / q.rows_per_group;
+    const int n = dact_parts(M, N, q.rows_per_group);
+    float *bparts = q.dbias ? parts : nullptr, *gparts = q.dgate ? parts + groups * n * N : nullptr;
     const dim3 grid((uint32_t)((N + 511) / 512), n, (uint32_t)groups);
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        dense_dact<D><<<grid, 256, 0, s>>>(static_cast<const value_t<D>*>(dy), dy_row, static_cast<const value_t<D>*>(h),
-                                           act, gate, gate_dt, rows_per_group, static_cast<value_t<D>*>(dh), bparts,
-                                           gparts, (int)N);
+        dense_dact<D><<<grid, 256, 0, s>>>(static_cast<const value_t<D>*>(q.dy), q.dy_row, static_cast<const value_t<D>*>(q.h),
+                                           q.act, q.gate, q.gate_dt, q.rows_per_group, static_cast<value_t<D>*>(q.dh),
+                                           q.dh_row, bparts, gparts, (int)N);
     };
     if (dt == WF_BF16) go(std::integral_constant<int, WF_BF16>{});
     else go(std::integral_constant<int, WF_F16>{});
-    WF_LAUNCH_CHECK("wf_dense_grad launch");
     const uint32_t cols = (uint32_t)((N + 63) / 64);
-    if (dbias) {
-        const ColumnSums q = {bparts, dbias, bias_dt, (int)(groups * n)};          // every group's rows: one sum
-        column_sums<<<dim3(cols, 1, 1), 1024, 0, s>>>(q, q, (int)N);
+    if (q.dbias) {
+        const ColumnSums b = {bparts, q.dbias, q.bias_dt, (int)(groups * n)};      // every group's rows: one sum
+        column_sums<<<dim3(cols, 1, 1), 1024, 0, s>>>(b, b, (int)N);
     }
-    if (dgate) {
-        const ColumnSums q = {gparts, dgate, gate_dt, n};
-        column_sums<<<dim3(cols, (uint32_t)groups, 1), 1024, 0, s>>>(q, q, (int)N);
+    if (q.dgate) {
+        const ColumnSums b = {gparts, q.dgate, q.gate_dt, n};
+        column_sums<<<dim3(cols, (uint32_t)groups, 1), 1024, 0, s>>>(b, b, (int)N);
     }
-    WF_LAUNCH_CHECK("wf_dense_grad sums launch");
-    return WF_OK;
 }
+
+}  // namespace wf

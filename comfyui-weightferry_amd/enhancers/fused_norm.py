@@ -11,65 +11,69 @@ import ctypes
 import torch
 
 from .. import _native
-from .operands import CODES, groups_of, plain, ptr, rows_of, wants_grad
+from .operands import CODES, Sizes, groups_of, once, plain, ptr, rows_of, wants_grad, whole
 
 MAX_WIDTH = 32768
 
 
-def _forward(x2, weight, bias, code, pcode, groups, eps, modulation, keep):
+def _ask(rows, width, rows_per_group, code):
+    need = ctypes.c_int64()
+    _native.call("wf_layer_norm_bwd_workspace", rows, width, rows_per_group, code, ctypes.byref(need))
+    return need.value
+
+
+_bytes = Sizes(_ask)
+
+
+def _launch(x2, w, b, code, pcode, groups, eps, modulation, stats):
     rows, width = x2.shape
     dev = x2.device
     y = torch.empty((rows, width), dtype=x2.dtype, device=dev)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep else None
     if rows:
         with _native.on_device(dev):
-            _native.call("wf_layer_norm", x2.data_ptr(), x2.stride(0), code, ptr(weight), ptr(bias), pcode,
-                         1 if modulation else 0, rows // groups, eps, y.data_ptr(), ptr(stats), rows, width,
-                         _native.stream_of(dev))
-    return y, stats
+            rc = _native.lib().wf_layer_norm(x2.data_ptr(), x2.stride(0), code, ptr(w), ptr(b), pcode, modulation,
+                                             rows // groups, eps, y.data_ptr(), ptr(stats), rows, width,
+                                             _native.stream_of(dev))
+        if rc:
+            _native.must(rc, "wf_layer_norm")
+    return y
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, modulation):
-        x2 = rows_of(x, x.shape[-1])
-        w = None if weight is None else weight.contiguous()
-        b = None if bias is None else bias.contiguous()
-        p = w if w is not None else b
-        ctx.code, ctx.pcode = CODES[x.dtype], CODES[x.dtype if p is None else p.dtype]
-        ctx.groups, ctx.modulation, ctx.shape = groups, modulation, x.shape
-        ctx.wshape = None if weight is None else weight.shape
-        ctx.bshape = None if bias is None else bias.shape
-        y, stats = _forward(x2, w, b, ctx.code, ctx.pcode, groups, eps, modulation, True)
+    def forward(ctx, x, weight, bias, code, pcode, groups, eps, modulation):
+        x2, w = rows_of(x, x.shape[-1]), whole(weight)
+        stats = torch.empty((x2.shape[0], 2), dtype=torch.float32, device=x2.device)
+        y = _launch(x2, w, whole(bias), code, pcode, groups, eps, modulation, stats)
+        ctx.how = (code, pcode, groups, modulation, x.shape, None if weight is None else weight.shape,
+                   None if bias is None else bias.shape)
         ctx.save_for_backward(x2, w, stats)
-        return y.view(x.shape)
+        return y if x.dim() == 2 else y.view(x.shape)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dy):
         x2, w, stats = ctx.saved_tensors
-        rows, width = x2.shape
-        dev = x2.device
-        dt = x2.dtype
-        pdt = torch.float32 if ctx.pcode == 2 else dt
+        code, pcode, groups, modulation, shape, wshape, bshape = ctx.how
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        rows, width = x2.shape
+        dev, dt = x2.device, x2.dtype
+        pdt = torch.float32 if pcode == 2 else dt
         new = torch.empty if rows else torch.zeros
-        dx = new((rows, width), dtype=dt, device=dev) if need_x else None
-        dw = new(ctx.wshape, dtype=pdt, device=dev) if need_w else None
-        db = new(ctx.bshape, dtype=pdt, device=dev) if need_b else None
+        dx = new(shape, dtype=dt, device=dev) if need_x else None
+        dw = new(wshape, dtype=pdt, device=dev) if need_w else None
+        db = new(bshape, dtype=pdt, device=dev) if need_b else None
         if rows:
-            d2 = rows_of(dy, width)
-            ws = None
+            d2, ws, need = rows_of(dy, width), None, 0
             if need_w or need_b:
-                need = ctypes.c_int64()
-                _native.call("wf_layer_norm_bwd_workspace", rows, width, rows // ctx.groups, ctx.code, ctypes.byref(need))
-                ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+                need = _bytes((rows, width, rows // groups, code))
+                ws = torch.empty(need, dtype=torch.uint8, device=dev)
             with _native.on_device(dev):
-                _native.call("wf_layer_norm_bwd", x2.data_ptr(), x2.stride(0), d2.data_ptr(), d2.stride(0), ctx.code,
-                             ptr(w), ctx.pcode, 1 if ctx.modulation else 0, rows // ctx.groups, stats.data_ptr(), ptr(dx),
-                             ptr(dw), ptr(db), rows, width, ptr(ws), 0 if ws is None else ws.numel(),
-                             _native.stream_of(dev))
-        return None if dx is None else dx.view(ctx.shape), dw, db, None, None, None
+                rc = _native.lib().wf_layer_norm_bwd(x2.data_ptr(), x2.stride(0), d2.data_ptr(), d2.stride(0), code, ptr(w),
+                                                     pcode, modulation, rows // groups, stats.data_ptr(), ptr(dx), ptr(dw),
+                                                     ptr(db), rows, width, ptr(ws), need, _native.stream_of(dev))
+            if rc:
+                _native.must(rc, "wf_layer_norm_bwd")
+        return dx, dw, db, None, None, None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, modulation=False):
@@ -78,27 +82,30 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, modulation=False):
     ``x``; of x's type or both float32. Any strides; float16, bfloat16 and float32. None when it is not the kernel's case
     (not a plain GPU tensor, another type, K > 32768, more than 65535 groups); ValueError when the shapes do not fit
     together."""
-    code = CODES.get(x.dtype)
-    if code is None or not x.is_cuda or x.dim() == 0 or not plain(x, x.device):
+    dt, dev = x.dtype, x.device
+    pcode = code = CODES.get(dt)
+    dims = x.dim()
+    if code is None or dims == 0 or dev.type != "cuda" or not plain(dev, x, weight, bias):
         return None
     width = x.shape[-1]
-    if not 0 < width <= MAX_WIDTH or x.numel() // width >= 1 << 31:
+    if not 0 < width <= MAX_WIDTH:
         return None
-    rows = x.numel() // width
-    groups, pcode, shared = 1, code, None
+    rows = x.shape[0] if dims == 2 else x.numel() // width
+    groups, first = 1, None
     for t, what in ((weight, "weight"), (bias, "bias")):
         if t is None:
             continue
-        if not plain(t, x.device) or (t.dtype != x.dtype and t.dtype != torch.float32):
-            return None
+        if t.dtype != dt:
+            if t.dtype != torch.float32:
+                return None
+            pcode = 2
         groups = groups_of(t, rows, width, what)
-        if shared is not None and (shared.dtype != t.dtype or shared.numel() != t.numel()):
-            raise ValueError(f"weight {shared.dtype} {tuple(shared.shape)} and bias {t.dtype} {tuple(t.shape)} differ")
-        shared, pcode = t, CODES[t.dtype]
-    if groups > 65535:
+        if first is not None and (first.dtype != t.dtype or first.numel() != t.numel()):
+            raise ValueError(f"weight {first.dtype} {tuple(first.shape)} and bias {t.dtype} {tuple(t.shape)} differ")
+        first = t
+    if groups > 65535 or rows >= 1 << 31:
         return None
     if wants_grad(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, groups, float(eps), bool(modulation))
-    y, _ = _forward(rows_of(x, width), None if weight is None else weight.contiguous(),
-                    None if bias is None else bias.contiguous(), code, pcode, groups, float(eps), modulation, False)
-    return y if x.dim() == 2 else y.view(x.shape)
+        return _LayerNorm.apply(x, weight, bias, code, pcode, groups, float(eps), 1 if modulation else 0)
+    y = _launch(rows_of(x, width), whole(weight), whole(bias), code, pcode, groups, eps, 1 if modulation else 0, None)
+    return y if dims == 2 else y.view(x.shape)

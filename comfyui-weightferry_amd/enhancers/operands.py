@@ -1,15 +1,27 @@
 """What the training-step operators (fused_norm, fused_dense, fused_adamw) ask of their tensors. The kernels read memory,
-so tensors that are more than memory (subclasses, functorch wrappers, forward-mode duals) are not their case."""
+so tensors that are more than memory (subclasses, functorch wrappers, forward-mode duals, negative views) are not their
+case. These questions run once per call, so each is asked in its cheapest form."""
 import torch
+from torch.autograd import forward_ad
 
 CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}      # the library's dtype codes
+_TYPES = frozenset((torch.Tensor, torch.nn.Parameter))
+_level = torch._C._functorch.maybe_current_level
+_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
+_grad_enabled = torch.is_grad_enabled
 
 
-def plain(t, device):
-    """Whether ``t`` is an ordinary tensor on ``device``."""
-    return (type(t) in (torch.Tensor, torch.nn.Parameter) and t.device == device
-            and not torch._C._functorch.is_functorch_wrapped_tensor(t) and not t._is_zerotensor() and not t.is_neg()
-            and torch.autograd.forward_ad.unpack_dual(t).tangent is None)
+def plain(device, *tensors):
+    """Whether each of ``tensors`` is None or an ordinary tensor on ``device``."""
+    deep = _level() is not None or forward_ad._current_level >= 0    # functorch or forward mode is at work somewhere
+    for t in tensors:
+        if t is None:
+            continue
+        if type(t) not in _TYPES or t.device != device or t.is_neg():
+            return False
+        if deep and (_wrapped(t) or t._is_zerotensor() or forward_ad.unpack_dual(t).tangent is not None):
+            return False
+    return True
 
 
 def rows_of(t, width):
@@ -18,20 +30,55 @@ def rows_of(t, width):
     return t2 if t2.stride(1) == 1 or width == 1 else t2.contiguous()
 
 
+def whole(t):
+    """``t`` contiguous, or None for None."""
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def groups_of(t, rows, width, what):
     """The number of row groups that a parameter [width] or [..., groups, width] stands for; ValueError when it is not one
     row a group of ``rows // groups`` consecutive rows."""
-    if t.dim() == 0 or t.shape[-1] != width:
-        raise ValueError(f"{what} has shape {tuple(t.shape)}: its last dimension has to be {width}")
-    groups = t.numel() // width
+    shape = t.shape
+    if not shape or shape[-1] != width:
+        raise ValueError(f"{what} has shape {tuple(shape)}: its last dimension has to be {width}")
+    groups = 1 if len(shape) == 1 else t.numel() // width
     if groups == 0 or rows % groups:
-        raise ValueError(f"{what} has shape {tuple(t.shape)}: {rows} rows are no whole number of its {groups} groups")
+        raise ValueError(f"{what} has shape {tuple(shape)}: {rows} rows are no whole number of its {groups} groups")
     return groups
 
 
 def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if _grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def once(backward):
+    """A Function's backward that is differentiable once: with create_graph, torch's own wrapper (whose result refuses a
+    second derivative); without, as it nearly always is, the bare function."""
+    wrapped = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, dy):
+        return wrapped(ctx, dy) if _grad_enabled() else backward(ctx, dy)
+    return staticmethod(run)
+
+
+class Sizes:
+    """Workspace bytes by call shape: the library's answer depends on nothing else, so it is asked once a shape."""
+
+    def __init__(self, ask):
+        self._ask, self._known = ask, {}
+
+    def __call__(self, key):
+        need = self._known.get(key)
+        if need is None:
+            if len(self._known) > 4096:
+                self._known.clear()
+            need = self._known[key] = self._ask(*key)
+        return need

@@ -197,8 +197,7 @@ int wf_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldd, i
  * sums with the bias, [M, N] of type dt, what wf_dense_grad reads (float16: kept finite). M, N <= 2^24, K <= 2^20.
  * The workspace (256-byte aligned, at least the bytes that wf_dense_workspace gives for the same operands) holds copies of
  * operands that cannot be loaded as they are, and the partial sums of products that run in slices of K; it need not be
- * cleared and is free again when the call's work on the stream is done. The products of the backward pass are this call
- * too: dx = dh . w is (dh, w with row and col exchanged), dw = dh^T . x both exchanged. */
+ * cleared and is free again when the call's work on the stream is done. */
 int wf_dense_workspace(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt,
                        int64_t M, int64_t N, int64_t K, int64_t* bytes);
 int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt, int64_t M,
@@ -206,13 +205,19 @@ int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t
              int64_t rows_per_group, const void* resid, int64_t resid_row, void* y, void* h, void* workspace,
              int64_t workspace_bytes, void* stream);
 
-/* The element-wise part of its backward pass: dh = dy gate act'(h) [M, N], dbias = the sum over rows of dh (bias_dt), dgate =
- * the sum over each group's rows of dy act(h) (gate_dt); any of the three may be NULL. dy: rows dy_row values apart; h
- * may be NULL when act is 0 and dgate NULL. Workspace as above, 4-byte aligned, only for dbias and dgate. */
-int wf_dense_grad_workspace(int64_t M, int64_t N, int64_t rows_per_group, int64_t* bytes);
-int wf_dense_grad(const void* dy, int64_t dy_row, const void* h, int dt, int act, const void* gate, int gate_dt,
-                  int64_t rows_per_group, void* dh, void* dbias, int bias_dt, void* dgate, int64_t M, int64_t N,
-                  void* workspace, int64_t workspace_bytes, void* stream);
+/* Its backward pass for the gradient dy of y (rows dy_row values apart), h as wf_dense left it (NULL without an activation
+ * and dgate): dh = dy gate act'(h) is rounded to dt, then dx = dh . w [M, K], dw = dh^T . x [N, K], dbias = the sum over rows
+ * of the unrounded dh (bias_dt), dgate = the sum over each group's rows of dy act(h) (gate_dt); any of the four may be NULL.
+ * (resid's gradient is dy.) x: rows x_row values apart; w as in wf_dense. M, N, K <= 2^20, at most 65535 groups. The workspace
+ * (256-byte aligned; wf_dense_bwd_workspace for the same operands, gated: whether there is a gate, dx, dw: whether they
+ * are wanted, sums: dbias or dgate is) holds dh, partial sums and what the products need. Every sum has a fixed order. */
+int wf_dense_bwd_workspace(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, const void* dy,
+                           int64_t dy_row, int dt, int act, int gated, int64_t rows_per_group, int64_t M, int64_t N,
+                           int64_t K, int dx, int dw, int sums, int64_t* bytes);
+int wf_dense_bwd(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, const void* dy, int64_t dy_row,
+                 const void* h, int dt, int act, const void* gate, int gate_dt, int64_t rows_per_group, int64_t M,
+                 int64_t N, int64_t K, void* dx, void* dw, void* dbias, int bias_dt, void* dgate, void* workspace,
+                 int64_t workspace_bytes, void* stream);
 
 /* One AdamW step (step >= 1) of `count` tensors of type dt, in place: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
  * p = (1 - lr decay) p - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps). table: host memory, read before the
