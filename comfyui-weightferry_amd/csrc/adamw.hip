@@ -15,8 +15,13 @@
 // wave reduction and nothing is read twice. A gradient that is not finite makes its block's scales so, and the block's
 // moments NaN from then on.
 //
-// Products, sums, quotients and roots of the moments and their codes are rounded one by one (no contraction), in the
-// order written here: the codes are defined to the bit.
+// The moments and their codes are defined to the bit: products, sums, quotients and roots rounded correctly one by one (no
+// contraction), in the order written here. Correct quotients and roots are a dozen instructions each, and with them the
+// 8-bit step was bound by the vector unit (118 instructions a value: 141.6 M bfloat16 values 431 us). So a code is
+// computed by the hardware's one-ulp reciprocal and root first, which decides it unless the unrounded code lies within
+// 2^-11 of a half -- four times what the two ways can differ by -- and only then the correct way, for the four values of a
+// lane: 278 us, 5.1 TB/s. The parameter's step uses the one-ulp forms throughout; its error is far below the parameter's own
+// rounding.
 
 #include <algorithm>
 #include <cmath>
@@ -28,7 +33,7 @@ namespace wf {
 
 constexpr int kBlock = 256;               // values that share a scale: 64 lanes of 4
 constexpr int kAdamTensors = 96;          // tensors a launch (its arguments stay below 4 KiB)
-constexpr int kSpan = 4;                  // blocks a wave
+constexpr int kSpan = 2;                  // blocks a wave (2, 4, 8: 71, 77, 88 us for 14.7 M float32 values in 8 bits)
 constexpr int kAdamWg = 4 * kSpan;        // blocks a workgroup of 4 waves
 
 struct AdamTable {
@@ -44,28 +49,36 @@ struct AdamConst {
     float b1, b1c, b2, b2c, keep, rate, root, eps;   // b1c = 1 - b1; keep = 1 - lr decay; rate = lr / (1 - b1^t); root
 };                                                   // = 1 / sqrt(1 - b2^t)
 
-// 4 values at p (the alignment of one value), the first n of them
-template <int D>
+// 4 values at p (the alignment of one value), the first n of them; STREAM: past the caches' ordinary replacement
+template <int D, bool STREAM>
 __device__ __forceinline__ void load4(float (&v)[4], const value_t<D>* p, int n) {
-    value_t<D> r[4] = {0, 0, 0, 0};
-    if (n >= 4) __builtin_memcpy(r, p, sizeof(r));
-    else
+    typedef value_t<D> quad __attribute__((ext_vector_type(4), aligned(sizeof(value_t<D>))));
+    quad r = {0, 0, 0, 0};
+    if (n >= 4) {
+        if constexpr (STREAM) r = __builtin_nontemporal_load(reinterpret_cast<const quad*>(p));
+        else r = *reinterpret_cast<const quad*>(p);
+    } else {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (i < n) r[i] = p[i];
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) v[i] = to_f32<D>(r[i]);
 }
-template <int D>
+template <int D, bool STREAM>
 __device__ __forceinline__ void store4(const float (&v)[4], value_t<D>* p, int n) {
-    value_t<D> r[4];
+    typedef value_t<D> quad __attribute__((ext_vector_type(4), aligned(sizeof(value_t<D>))));
+    quad r;
 #pragma unroll
     for (int i = 0; i < 4; i++) r[i] = from_f32<D>(v[i]);
-    if (n >= 4) __builtin_memcpy(p, r, sizeof(r));
-    else
+    if (n >= 4) {
+        if constexpr (STREAM) __builtin_nontemporal_store(r, reinterpret_cast<quad*>(p));
+        else *reinterpret_cast<quad*>(p) = r;
+    } else {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (i < n) p[i] = r[i];
+    }
 }
 
 __device__ __forceinline__ float avg_value(int q, float scale) {
@@ -77,9 +90,27 @@ __device__ __forceinline__ float sq_value(uint32_t q, float scale) {
     const float u = c * c * scale;
     return u * u;
 }
-__device__ __forceinline__ bool usable(float scale) { return scale > 0.0f && scale <= 3.402823466e+38f; }
+// 4 codes rint(most * sqrt(x / s)) of a block with the largest x s; x: the magnitudes to one ulp, exact(i) to the bit
+// (valid for largest values above `low`: there the values whose magnitude the hardware's root may lose code to 0 either way)
+template <typename F>
+__device__ __forceinline__ void codes(int (&q)[4], const float (&x)[4], float s, float low, float most, F&& exact) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) q[i] = 0;
+    if (!(s > 0.0f && s <= 3.402823466e+38f)) return;              // an empty block, or one that is not finite
+    bool close = !(s > low && s < 1e30f);
+    const float inv = __builtin_amdgcn_rcpf(s);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float t = __builtin_amdgcn_sqrtf(x[i] * inv) * most, r = rintf(t);
+        q[i] = (int)r;
+        close = close || fabsf(t - r) > 0.5f - 0x1p-11f;
+    }
+    if (close)
+#pragma unroll
+        for (int i = 0; i < 4; i++) q[i] = (int)rintf(sqrtf(exact(i) / s) * most);
+}
 
-template <int D, bool EIGHT>
+template <int D, bool EIGHT, bool STREAM>
 __global__ __launch_bounds__(256) void adamw(AdamTable t, AdamConst k, void* __restrict__ m_, void* __restrict__ v_,
                                              float* __restrict__ ms, float* __restrict__ vs) {
     int lo = 0, hi = t.count - 1;                        // the last tensor whose first workgroup is not past this one
@@ -99,8 +130,8 @@ __global__ __launch_bounds__(256) void adamw(AdamTable t, AdamConst k, void* __r
         if ((b0 + b) * kBlock >= n) break;
         const int64_t at = (b0 + b) * kBlock + 4 * lane, blk = t.block[lo] + b0 + b, sat = blk * kBlock + 4 * lane;
         const int left = (int)min<int64_t>(4, n - at);
-        load4<D>(gv[b], g + at, left);
-        load4<D>(pv[b], p + at, left);
+        load4<D, STREAM>(gv[b], g + at, left);
+        load4<D, STREAM>(pv[b], p + at, left);
         if constexpr (EIGHT) {
             const uint32_t qm = *reinterpret_cast<const uint32_t*>(static_cast<const int8_t*>(m_) + sat);
             const uint32_t qv = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(v_) + sat);
@@ -111,8 +142,8 @@ __global__ __launch_bounds__(256) void adamw(AdamTable t, AdamConst k, void* __r
                 vv[b][i] = sq_value(qv >> (8 * i) & 255u, sv);
             }
         } else {
-            load4<WF_F32>(mv[b], static_cast<const float*>(m_) + sat, 4);
-            load4<WF_F32>(vv[b], static_cast<const float*>(v_) + sat, 4);
+            load4<WF_F32, STREAM>(mv[b], static_cast<const float*>(m_) + sat, 4);
+            load4<WF_F32, STREAM>(vv[b], static_cast<const float*>(v_) + sat, 4);
         }
     }
 #pragma unroll
@@ -120,33 +151,37 @@ __global__ __launch_bounds__(256) void adamw(AdamTable t, AdamConst k, void* __r
         if ((b0 + b) * kBlock >= n) break;
         const int64_t at = (b0 + b) * kBlock + 4 * lane, blk = t.block[lo] + b0 + b, sat = blk * kBlock + 4 * lane;
         const int left = (int)min<int64_t>(4, n - at);
-        float u[4], am = 0.0f, au = 0.0f;
+        float am[4], u[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             mv[b][i] = mv[b][i] * k.b1 + gv[b][i] * k.b1c;
             vv[b][i] = vv[b][i] * k.b2 + gv[b][i] * gv[b][i] * k.b2c;
-            u[i] = sqrtf(vv[b][i]);
+            am[i] = fabsf(mv[b][i]);
+            u[i] = __builtin_amdgcn_sqrtf(vv[b][i]);
+            if (vv[b][i] > 0.0f && vv[b][i] < 1e-30f) u[i] = sqrtf(vv[b][i]);      // (the hardware's drops subnormals)
             const float denom = u[i] * k.root + k.eps;
-            pv[b][i] = pv[b][i] * k.keep - mv[b][i] / denom * k.rate;
+            pv[b][i] = pv[b][i] * k.keep - mv[b][i] * __builtin_amdgcn_rcpf(denom) * k.rate;
         }
-        store4<D>(pv[b], p + at, left);
+        store4<D, STREAM>(pv[b], p + at, left);
         if constexpr (EIGHT) {
+            uint32_t bm = 0, bv = 0;                               // the largest by their bits: NaN above infinity
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const uint32_t bm = __float_as_uint(fabsf(mv[b][i])), bu = __float_as_uint(u[i]) & 0x7fffffffu;
-                am = __uint_as_float(max(__float_as_uint(am), bm));
-                au = __uint_as_float(max(__float_as_uint(au), bu));
+                bm = max(bm, __float_as_uint(am[i]));
+                bv = max(bv, __float_as_uint(vv[b][i]) & 0x7fffffffu);
             }
-            const float sm = wave_max_bits(am), su = wave_max_bits(au);
-            const bool okm = usable(sm), oku = usable(su);
+            // (the root is monotonic, rounded too: the largest root is the root of the largest)
+            const float sm = wave_max_bits(__uint_as_float(bm)), su = sqrtf(wave_max_bits(__uint_as_float(bv)));
+            int a[4], c[4];
+            codes(a, am, sm, 1e-30f, 127.0f, [&](int i) { return am[i]; });
+            codes(c, u, su, 1e-11f, 255.0f, [&](int i) { return sqrtf(vv[b][i]); });
+            const int least = su > 0.0f && su <= 3.402823466e+38f ? 1 : 0;
             uint32_t qm = 0, qv = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int a = okm ? (int)rintf(sqrtf(fabsf(mv[b][i]) / sm) * 127.0f) : 0;
-                int c = oku ? (int)rintf(sqrtf(u[i] / su) * 255.0f) : 0;
-                if (oku && u[i] > 0.0f) c = max(c, 1);
-                qm |= (uint32_t)((mv[b][i] < 0.0f ? -a : a) & 255) << (8 * i);
-                qv |= (uint32_t)(c & 255) << (8 * i);
+                if (vv[b][i] > 0.0f) c[i] = max(c[i], least);
+                qm |= (uint32_t)((mv[b][i] < 0.0f ? -a[i] : a[i]) & 255) << (8 * i);
+                qv |= (uint32_t)(c[i] & 255) << (8 * i);
             }
             *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(m_) + sat) = qm;
             *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(v_) + sat) = qv;
@@ -155,8 +190,8 @@ __global__ __launch_bounds__(256) void adamw(AdamTable t, AdamConst k, void* __r
                 vs[blk] = su;
             }
         } else {
-            store4<WF_F32>(mv[b], static_cast<float*>(m_) + sat, 4);
-            store4<WF_F32>(vv[b], static_cast<float*>(v_) + sat, 4);
+            store4<WF_F32, STREAM>(mv[b], static_cast<float*>(m_) + sat, 4);
+            store4<WF_F32, STREAM>(vv[b], static_cast<float*>(v_) + sat, 4);
         }
     }
 }
@@ -222,6 +257,9 @@ extern "C" int wf_adamw(const int64_t* table, int64_t count, int dt, int bits, v
     k.root = (float)(1 / std::sqrt(1 - std::pow(beta2, (double)step)));
     k.eps = (float)eps;
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    // float32 moments past what the 256 MB last-level cache could keep for the next step go by it: 141.6 M bfloat16 values
+    // (3.1 GB) 525 against 577 us; 14.7 M float32 values (0.4 GB) 75 against 66. In 8 bits no difference.
+    const bool stream_past = (double)blocks * kBlock * (16 + 3 * (double)size) > 1e9;
     AdamTable t;
     t.count = 0;
     block = 0;
@@ -230,8 +268,10 @@ extern "C" int wf_adamw(const int64_t* table, int64_t count, int dt, int bits, v
         t.wg[t.count] = wgs;
         auto go = [&](auto d) {
             constexpr int D = decltype(d)::value;
-            if (bits == 8) adamw<D, true><<<dim3(wgs), 256, 0, s>>>(t, k, exp_avg, exp_avg_sq, avg_scale, sq_scale);
-            else adamw<D, false><<<dim3(wgs), 256, 0, s>>>(t, k, exp_avg, exp_avg_sq, avg_scale, sq_scale);
+            if (bits == 8) adamw<D, true, false><<<dim3(wgs), 256, 0, s>>>(t, k, exp_avg, exp_avg_sq, avg_scale, sq_scale);
+            else if (stream_past)
+                adamw<D, false, true><<<dim3(wgs), 256, 0, s>>>(t, k, exp_avg, exp_avg_sq, avg_scale, sq_scale);
+            else adamw<D, false, false><<<dim3(wgs), 256, 0, s>>>(t, k, exp_avg, exp_avg_sq, avg_scale, sq_scale);
         };
         if (dt == WF_F16) go(std::integral_constant<int, WF_F16>{});
         else if (dt == WF_BF16) go(std::integral_constant<int, WF_BF16>{});

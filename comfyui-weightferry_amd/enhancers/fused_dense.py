@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from .. import _native
-from .operands import CODES, Sizes, groups_of, once, plain, ptr, rows_of, wants_grad, whole
+from .operands import CODES, Sizes, applier, groups_of, once, plain, ptr, rows_of, wants_grad, whole
 
 ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "relu": 4}
 MAX_ROWS, MAX_K = 1 << 24, 1 << 20
@@ -64,7 +64,8 @@ def _launch(x2, w, b, code, act, resid, gate, groups, keep):
 
 class _Dense(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, gate, code, act, groups):
+    def forward(ctx, x, weight, bias, residual, gate, how):
+        code, act, groups = how
         x2, w, g = rows_of(x, x.shape[-1]), _matrix(weight), whole(gate)
         n = w.shape[0]
         keep = act != 0 or ctx.needs_input_grad[4]       # the activation's slope and the gate's gradient read h
@@ -100,7 +101,10 @@ class _Dense(torch.autograd.Function):
                                                 need, _native.stream_of(dev))
             if rc:
                 _native.must(rc, "wf_dense_bwd")
-        return dx, dw, db, dy if need_r else None, dg, None, None, None
+        return dx, dw, db, dy if need_r else None, dg, None
+
+
+_apply = applier(_Dense)
 
 
 def dense(x, weight, bias=None, act=None, residual=None, gate=None):
@@ -144,7 +148,7 @@ def dense(x, weight, bias=None, act=None, residual=None, gate=None):
         return None
     code = CODES[dt]
     if grads:
-        return _Dense.apply(x, weight, bias, residual, gate, code, act_code, groups)
+        return _apply(x, weight, bias, residual, gate, (code, act_code, groups))
     y, _ = _launch(rows_of(x, k), _matrix(weight), whole(bias), code, act_code,
                    None if residual is None else rows_of(residual, n), whole(gate), groups, False)
     return y if dims == 2 else y.view(*xshape[:-1], n)

@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from .. import _native
-from .operands import CODES, Sizes, groups_of, once, plain, ptr, rows_of, wants_grad, whole
+from .operands import CODES, Sizes, applier, groups_of, once, plain, ptr, rows_of, wants_grad, whole
 
 MAX_WIDTH = 32768
 
@@ -41,7 +41,8 @@ def _launch(x2, w, b, code, pcode, groups, eps, modulation, stats):
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, code, pcode, groups, eps, modulation):
+    def forward(ctx, x, weight, bias, how):
+        code, pcode, groups, eps, modulation = how
         x2, w = rows_of(x, x.shape[-1]), whole(weight)
         stats = torch.empty((x2.shape[0], 2), dtype=torch.float32, device=x2.device)
         y = _launch(x2, w, whole(bias), code, pcode, groups, eps, modulation, stats)
@@ -59,7 +60,7 @@ class _LayerNorm(torch.autograd.Function):
         dev, dt = x2.device, x2.dtype
         pdt = torch.float32 if pcode == 2 else dt
         new = torch.empty if rows else torch.zeros
-        dx = new(shape, dtype=dt, device=dev) if need_x else None
+        dx = (torch.empty_like(dy) if dy.is_contiguous() else new(shape, dtype=dt, device=dev)) if need_x else None
         dw = new(wshape, dtype=pdt, device=dev) if need_w else None
         db = new(bshape, dtype=pdt, device=dev) if need_b else None
         if rows:
@@ -73,7 +74,10 @@ class _LayerNorm(torch.autograd.Function):
                                                      ptr(db), rows, width, ptr(ws), need, _native.stream_of(dev))
             if rc:
                 _native.must(rc, "wf_layer_norm_bwd")
-        return dx, dw, db, None, None, None, None, None
+        return dx, dw, db, None
+
+
+_apply = applier(_LayerNorm)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, modulation=False):
@@ -106,6 +110,6 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, modulation=False):
     if groups > 65535 or rows >= 1 << 31:
         return None
     if wants_grad(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, code, pcode, groups, float(eps), 1 if modulation else 0)
+        return _apply(x, weight, bias, (code, pcode, groups, float(eps), 1 if modulation else 0))
     y = _launch(rows_of(x, width), whole(weight), whole(bias), code, pcode, groups, eps, 1 if modulation else 0, None)
     return y if dims == 2 else y.view(x.shape)

@@ -69,6 +69,12 @@ def once(backward):
     return staticmethod(run)
 
 
+def applier(function):
+    """``function.apply`` without its Python layer, which unwraps functorch's tensors (``plain`` has refused them by then)
+    and costs as much as a launch's checks."""
+    return super(torch.autograd.Function, function).apply
+
+
 class Sizes:
     """Workspace bytes by call shape: the library's answer depends on nothing else, so it is asked once a shape."""
 

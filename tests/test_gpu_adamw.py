@@ -112,6 +112,23 @@ def test_small_moments_keep_a_code(native):
     assert bool(torch.isfinite(p).all()) and float(p.abs().max()) < 0.1 * 40 * 1.01 and float(p[1]) == 0.0
 
 
+@pytest.mark.parametrize("size", [1e-22, 1e-18, 1e-13, 1e-6, 1e12])
+def test_codes_at_the_ends_of_the_range(native, size):
+    # second moments from subnormal to huge, where the quick way to a code does not hold: to the bit all the same
+    g = torch.Generator().manual_seed(3)
+    grad = torch.randn(4096, generator=g) * size * 10.0 ** torch.empty(4096).uniform_(-3, 0, generator=g)
+    p = torch.zeros(4096, device="cuda")
+    state = fa.adamw_state([p], 8)
+    m, v = torch.zeros(4096), torch.zeros(4096)
+    for step in range(1, 4):
+        fa.adamw_step([p], [grad.cuda()], state, step, betas=(0.9, 0.99))
+        em, ev = encode_avg(m * 0.9 + grad * (1 - 0.9)), encode_sq(v * 0.99 + grad * grad * (1 - 0.99))
+        for k, t in enumerate((em[0], ev[0], em[1], ev[1])):
+            assert torch.equal(state[k].cpu(), t), (step, k)
+        m, v = decode([t.cpu() for t in state])
+    assert bool(torch.isfinite(p).all())
+
+
 def test_many_tensors_offsets_and_order(native):
     # more tensors than one launch takes, at every alignment of their type, give what one call each gives
     n = 230
