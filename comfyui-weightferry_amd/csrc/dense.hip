@@ -185,12 +185,15 @@ struct DenseCall {
     DenseRowsPlan rows;
     DensePlan tiles;
     int how_x, how_w;
-    int64_t w_at, parts_at, bytes;                    // offsets into the workspace, x's copy first
+    bool plain;                                       // the epilogue is at most a bias
+    bool summed;                                      // float32 partial sums first: slices, or operands across K with more
+    int64_t w_at, parts_at, bytes;                    // than a plain epilogue. Offsets into the workspace, x's copy first
     int slices() const { return few ? rows.slices : tiles.slices; }
 };
 
-static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, int64_t N, int64_t K) {
+static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, int64_t N, int64_t K, bool plain) {
     DenseCall d = {};
+    d.plain = plain;
     float us;
     d.tiles = dense_plan_tiles(M, N, K, us);
     d.how_w = dense_how(w, N, K, true);
@@ -206,7 +209,8 @@ static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, i
         d.w_at = dense_copy_bytes(d.how_x, M, K);
     }
     d.parts_at = copies;
-    d.bytes = d.parts_at + (d.slices() > 1 ? (int64_t)d.slices() * M * N * 4 : 0);
+    d.summed = d.slices() > 1 || (!d.few && !plain && is_across(d.how_w));
+    d.bytes = d.parts_at + (d.summed ? (int64_t)d.slices() * M * N * 4 : 0);
     return d;
 }
 
@@ -233,17 +237,17 @@ static DenseOperand dense_operand(const DenseView& v, int how, int64_t R, int64_
 
 static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w, int dt, int64_t M, int64_t N, int64_t K,
                       char* ws, const DenseEpilogue& e, hipStream_t s) {
-    float* parts = reinterpret_cast<float*>(ws + d.parts_at);
+    float* parts = d.summed ? reinterpret_cast<float*>(ws + d.parts_at) : nullptr;
     if (d.few) {
         dense_rows_run(dt, d.rows, static_cast<const uint16_t*>(x.p), x.row, static_cast<const uint16_t*>(w.p), w.row, (int)M,
                        (int)N, (int)K, parts, e, s);
     } else {
         const DenseOperand a = dense_operand(x, d.how_x, M, K, reinterpret_cast<uint16_t*>(ws), s);
         const DenseOperand b = dense_operand(w, d.how_w, N, K, reinterpret_cast<uint16_t*>(ws + d.w_at), s);
-        (a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : dense_gemm_along)(dt, a, b, (int)M, (int)N, (int)K, d.tiles,
-                                                                                parts, e, s);
+        auto run = a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : d.plain || parts ? dense_gemm_along : dense_gemm_along_full;
+        run(dt, a, b, (int)M, (int)N, (int)K, d.tiles, parts, e, s);
     }
-    if (d.slices() > 1) {
+    if (d.summed) {
         const dim3 grid((uint32_t)((M * ((N + 7) / 8) + 255) / 256));
         if (dt == WF_BF16) dense_sum<WF_BF16><<<grid, 256, 0, s>>>(parts, d.slices(), (int)M, (int)N, e);
         else dense_sum<WF_F16><<<grid, 256, 0, s>>>(parts, d.slices(), (int)M, (int)N, e);
@@ -271,8 +275,8 @@ static DenseBackward dense_backward(const void* x, int64_t x_row, const void* w,
     b.w_turned = {w, w_col, w_row, false};
     b.dh_turned = {dh, 1, b.dh_row, false};
     b.x_turned = {x, 1, x_row, false};
-    if (dx) b.dx = dense_call(b.dh_along, b.w_turned, M, K, N);
-    if (dw) b.dw = dense_call(b.dh_turned, b.x_turned, N, K, M);
+    if (dx) b.dx = dense_call(b.dh_along, b.w_turned, M, K, N, true);
+    if (dw) b.dw = dense_call(b.dh_turned, b.x_turned, N, K, M, true);
     b.bytes = b.product_at + std::max(b.dx.bytes, b.dw.bytes);
     return b;
 }
@@ -297,11 +301,11 @@ static int dense_check(const char* who, int dt, int64_t M, int64_t N, int64_t K,
 }  // namespace wf
 
 extern "C" int wf_dense_workspace(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col,
-                                  int dt, int64_t M, int64_t N, int64_t K, int64_t* bytes) {
+                                  int dt, int64_t M, int64_t N, int64_t K, int plain, int64_t* bytes) {
     using namespace wf;
     if (!bytes) { set_error("wf_dense_workspace: null pointer"); return WF_EINVAL; }
     if (const int rc = dense_check("wf_dense_workspace", dt, M, N, K, x_row, x_col, w_row, w_col)) return rc;
-    *bytes = M && N ? dense_call({x, x_row, x_col, false}, {w, w_row, w_col, false}, M, N, K).bytes : 0;
+    *bytes = M && N ? dense_call({x, x_row, x_col, false}, {w, w_row, w_col, false}, M, N, K, plain).bytes : 0;
     return WF_OK;
 }
 
@@ -325,7 +329,7 @@ extern "C" int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void*
         return WF_EINVAL;
     }
     const DenseView xv = {x, x_row, x_col, false}, wv = {w, w_row, w_col, false};
-    const DenseCall d = dense_call(xv, wv, M, N, K);
+    const DenseCall d = dense_call(xv, wv, M, N, K, act == ACT_NONE && !gate && !resid && !h);
     if (d.bytes && (!workspace || workspace_bytes < d.bytes || !aligned(workspace, 256))) {
         set_error("wf_dense: a workspace of %lld bytes is required", (long long)d.bytes);
         return WF_EINVAL;

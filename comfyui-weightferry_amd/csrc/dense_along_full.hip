@@ -1,0 +1,12 @@
+// Tiled kernels of the 16-bit linear, both operands along K, any epilogue: a linear's forward product.
+#include "dense_gemm.h"
+
+namespace wf {
+
+void dense_gemm_along_full(int dt, const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p,
+                           float* parts, const DenseEpilogue& e, hipStream_t s) {
+    if (dt == WF_BF16) dense_tiling<WF_BF16, false, false, false>(a, b, M, N, K, p, parts, e, s);
+    else dense_tiling<WF_F16, false, false, false>(a, b, M, N, K, p, parts, e, s);
+}
+
+}  // namespace wf

@@ -36,8 +36,10 @@ __device__ __forceinline__ DenseTile dense_tile(const DenseOperand& o, int r0) {
     return {tile_rsrc(o.p + at, (end - at) * 2), (uint32_t)o.row * 2u, (uint32_t)o.k * 2u};
 }
 
-// workgroup (tile, slice); parts: [slices, M, N] float32 partial sums, or NULL: one slice and the epilogue
-template <int D, bool AX, bool BX, typename S>
+// Workgroup (tile, slice). parts: [slices, M, N] float32 partial sums, or NULL: one slice, and the outputs. PLAIN: the
+// epilogue is at most a bias, and the rounded outputs pass through LDS (wl_store_tile): 4096 x 5120 outputs at K = 64 take
+// 12.5 us, by the other way 19.6.
+template <int D, bool AX, bool BX, bool PLAIN, typename S>
 __global__ __launch_bounds__(S::NT) void dense_gemm(DenseOperand a, DenseOperand b, int M, int N, int K, int slice_stages,
                                                     float* __restrict__ parts, DenseEpilogue e) {
     constexpr int WM = S::WM, WN = S::WN, TC = WN * 32;
@@ -65,26 +67,31 @@ __global__ __launch_bounds__(S::NT) void dense_gemm(DenseOperand a, DenseOperand
                               [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<D>(c, x, y); });
     const int mw = m0 + wave / S::VN * WM * 32, nw = n0 + wave % S::VN * TC;
     const int lr = lane & 31, lk = lane >> 5;
+    if (PLAIN && !parts) {
+        wl_store_tile<WM, WN>(wl_out_region<S>(sb0, sb1, wave), static_cast<uint16_t*>(e.y), M, N, mw, nw, lane,
+                              [&](int i, int j, int x) { return from_f32<D>(acc[i][j][x]); });
+        return;
+    }
     // the wave's region: 16 rows x TC float32
     constexpr int PER_BUF = S::SLOTS * 16 / (16 * TC * 4);
     static_assert(2 * PER_BUF >= S::NW, "the output rows fit in the stage buffers");
     float* ot = reinterpret_cast<float*>(wave < PER_BUF ? sb0 : sb1) + (wave % PER_BUF) * 16 * TC;
     constexpr int RUNS = TC / 8;
     // (the loop over runs stays a loop: unrolled, the epilogue's code took longer to fetch than to run. What a run needs
-    // from memory is loaded one run ahead.)
-    auto at_run = [&](int mi, int it, auto&& f) {
-        const int q = it * 64 + lane, m = mi + q / RUNS, n = nw + 8 * (q % RUNS);
+    // from memory is loaded two runs ahead.)
+    auto at_run = [&](int half, int it, auto&& f) {
+        const int over = it >= WN, q = (over ? it - WN : it) * 64 + lane;
+        const int m = mw + (half + over) * 16 + q / RUNS, n = nw + 8 * (q % RUNS);
         return f(q, m, n, m < M ? N - n : 0);
     };
+    auto ahead = [&](int half, int it) {
+        return at_run(half, it, [&](int, int m, int n, int cnt) { return epilogue_ahead<D>(e, m, n, N, cnt); });
+    };
+    EpilogueAhead<D> next[2];
+    if (!PLAIN && !parts) next[0] = ahead(0, 0), next[1] = ahead(0, 1);
 #pragma unroll
     for (int half = 0; half < 2 * WM; half++) {
-        const int mi = mw + half * 16;
-        if (mi >= M) break;
-        auto ahead = [&](int it) {
-            return at_run(mi, it, [&](int, int m, int n, int cnt) { return epilogue_ahead<D>(e, m, n, N, cnt); });
-        };
-        EpilogueAhead<D> next;
-        if (!parts) next = ahead(0);
+        if (mw + half * 16 >= M) break;
 #pragma unroll
         for (int x = 0; x < 8; x++)
 #pragma unroll
@@ -92,13 +99,17 @@ __global__ __launch_bounds__(S::NT) void dense_gemm(DenseOperand a, DenseOperand
                 ot[(8 * (x >> 2) + 4 * lk + (x & 3)) * TC + j * 32 + lr] = acc[half / 2][j][8 * (half & 1) + x];
 #pragma unroll 1
         for (int it = 0; it < WN; it++) {
-            const EpilogueAhead<D> now = next;
-            if (!parts && it + 1 < WN) next = ahead(it + 1);
-            at_run(mi, it, [&](int q, int m, int n, int cnt) {
+            EpilogueAhead<D> now;
+            if (!PLAIN && !parts) {
+                now = next[0];
+                next[0] = next[1];
+                next[1] = ahead(half, it + 2);
+            }
+            at_run(half, it, [&](int q, int m, int n, int cnt) {
                 const float4 lo = reinterpret_cast<const float4*>(ot)[2 * q], hi = reinterpret_cast<const float4*>(ot)[2 * q + 1];
                 float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
                 if (cnt <= 0) return;
-                if (!parts) {
+                if (!PLAIN && !parts) {
                     epilogue_run<D, false>(e, v, now, m, n, N, cnt);
                     return;
                 }
@@ -117,33 +128,35 @@ struct DensePlan {
     int tiling, slices, slice_stages;
 };
 
-template <int D, bool AX, bool BX, int VM, int VN, int WM, int WN>
+template <int D, bool AX, bool BX, bool PLAIN, int VM, int VN, int WM, int WN>
 static void dense_launch(const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p,
                          float* parts, const DenseEpilogue& e, hipStream_t s) {
     using S = DenseShape<VM, VN, WM, WN>;
     const int tiles = ((M + S::BM - 1) / S::BM) * ((N + S::BN - 1) / S::BN);
-    dense_gemm<D, AX, BX, S><<<dim3(tiles, p.slices), S::NT, 0, s>>>(a, b, M, N, K, p.slice_stages,
-                                                                     p.slices > 1 ? parts : nullptr, e);
+    dense_gemm<D, AX, BX, PLAIN, S><<<dim3(tiles, p.slices), S::NT, 0, s>>>(a, b, M, N, K, p.slice_stages, parts, e);
 }
 
 // the tilings by number; kDense in dense.hip has their sizes
-template <int D, bool AX, bool BX>
+template <int D, bool AX, bool BX, bool PLAIN>
 static void dense_tiling(const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p, float* parts,
                          const DenseEpilogue& e, hipStream_t s) {
     switch (p.tiling) {
-    case 0: dense_launch<D, AX, BX, 4, 2, 2, 5>(a, b, M, N, K, p, parts, e, s); break;
-    case 1: dense_launch<D, AX, BX, 2, 4, 4, 2>(a, b, M, N, K, p, parts, e, s); break;
-    case 2: dense_launch<D, AX, BX, 4, 2, 2, 3>(a, b, M, N, K, p, parts, e, s); break;
-    case 3: dense_launch<D, AX, BX, 4, 1, 1, 5>(a, b, M, N, K, p, parts, e, s); break;
-    case 4: dense_launch<D, AX, BX, 2, 2, 2, 2>(a, b, M, N, K, p, parts, e, s); break;
-    case 5: dense_launch<D, AX, BX, 1, 4, 2, 1>(a, b, M, N, K, p, parts, e, s); break;
-    default: dense_launch<D, AX, BX, 1, 4, 1, 1>(a, b, M, N, K, p, parts, e, s); break;
+    case 0: dense_launch<D, AX, BX, PLAIN, 4, 2, 2, 5>(a, b, M, N, K, p, parts, e, s); break;
+    case 1: dense_launch<D, AX, BX, PLAIN, 2, 4, 4, 2>(a, b, M, N, K, p, parts, e, s); break;
+    case 2: dense_launch<D, AX, BX, PLAIN, 4, 2, 2, 3>(a, b, M, N, K, p, parts, e, s); break;
+    case 3: dense_launch<D, AX, BX, PLAIN, 4, 1, 1, 5>(a, b, M, N, K, p, parts, e, s); break;
+    case 4: dense_launch<D, AX, BX, PLAIN, 2, 2, 2, 2>(a, b, M, N, K, p, parts, e, s); break;
+    case 5: dense_launch<D, AX, BX, PLAIN, 1, 4, 2, 1>(a, b, M, N, K, p, parts, e, s); break;
+    default: dense_launch<D, AX, BX, PLAIN, 1, 4, 1, 1>(a, b, M, N, K, p, parts, e, s); break;
     }
 }
 
-// one source each: both operands along K, B across, both across
+// One source each: both operands along K with a plain and with any epilogue, B across, both across (plain, or into parts).
+// parts: NULL where the outputs are stored.
 void dense_gemm_along(int dt, const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p,
                       float* parts, const DenseEpilogue& e, hipStream_t s);
+void dense_gemm_along_full(int dt, const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p,
+                           float* parts, const DenseEpilogue& e, hipStream_t s);
 void dense_gemm_b_across(int dt, const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p,
                          float* parts, const DenseEpilogue& e, hipStream_t s);
 void dense_gemm_across(int dt, const DenseOperand& a, const DenseOperand& b, int M, int N, int K, const DensePlan& p,

@@ -113,7 +113,7 @@ static void launch(const DenseRowsPlan& p, const uint16_t* x, int64_t ldx, const
     auto go = [&](auto rt) {
         constexpr int RT = decltype(rt)::value;
         const dim3 grid((uint32_t)((N + 16 * RT - 1) / (16 * RT)), p.slices, (uint32_t)((M + 15) / 16));
-        dense_rows<D, RT><<<grid, 256, 0, s>>>(x, ldx, w, ldw, M, N, K, p.slices > 1 ? parts : nullptr, e);
+        dense_rows<D, RT><<<grid, 256, 0, s>>>(x, ldx, w, ldw, M, N, K, parts, e);
     };
     if (p.tiles == 1) go(std::integral_constant<int, 1>{});
     else go(std::integral_constant<int, 2>{});
