@@ -3,6 +3,8 @@
 // on runs of 8 consecutive outputs of a row.
 #pragma once
 
+#include <type_traits>
+
 #include "values.h"
 
 namespace wf {
@@ -28,22 +30,33 @@ __device__ __forceinline__ float tanh_factor(float h) {
 }
 __device__ __forceinline__ float logistic(float h) { return rcp_of(1.0f + exp2_of(h * -1.4426950408889634f)); }
 
+template <int KIND>
+__device__ __forceinline__ float act_of(float h) {
+    float e;
+    if constexpr (KIND == ACT_GELU) return h * normal_cdf(h, e);
+    else if constexpr (KIND == ACT_GELU_TANH) return h * tanh_factor(h);
+    else if constexpr (KIND == ACT_SILU) return h * logistic(h);
+    else if constexpr (KIND == ACT_RELU) return h < 0.0f ? 0.0f : h;
+    else return h;
+}
+
+// f with the activation as a constant
+template <typename F>
+__device__ __forceinline__ void by_act(int kind, F&& f) {
+    using std::integral_constant;
+    if (kind == ACT_GELU_TANH) f(integral_constant<int, ACT_GELU_TANH>{});
+    else if (kind == ACT_GELU) f(integral_constant<int, ACT_GELU>{});
+    else if (kind == ACT_SILU) f(integral_constant<int, ACT_SILU>{});
+    else if (kind == ACT_RELU) f(integral_constant<int, ACT_RELU>{});
+    else f(integral_constant<int, ACT_NONE>{});
+}
+
 // v = act(v) on a run of values; one decision a run
 __device__ __forceinline__ void act_run(int kind, float (&v)[8]) {
-    float e;
-    if (kind == ACT_GELU_TANH) {
+    by_act(kind, [&](auto k) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= tanh_factor(v[i]);
-    } else if (kind == ACT_GELU) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= normal_cdf(v[i], e);
-    } else if (kind == ACT_SILU) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= logistic(v[i]);
-    } else if (kind == ACT_RELU) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];
-    }
+        for (int i = 0; i < 8; i++) v[i] = act_of<decltype(k)::value>(v[i]);
+    });
 }
 
 // a = act(h) and its slope, from finite h (keep_finite)

@@ -130,10 +130,10 @@ static DensePlan dense_plan_tiles(int64_t M, int64_t N, int64_t K, float& us) {
     return best;
 }
 
-// The few-rows form: weight bytes at 5.2 TB/s, up to 1.4 times that time as 16 rows fill up, more with every 16 rows.
+// The few-rows form: weight bytes at 5.2 TB/s, up to 1.6 times that time as 16 rows fill up, more with every 16 rows.
 // 1 x 13824 x 5120 30 us, 16 x 13824 x 5120 42 (the tiles 35), 16 x 2048 x 8192 12 (19), 32 x 2048 x 2048 5.9 (8.9).
 static float dense_rows_time(int64_t M, int64_t N, int64_t K) {
-    const float fill = 1.0f + 0.4f * (float)std::min<int64_t>(M - 1, 15) / 15.0f;
+    const float fill = 1.0f + 0.6f * (float)std::min<int64_t>(M - 1, 15) / 15.0f;
     const int64_t groups = (M + 15) / 16;
     return 4.0f + (float)(N * K) * 2.0f / 5.2e6f * fill * (groups > 1 ? 0.87f * (float)groups : 1.0f);
 }

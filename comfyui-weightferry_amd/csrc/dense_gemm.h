@@ -37,8 +37,7 @@ __device__ __forceinline__ DenseTile dense_tile(const DenseOperand& o, int r0) {
 }
 
 // Workgroup (tile, slice). parts: [slices, M, N] float32 partial sums, or NULL: one slice, and the outputs. PLAIN: the
-// epilogue is at most a bias, and the rounded outputs pass through LDS (wl_store_tile): 4096 x 5120 outputs at K = 64 take
-// 12.5 us, by the other way 19.6.
+// epilogue is at most a bias.
 template <int D, bool AX, bool BX, bool PLAIN, typename S>
 __global__ __launch_bounds__(S::NT) void dense_gemm(DenseOperand a, DenseOperand b, int M, int N, int K, int slice_stages,
                                                     float* __restrict__ parts, DenseEpilogue e) {
@@ -67,9 +66,19 @@ __global__ __launch_bounds__(S::NT) void dense_gemm(DenseOperand a, DenseOperand
                               [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<D>(c, x, y); });
     const int mw = m0 + wave / S::VN * WM * 32, nw = n0 + wave % S::VN * TC;
     const int lr = lane & 31, lk = lane >> 5;
-    if (PLAIN && !parts) {
-        wl_store_tile<WM, WN>(wl_out_region<S>(sb0, sb1, wave), static_cast<uint16_t*>(e.y), M, N, mw, nw, lane,
-                              [&](int i, int j, int x) { return from_f32<D>(acc[i][j][x]); });
+    // without gate and residual the outputs are computed in the accumulators and pass through LDS rounded, the
+    // pre-activations, where they are kept, before them
+    if (!parts && (PLAIN || (!e.gate && !e.resid))) {
+        auto store = [&](void* out, auto&& f) {
+            wl_store_tile<WM, WN>(wl_out_region<S>(sb0, sb1, wave), static_cast<uint16_t*>(out), M, N, mw, nw, lane,
+                                  [&](int i, int j, int x) { return from_f32<D>(f(acc[i][j][x])); });
+        };
+        if constexpr (PLAIN) {
+            store(e.y, [](float v) { return v; });
+        } else {
+            if (e.h) store(e.h, [](float v) { return keep_finite<D>(v); });
+            by_act(e.act, [&](auto k) { store(e.y, [](float v) { return act_of<decltype(k)::value>(v); }); });
+        }
         return;
     }
     // the wave's region: 16 rows x TC float32
@@ -79,49 +88,59 @@ __global__ __launch_bounds__(S::NT) void dense_gemm(DenseOperand a, DenseOperand
     constexpr int RUNS = TC / 8;
     // (the loop over runs stays a loop: unrolled, the epilogue's code took longer to fetch than to run. What a run needs
     // from memory is loaded two runs ahead.)
-    auto at_run = [&](int half, int it, auto&& f) {
-        const int over = it >= WN, q = (over ? it - WN : it) * 64 + lane;
-        const int m = mw + (half + over) * 16 + q / RUNS, n = nw + 8 * (q % RUNS);
-        return f(q, m, n, m < M ? N - n : 0);
-    };
-    auto ahead = [&](int half, int it) {
-        return at_run(half, it, [&](int, int m, int n, int cnt) { return epilogue_ahead<D>(e, m, n, N, cnt); });
-    };
-    EpilogueAhead<D> next[2];
-    if (!PLAIN && !parts) next[0] = ahead(0, 0), next[1] = ahead(0, 1);
-#pragma unroll
-    for (int half = 0; half < 2 * WM; half++) {
-        if (mw + half * 16 >= M) break;
-#pragma unroll
-        for (int x = 0; x < 8; x++)
-#pragma unroll
-            for (int j = 0; j < WN; j++)
-                ot[(8 * (x >> 2) + 4 * lk + (x & 3)) * TC + j * 32 + lr] = acc[half / 2][j][8 * (half & 1) + x];
-#pragma unroll 1
-        for (int it = 0; it < WN; it++) {
-            EpilogueAhead<D> now;
-            if (!PLAIN && !parts) {
-                now = next[0];
-                next[0] = next[1];
-                next[1] = ahead(half, it + 2);
-            }
-            at_run(half, it, [&](int q, int m, int n, int cnt) {
-                const float4 lo = reinterpret_cast<const float4*>(ot)[2 * q], hi = reinterpret_cast<const float4*>(ot)[2 * q + 1];
-                float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                if (cnt <= 0) return;
-                if (!PLAIN && !parts) {
-                    epilogue_run<D, false>(e, v, now, m, n, N, cnt);
-                    return;
-                }
-                float* o = parts + ((int64_t)blockIdx.y * M + m) * N + n;
-                if (cnt >= 8) __builtin_memcpy(o, v, 32);
-                else
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (i < cnt) o[i] = v[i];
+    // WHOLE: every run is 8 outputs.
+    auto body = [&](auto whole) {
+        auto at_run = [&](int half, int it, auto&& f) {
+            const int over = it >= WN, q = (over ? it - WN : it) * 64 + lane;
+            const int m = mw + (half + over) * 16 + q / RUNS, n = nw + 8 * (q % RUNS);
+            return f(q, m, n, m < M && n < N ? (decltype(whole)::value ? 8 : N - n) : 0);
+        };
+        auto ahead = [&](int half, int it) {
+            return at_run(half, it, [&](int, int m, int n, int cnt) {
+                EpilogueAhead<D> a = {};
+                if (cnt > 0) a = epilogue_ahead<D>(e, m, n, N, decltype(whole)::value ? 8 : cnt);
+                return a;
             });
+        };
+        EpilogueAhead<D> next[2];
+        if (!PLAIN && !parts) next[0] = ahead(0, 0), next[1] = ahead(0, 1);
+#pragma unroll
+        for (int half = 0; half < 2 * WM; half++) {
+            if (mw + half * 16 >= M) break;
+#pragma unroll
+            for (int x = 0; x < 8; x++)
+#pragma unroll
+                for (int j = 0; j < WN; j++)
+                    ot[(8 * (x >> 2) + 4 * lk + (x & 3)) * TC + j * 32 + lr] = acc[half / 2][j][8 * (half & 1) + x];
+#pragma unroll 1
+            for (int it = 0; it < WN; it++) {
+                EpilogueAhead<D> now;
+                if (!PLAIN && !parts) {
+                    now = next[0];
+                    next[0] = next[1];
+                    next[1] = ahead(half, it + 2);
+                }
+                at_run(half, it, [&](int q, int m, int n, int count) {
+                    const float4 lo = reinterpret_cast<const float4*>(ot)[2 * q], hi = reinterpret_cast<const float4*>(ot)[2 * q + 1];
+                    float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                    if (count <= 0) return;
+                    const int cnt = decltype(whole)::value ? 8 : count;
+                    if (!PLAIN && !parts) {
+                        epilogue_run<D, false>(e, v, now, m, n, N, cnt);
+                        return;
+                    }
+                    float* o = parts + ((int64_t)blockIdx.y * M + m) * N + n;
+                    if (cnt >= 8) __builtin_memcpy(o, v, 32);
+                    else
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (i < cnt) o[i] = v[i];
+                });
+            }
         }
-    }
+    };
+    if ((N & 7) == 0) body(std::true_type{});
+    else body(std::false_type{});
 }
 
 struct DensePlan {
