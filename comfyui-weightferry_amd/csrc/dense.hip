@@ -130,12 +130,14 @@ static DensePlan dense_plan_tiles(int64_t M, int64_t N, int64_t K, float& us) {
     return best;
 }
 
-// The few-rows form: weight bytes at 5.2 TB/s, up to 1.6 times that time as 16 rows fill up, more with every 16 rows.
-// 1 x 13824 x 5120 30 us, 16 x 13824 x 5120 42 (the tiles 35), 16 x 2048 x 8192 12 (19), 32 x 2048 x 2048 5.9 (8.9).
-static float dense_rows_time(int64_t M, int64_t N, int64_t K) {
+// The few-rows form: weight bytes at 5.2 TB/s, up to 1.6 times that time as 16 rows fill up, more with every 16 rows, and
+// nearly twice where odd row lengths put the 16-byte loads at odd places (`odd`).
+// 1 x 13824 x 5120 30 us, 16 x 2048 x 8192 12 (the tiles 19), 128 x 1000 x 1024 5.1 (8.0), 12 x 5896 x 9106 36 (75 with the
+// copies that the tiles need); 16 x 5120 x 5120 20 (17), 77 x 2607 x 1531 24 (20).
+static float dense_rows_time(int64_t M, int64_t N, int64_t K, bool odd) {
     const float fill = 1.0f + 0.6f * (float)std::min<int64_t>(M - 1, 15) / 15.0f;
     const int64_t groups = (M + 15) / 16;
-    return 4.0f + (float)(N * K) * 2.0f / 5.2e6f * fill * (groups > 1 ? 0.87f * (float)groups : 1.0f);
+    return 4.0f + (float)(N * K) * 2.0f / 5.2e6f * fill * (groups > 1 ? 0.87f * (float)groups : 1.0f) * (odd ? 1.9f : 1.0f);
 }
 // Two weight tiles a workgroup share x's loads (16 x 5120 x 5120 20 against 25 us) where that leaves 128 workgroups; a
 // single or double row of a wide weight has little of x to share (1 x 13824 x 5120 30.5 against 32.3). A long K of a narrow
@@ -154,7 +156,7 @@ struct DenseView {                                    // value (r, k) at r * row
     bool zeros;                                       // along K: rows hold zeros from K up to the next multiple of 8
 };
 
-constexpr int64_t kRowsMost = 64;
+constexpr int64_t kRowsMost = 256;
 
 // How an operand gets to the tiles: as it lies along K or across it, or copied into rows that can be loaded, which keeps
 // that order (along, across) or turns it (any strides, to rows along K).
@@ -201,7 +203,7 @@ static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, i
     int64_t copies = dense_copy_bytes(d.how_x, M, K);
     if (copies) us += 3.0f + (float)copies * 0.5e-6f;                             // (read and written at 4 TB/s)
     if (const int64_t c = dense_copy_bytes(d.how_w, N, K)) us += 3.0f + (float)c * 0.5e-6f, copies += c;
-    if (M <= kRowsMost && x.col == 1 && w.col == 1 && dense_rows_time(M, N, K) < us) {
+    if (M <= kRowsMost && x.col == 1 && w.col == 1 && dense_rows_time(M, N, K, ((x.row | w.row) & 1) != 0) < us) {
         d.few = true;
         d.rows = dense_plan_rows(M, N, K);
         copies = 0;
