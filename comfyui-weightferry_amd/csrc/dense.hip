@@ -85,20 +85,20 @@ __global__ __launch_bounds__(256) void dense_pack(const uint16_t* __restrict__ p
 }
 
 // ------------------------------------------------------------------------------------------------- host side
-// The modelled time of a product in us, fitted to 2,240 measurements (30 shapes of 20-16384 rows, 64-13824 columns and K
-// 256-16384, every tiling, 1-16 slices, both orders of the operands; typically 5-10 % off): a workgroup takes `fixed` and
-// `stage` for each 64 values of K on a CU of its own, `shared` where `per_cu` of them share one; operands stream at 5 TB/s,
-// less with few workgroups; a second kernel adds the slices. Choosing by it stays within 5 % of the best measured way on
-// 21 of the shapes and within 13 % on all but one (600 x 800 x 13000: 61 against 46 us).
+// The modelled time of a product in us, fitted to 2,230 measurements (30 shapes of 20-16384 rows, 64-13824 columns and K
+// 256-16384, every tiling, 1-16 slices, operands along and across K): a workgroup takes `fixed` and `stage` for each 64
+// values of K on a CU of its own, `shared` where `per_cu` of them share one; a last round that fills part of the chip runs
+// faster than a whole one, which the power limit holds back; operands stream at 4.6 TB/s, less with few workgroups; a second
+// kernel adds the slices. The way it chooses took 3 % longer than the best measured one on average over the 60 (shape,
+// order) pairs, at most 17 % (304 x 304 x 8192, 18 against 15 us).
 struct DenseTiling {
     int bm, bn, per_cu;
     float fixed, stage, shared;
 };
-constexpr DenseTiling kDense[] = {{256, 320, 1, 6.36f, 1.443f, 1.443f}, {256, 256, 1, 3.72f, 1.281f, 1.281f},
-                                  {256, 192, 1, 3.12f, 1.124f, 1.124f}, {128, 160, 2, 4.02f, 0.722f, 0.582f},
-                                  {128, 128, 2, 2.66f, 0.647f, 0.511f}, {64, 128, 3, 1.77f, 0.499f, 0.376f},
-                                  {32, 128, 3, 2.06f, 0.428f, 0.326f}};
-constexpr float kDenseLaunch = 4.7f;
+constexpr DenseTiling kDense[] = {{256, 320, 1, 2.2f, 1.65f, 1.65f},    {256, 256, 1, 3.0f, 1.252f, 1.252f},
+                                  {256, 192, 1, 1.8f, 1.076f, 1.076f},  {128, 192, 2, 0.8f, 0.785f, 0.694f},
+                                  {128, 160, 2, 1.6f, 0.72f, 0.606f},   {128, 128, 2, 1.5f, 0.634f, 0.519f},
+                                  {64, 128, 3, 0.8f, 0.47f, 0.367f},    {32, 128, 3, 1.6f, 0.435f, 0.315f}};
 
 static DensePlan dense_plan_tiles(int64_t M, int64_t N, int64_t K, float& us) {
     const int64_t stages = (K + 63) / 64;
@@ -119,11 +119,12 @@ static DensePlan dense_plan_tiles(int64_t M, int64_t N, int64_t K, float& us) {
                 const float more = q.per_cu > 1 ? (q.shared * q.per_cu - q.stage) * (n - 1) / (q.per_cu - 1) : 0.0f;
                 return q.fixed + (float)per * (q.stage + more);
             };
-            const float busy = (float)full * together(q.per_cu) + together(rest);
-            const float mem = bytes / 5.0e6f * (1.0f + 0.232f * 256.0f / (float)wgs);
+            float busy = (float)full * together(q.per_cu) + together(rest);
+            if (on > q.per_cu && want == 1) busy *= 0.5f + 0.5f * (float)wgs / (256.0f * (float)on);
+            const float mem = bytes / 4.6e6f * (1.0f + 0.12f * 256.0f / (float)wgs);
             const float hi = std::max(busy, mem), r = std::min(busy, mem) / hi;
-            float c = kDenseLaunch + hi * (1.0f + 0.26f * r * r * r);
-            if (want > 1) c += 1.64e-6f * (float)(M * N) * (float)(slices + 1);
+            float c = 4.4f + hi * (1.0f + 0.26f * r * r * r);
+            if (want > 1) c += 1.3f + 1.5e-6f * (float)(M * N) * (float)(slices + 1);
             if (c < us) us = c, best = {t, (int)slices, (int)per};
         }
     }

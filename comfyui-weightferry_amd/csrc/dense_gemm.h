@@ -39,7 +39,7 @@ __device__ __forceinline__ DenseTile dense_tile(const DenseOperand& o, int r0) {
 // Workgroup (tile, slice). parts: [slices, M, N] float32 partial sums, or NULL: one slice, and the outputs. PLAIN: the
 // epilogue is at most a bias.
 template <int D, bool AX, bool BX, bool PLAIN, typename S>
-__global__ __launch_bounds__(S::NT) void dense_gemm(DenseOperand a, DenseOperand b, int M, int N, int K, int slice_stages,
+__global__ __launch_bounds__(S::NT, S::WAVES) void dense_gemm(DenseOperand a, DenseOperand b, int M, int N, int K, int slice_stages,
                                                     float* __restrict__ parts, DenseEpilogue e) {
     constexpr int WM = S::WM, WN = S::WN, TC = WN * 32;
     __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS];
@@ -215,11 +215,12 @@ static void dense_tiling(const DenseOperand& a, const DenseOperand& b, int M, in
                          const DenseEpilogue& e, hipStream_t s) {
     switch (p.tiling) {
     case 0: dense_launch<D, AX, BX, PLAIN, 4, 2, 2, 5>(a, b, M, N, K, p, parts, e, s); break;
-    case 1: dense_launch<D, AX, BX, PLAIN, 2, 4, 4, 2>(a, b, M, N, K, p, parts, e, s); break;
-    case 2: dense_launch<D, AX, BX, PLAIN, 4, 2, 2, 3>(a, b, M, N, K, p, parts, e, s); break;
-    case 3: dense_launch<D, AX, BX, PLAIN, 4, 1, 1, 5>(a, b, M, N, K, p, parts, e, s); break;
-    case 4: dense_launch<D, AX, BX, PLAIN, 2, 2, 2, 2>(a, b, M, N, K, p, parts, e, s); break;
-    case 5: dense_launch<D, AX, BX, PLAIN, 1, 4, 2, 1>(a, b, M, N, K, p, parts, e, s); break;
+    case 1: dense_launch<D, AX, BX, PLAIN, 2, 2, 4, 4>(a, b, M, N, K, p, parts, e, s); break;
+    case 2: dense_launch<D, AX, BX, PLAIN, 2, 2, 4, 3>(a, b, M, N, K, p, parts, e, s); break;
+    case 3: dense_launch<D, AX, BX, PLAIN, 2, 2, 2, 3>(a, b, M, N, K, p, parts, e, s); break;
+    case 4: dense_launch<D, AX, BX, PLAIN, 4, 1, 1, 5>(a, b, M, N, K, p, parts, e, s); break;
+    case 5: dense_launch<D, AX, BX, PLAIN, 2, 2, 2, 2>(a, b, M, N, K, p, parts, e, s); break;
+    case 6: dense_launch<D, AX, BX, PLAIN, 1, 4, 2, 1>(a, b, M, N, K, p, parts, e, s); break;
     default: dense_launch<D, AX, BX, PLAIN, 1, 4, 1, 1>(a, b, M, N, K, p, parts, e, s); break;
     }
 }

@@ -1,8 +1,21 @@
-// Main loop of the 16-bit linear's GEMM (dense_gemm.h): C[BM x BN] += A[BM rows, K] . B[BN rows, K]^T through the two LDS
-// stage buffers and the barrier discipline of wl_ring.h -- a stage is 64 values of K of every row, loaded global -> LDS;
-// stage p + 1 flies while stage p is computed; one barrier a stage, before its last K step's MFMAs, behind which the
-// loads of stage p + 2 and the first fragment reads of stage p + 1 go out between those MFMAs. What differs: each operand
-// lies in memory one of two ways, with a row length of its own, and K need not be whole stages.
+// Main loop of the 16-bit linear's GEMM (dense_gemm.h): C[BM x BN] += A[BM rows, K] . B[BN rows, K]^T through two LDS stage
+// buffers -- a stage is 64 values of K of every row, four K steps of the MFMA, loaded global -> LDS; stage p + 1 flies while
+// stage p is computed.
+//
+// Eight waves (256 x 320): the barrier discipline of wl_ring.h, one barrier a stage, before its last K step's MFMAs, behind
+// which the loads of stage p + 2 and the first fragment reads of stage p + 1 go out between those MFMAs.
+//
+// Four waves, one a SIMD with twice the registers: larger wave tiles read fewer bytes of LDS a MFMA (128 x 128: 8 fragments
+// for 16 MFMAs, against 7 for 10 of 64 x 160), but a lone wave's MFMAs stop whenever it does, and 16 loads behind one K step
+// queue up at the load unit, which takes as long for a stage's loads as the matrix unit for half the stage. So the
+// fragments of a whole stage are in registers (four sets): step 0 multiplies and reads steps 2 and 3; behind a barrier the
+// buffer is free, and the loads of stage p + 2 spread over steps 1 to 3; a second barrier behind step 1 certifies stage p +
+// 1, whose steps 0 and 1 are read during steps 2 and 3. us, eight waves by one barrier / four waves by one / by two: 8192 x
+// 8192 x 8192 in 256 x 256 tiles 841 / 831 / 763; 1560 x 13824 x 5120 in 256 x 192 tiles 220 / - / 197; 2048 x 5120 x 5120
+// 118 / - / 85.
+//
+// What differs from wl_ring.h besides: each operand lies in memory one of two ways, with a row length of its own, and K need
+// not be whole stages.
 //
 // Along K (DenseAlong): a row's K values are consecutive. A 1 KiB load covers 8 rows of a stage's 128 bytes; the chunks of
 // the last stage that lie past K load zeros. Across K (DenseAcross): value (r, k) is at k * row + r -- the operands of a
@@ -24,8 +37,10 @@ struct DenseShape {
     static constexpr int VM = VM_, VN = VN_, WM = WM_, WN = WN_;
     static constexpr int NT = 64 * VM * VN, NW = NT / 64;
     static constexpr int BM = VM * WM * 32, BN = VN * WN * 32;
+    static constexpr bool DEEP = NW == 4;                         // four sets of fragments and two barriers a stage
     static constexpr int AW = BM / 8 / NW, BW = BN / 8 / NW;      // 1 KiB loads of each operand a wave and stage
     static constexpr int ASLOTS = BM * 8, SLOTS = (BM + BN) * 8;  // 16-byte slots of a stage buffer, A's first
+    static constexpr int WAVES = DEEP ? (160 * 1024) / (2 * SLOTS * 16) : 2;   // a SIMD, as many as LDS lets share a CU
     static_assert(AW * NW * 8 == BM && BW * NW * 8 == BN, "whole loads for every wave");
     static_assert(2 * SLOTS * 16 <= 160 * 1024, "two stage buffers fit the LDS");
 };
@@ -140,30 +155,41 @@ __device__ __forceinline__ void dense_mainloop(const DenseTile& ta, const DenseT
         if constexpr (q < AW) a.template load<q>(st, wave, kt);
         else b.template load<q - AW>(st + S::ASLOTS, wave, kt);
     };
-    wl_frag fa[2][WM], fb[2][WN];
+    constexpr int SETS = S::DEEP ? 4 : 2;
+    wl_frag fa[SETS][WM], fb[SETS][WN];
     auto fread = [&](const wl_frag* st, int ks, int set, auto rc) {    // read rc of a K step: a0, the b's, the other a's
         constexpr int r = decltype(rc)::value;
         if constexpr (r == 0) fa[set][0] = a.template read<0>(st, ks);
         else if constexpr (r <= WN) fb[set][r - 1] = b.template read<r - 1>(st + S::ASLOTS, ks);
         else fa[set][r - WN] = a.template read<r - WN>(st, ks);
     };
-    auto kstep = [&](auto load, int set, const wl_frag* st, int ks, wl_frag* free_, int kt) {
+    // The MFMAs of `set`, between them NR steps' fragment reads -- K step ks of st into set rs, then ks + 1 into rs + 1 -- and
+    // the loads [L0, L1) of stage kt into `free_`. Two steps' reads are done by three quarters of the MFMAs, so that none
+    // is waited for at the barrier behind them.
+    auto kstep = [&](auto nr, auto l0, auto l1, int set, const wl_frag* st, int ks, int rs, wl_frag* free_, int kt) {
+        constexpr int NR = decltype(nr)::value * READS, L0 = decltype(l0)::value, L = decltype(l1)::value - L0;
+        constexpr int OVER = decltype(nr)::value == 2 && MFMAS > 4 ? MFMAS * 3 / 4 : MFMAS;
         static_for<MFMAS>([&](auto mc) {
             constexpr int m = decltype(mc)::value;
             acc[m / WN][m % WN] = mma(acc[m / WN][m % WN], fa[set][m / WN], fb[set][m % WN]);
-            constexpr int r0 = m * READS / MFMAS, r1 = (m + 1) * READS / MFMAS;
+            constexpr int r0 = m < OVER ? m * NR / OVER : NR, r1 = m + 1 < OVER ? (m + 1) * NR / OVER : NR;
             static_for<r1 - r0>([&](auto x) {
-                fread(st, ks, set ^ 1, std::integral_constant<int, r0 + decltype(x)::value>{});
+                constexpr int r = r0 + decltype(x)::value;
+                fread(st, ks + r / READS, rs + r / READS, std::integral_constant<int, r % READS>{});
             });
-            if constexpr (decltype(load)::value) {
-                constexpr int q0 = m * IPW / MFMAS, q1 = (m + 1) * IPW / MFMAS;
-                static_for<q1 - q0>([&](auto x) {
-                    issue(free_, kt, std::integral_constant<int, q0 + decltype(x)::value>{});
-                });
-            }
+            constexpr int q0 = L0 + m * L / MFMAS, q1 = L0 + (m + 1) * L / MFMAS;
+            static_for<q1 - q0>([&](auto x) {
+                issue(free_, kt, std::integral_constant<int, q0 + decltype(x)::value>{});
+            });
             __builtin_amdgcn_sched_barrier(0);
         });
     };
+    constexpr std::integral_constant<int, 0> none{};
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, IPW / 3> third{};
+    constexpr std::integral_constant<int, 2 * IPW / 3> thirds{};
+    constexpr std::integral_constant<int, IPW> all{};
     auto begin = [&](int kt) {
         a.begin(kt);
         b.begin(kt);
@@ -175,15 +201,29 @@ __device__ __forceinline__ void dense_mainloop(const DenseTile& ta, const DenseT
     wait_vm<IPW>();                                      // the first stage landed; the second may be in flight
     wave_barrier_sync();
     static_for<READS>([&](auto rc) { fread(sb0, 0, 0, rc); });
+    if constexpr (S::DEEP) static_for<READS>([&](auto rc) { fread(sb0, 1, 1, rc); });
+    // stage p in cur (its first fragments already read), stage p + 1 flying into oth
     auto step = [&](int p, wl_frag* cur, wl_frag* oth) {
-        kstep(std::false_type{}, 0, cur, 1, nullptr, 0);
-        kstep(std::false_type{}, 1, cur, 2, nullptr, 0);
-        kstep(std::false_type{}, 0, cur, 3, nullptr, 0);
-        begin(p + 2);
-        wait_vm<0>();                                    // stage p + 1 landed (this wave's loads)
-        __builtin_amdgcn_s_waitcnt(0xc07f);              // lgkmcnt(0): this wave's reads of cur are done
-        wave_barrier_sync();                             // ... and every wave's: cur is free, p + 1 is whole
-        kstep(std::true_type{}, 1, oth, 0, cur, p + 2);
+        if constexpr (S::DEEP) {
+            kstep(two, none, none, 0, cur, 2, 2, nullptr, 0);
+            begin(p + 2);
+            __builtin_amdgcn_s_waitcnt(0xc07f);          // lgkmcnt(0): this wave's reads of cur are done
+            wave_barrier_sync();                         // ... and every wave's: cur is free
+            kstep(none, none, third, 1, nullptr, 0, 0, cur, p + 2);
+            wait_vm<IPW / 3>();                          // stage p + 1 landed (this wave's loads, all but the newest)
+            wave_barrier_sync();                         // ... and every wave's: p + 1 is whole
+            kstep(one, third, thirds, 2, oth, 0, 0, cur, p + 2);
+            kstep(one, thirds, all, 3, oth, 1, 1, cur, p + 2);
+        } else {
+            kstep(one, none, none, 0, cur, 1, 1, nullptr, 0);
+            kstep(one, none, none, 1, cur, 2, 0, nullptr, 0);
+            kstep(one, none, none, 0, cur, 3, 1, nullptr, 0);
+            begin(p + 2);
+            wait_vm<0>();                                // stage p + 1 landed (this wave's loads)
+            __builtin_amdgcn_s_waitcnt(0xc07f);
+            wave_barrier_sync();                         // cur is free, p + 1 is whole
+            kstep(one, none, all, 1, oth, 0, 0, cur, p + 2);
+        }
     };
     int p = 0;
     for (; p + 2 <= nk; p += 2) {
