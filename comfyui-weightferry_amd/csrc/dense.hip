@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void dense_pack(const uint16_t* __restrict__ p
 // values of K on a CU of its own, `shared` where `per_cu` of them share one; a last round that fills part of the chip runs
 // faster than a whole one, which the power limit holds back; operands stream at 4.6 TB/s, less with few workgroups; a second
 // kernel adds the slices. The way it chooses took 3 % longer than the best measured one on average over the 60 (shape,
-// order) pairs, at most 17 % (304 x 304 x 8192, 18 against 15 us).
+// order) pairs, at most 21 % (2048 x 2048 x 256, 8.0 against 6.6 us).
 struct DenseTiling {
     int bm, bn, per_cu;
     float fixed, stage, shared;
@@ -100,7 +100,17 @@ constexpr DenseTiling kDense[] = {{256, 320, 1, 2.2f, 1.65f, 1.65f},    {256, 25
                                   {128, 160, 2, 1.6f, 0.72f, 0.606f},   {128, 128, 2, 1.5f, 0.634f, 0.519f},
                                   {64, 128, 3, 0.8f, 0.47f, 0.367f},    {32, 128, 3, 1.6f, 0.435f, 0.315f}};
 
-static DensePlan dense_plan_tiles(int64_t M, int64_t N, int64_t K, float& us) {
+// What an epilogue adds to a workgroup's time: an activation's arithmetic, the kept pre-activations' stores, the residual's
+// loads. Eight waves hide more of it than four, and workgroups that share a CU hide each other's: 4096 x 13824 x 5120 with
+// GELU 465 us in 256 x 320 tiles, 486 in 256 x 256, which without it are as fast.
+enum { EPI_ACT = 1, EPI_KEEP = 2, EPI_MORE = 4 };
+static float dense_epilogue_time(const DenseTiling& q, int epilogue) {
+    const float us = (epilogue & EPI_ACT ? 5.0f : 0.0f) + (epilogue & EPI_KEEP ? 10.0f : 0.0f) +
+                     (epilogue & EPI_MORE ? 8.0f : 0.0f);
+    return us * (float)(q.bm * q.bn) / 65536.0f * (q.bn == 320 ? 0.5f : q.per_cu > 1 ? 0.75f : 1.0f);
+}
+
+static DensePlan dense_plan_tiles(int64_t M, int64_t N, int64_t K, int epilogue, float& us) {
     const int64_t stages = (K + 63) / 64;
     DensePlan best = {0, 1, (int)stages};
     us = 1e30f;
@@ -114,13 +124,14 @@ static DensePlan dense_plan_tiles(int64_t M, int64_t N, int64_t K, float& us) {
             // workgroups of the busiest CU: full rounds of per_cu together, then a rest
             const int64_t wgs = tiles * slices, on = (wgs + 255) / 256, full = on / q.per_cu;
             const int rest = (int)(on % q.per_cu);
+            const float after = want == 1 ? dense_epilogue_time(q, epilogue) : 0.0f;
             auto together = [&](int n) {
                 if (n == 0) return 0.0f;
                 const float more = q.per_cu > 1 ? (q.shared * q.per_cu - q.stage) * (n - 1) / (q.per_cu - 1) : 0.0f;
-                return q.fixed + (float)per * (q.stage + more);
+                return q.fixed + after + (float)per * (q.stage + more);
             };
             float busy = (float)full * together(q.per_cu) + together(rest);
-            if (on > q.per_cu && want == 1) busy *= 0.5f + 0.5f * (float)wgs / (256.0f * (float)on);
+            if (on > q.per_cu && want == 1) busy *= 0.65f + 0.35f * (float)wgs / (256.0f * (float)on);
             const float mem = bytes / 4.6e6f * (1.0f + 0.12f * 256.0f / (float)wgs);
             const float hi = std::max(busy, mem), r = std::min(busy, mem) / hi;
             float c = 4.4f + hi * (1.0f + 0.26f * r * r * r);
@@ -188,17 +199,17 @@ struct DenseCall {
     DenseRowsPlan rows;
     DensePlan tiles;
     int how_x, how_w;
-    bool plain;                                       // the epilogue is at most a bias
+    int epilogue;                                     // 0: at most a bias
     bool summed;                                      // float32 partial sums first: slices, or operands across K with more
     int64_t w_at, parts_at, bytes;                    // than a plain epilogue. Offsets into the workspace, x's copy first
     int slices() const { return few ? rows.slices : tiles.slices; }
 };
 
-static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, int64_t N, int64_t K, bool plain) {
+static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, int64_t N, int64_t K, int epilogue) {
     DenseCall d = {};
-    d.plain = plain;
+    d.epilogue = epilogue;
     float us;
-    d.tiles = dense_plan_tiles(M, N, K, us);
+    d.tiles = dense_plan_tiles(M, N, K, epilogue, us);
     d.how_w = dense_how(w, N, K, true);
     d.how_x = dense_how(x, M, K, is_across(d.how_w));
     int64_t copies = dense_copy_bytes(d.how_x, M, K);
@@ -212,7 +223,7 @@ static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, i
         d.w_at = dense_copy_bytes(d.how_x, M, K);
     }
     d.parts_at = copies;
-    d.summed = d.slices() > 1 || (!d.few && !plain && is_across(d.how_w));
+    d.summed = d.slices() > 1 || (!d.few && epilogue && is_across(d.how_w));
     d.bytes = d.parts_at + (d.summed ? (int64_t)d.slices() * M * N * 4 : 0);
     return d;
 }
@@ -247,7 +258,7 @@ static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w
     } else {
         const DenseOperand a = dense_operand(x, d.how_x, M, K, reinterpret_cast<uint16_t*>(ws), s);
         const DenseOperand b = dense_operand(w, d.how_w, N, K, reinterpret_cast<uint16_t*>(ws + d.w_at), s);
-        auto run = a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : d.plain || parts ? dense_gemm_along : dense_gemm_along_full;
+        auto run = a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : !d.epilogue || parts ? dense_gemm_along : dense_gemm_along_full;
         run(dt, a, b, (int)M, (int)N, (int)K, d.tiles, parts, e, s);
     }
     if (d.summed) {
@@ -278,8 +289,8 @@ static DenseBackward dense_backward(const void* x, int64_t x_row, const void* w,
     b.w_turned = {w, w_col, w_row, false};
     b.dh_turned = {dh, 1, b.dh_row, false};
     b.x_turned = {x, 1, x_row, false};
-    if (dx) b.dx = dense_call(b.dh_along, b.w_turned, M, K, N, true);
-    if (dw) b.dw = dense_call(b.dh_turned, b.x_turned, N, K, M, true);
+    if (dx) b.dx = dense_call(b.dh_along, b.w_turned, M, K, N, 0);
+    if (dw) b.dw = dense_call(b.dh_turned, b.x_turned, N, K, M, 0);
     b.bytes = b.product_at + std::max(b.dx.bytes, b.dw.bytes);
     return b;
 }
@@ -304,11 +315,11 @@ static int dense_check(const char* who, int dt, int64_t M, int64_t N, int64_t K,
 }  // namespace wf
 
 extern "C" int wf_dense_workspace(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col,
-                                  int dt, int64_t M, int64_t N, int64_t K, int plain, int64_t* bytes) {
+                                  int dt, int64_t M, int64_t N, int64_t K, int epilogue, int64_t* bytes) {
     using namespace wf;
-    if (!bytes) { set_error("wf_dense_workspace: null pointer"); return WF_EINVAL; }
+    if (!bytes || epilogue < 0 || epilogue > 7) { set_error("wf_dense_workspace: null pointer or epilogue %d", epilogue); return WF_EINVAL; }
     if (const int rc = dense_check("wf_dense_workspace", dt, M, N, K, x_row, x_col, w_row, w_col)) return rc;
-    *bytes = M && N ? dense_call({x, x_row, x_col, false}, {w, w_row, w_col, false}, M, N, K, plain).bytes : 0;
+    *bytes = M && N ? dense_call({x, x_row, x_col, false}, {w, w_row, w_col, false}, M, N, K, epilogue).bytes : 0;
     return WF_OK;
 }
 
@@ -332,7 +343,8 @@ extern "C" int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void*
         return WF_EINVAL;
     }
     const DenseView xv = {x, x_row, x_col, false}, wv = {w, w_row, w_col, false};
-    const DenseCall d = dense_call(xv, wv, M, N, K, act == ACT_NONE && !gate && !resid && !h);
+    const int epilogue = (act != ACT_NONE ? EPI_ACT : 0) | (h ? EPI_KEEP : 0) | (gate || resid ? EPI_MORE : 0);
+    const DenseCall d = dense_call(xv, wv, M, N, K, epilogue);
     if (d.bytes && (!workspace || workspace_bytes < d.bytes || !aligned(workspace, 256))) {
         set_error("wf_dense: a workspace of %lld bytes is required", (long long)d.bytes);
         return WF_EINVAL;

@@ -49,8 +49,8 @@ def _launch(x2, w, b, code, act, resid, gate, groups, keep):
     if rows and n:
         xp, wp, xr = x2.data_ptr(), w.data_ptr(), x2.stride(0)
         w_row, w_col = w.stride()
-        plain_ = 1 if act == 0 and gate is None and resid is None and h is None else 0
-        need = _bytes((xp & 15, xr, 1, wp & 15, w_row, w_col, code, rows, n, k, plain_))
+        epilogue = (1 if act else 0) | (2 if keep else 0) | (0 if gate is None and resid is None else 4)
+        need = _bytes((xp & 15, xr, 1, wp & 15, w_row, w_col, code, rows, n, k, epilogue))
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         with _native.on_device(dev):
             rc = _native.lib().wf_dense(xp, xr, 1, wp, w_row, w_col, code, rows, n, k, ptr(b),

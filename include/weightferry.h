@@ -195,12 +195,12 @@ int wf_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldd, i
  * NULL; bias and gate have type dt or WF_F32 (bias_dt, gate_dt). An operand's value (r, k) is at r * row + k * col, so
  * transposed views need no copy by the caller; resid's rows are resid_row values apart; y is [M, N]. h (may be NULL): the
  * sums with the bias, [M, N] of type dt, what wf_dense_grad reads (float16: kept finite). M, N <= 2^24, K <= 2^20.
- * The workspace (256-byte aligned, at least the bytes that wf_dense_workspace gives for the same operands; plain: whether
- * act is 0 and gate, resid and h are NULL) holds copies of
- * operands that cannot be loaded as they are, and the partial sums of products that run in slices of K; it need not be
+ * The workspace (256-byte aligned, at least the bytes that wf_dense_workspace gives for the same operands; epilogue: 1 with an
+ * activation, + 2 where h is kept, + 4 with a gate or resid) holds copies of operands that cannot be loaded as they are, and
+ * the partial sums of products that run in slices of K; it need not be
  * cleared and is free again when the call's work on the stream is done. */
 int wf_dense_workspace(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt,
-                       int64_t M, int64_t N, int64_t K, int plain, int64_t* bytes);
+                       int64_t M, int64_t N, int64_t K, int epilogue, int64_t* bytes);
 int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt, int64_t M,
              int64_t N, int64_t K, const void* bias, int bias_dt, int act, const void* gate, int gate_dt,
              int64_t rows_per_group, const void* resid, int64_t resid_row, void* y, void* h, void* workspace,

@@ -56,18 +56,19 @@ def test_dense_argument_checks():
     assert dense(M=0) == native.OK and dense(N=0) == native.OK
     # a product that runs in slices asks for its workspace
     need = ctypes.c_int64()
-    assert lib.wf_dense_workspace(p, 5120, 1, p, 5120, 1, 1, 256, 5120, 5120, 1, ctypes.byref(need)) == native.OK
+    assert lib.wf_dense_workspace(p, 5120, 1, p, 5120, 1, 1, 256, 5120, 5120, 0, ctypes.byref(need)) == native.OK
     assert need.value > 0 and need.value % (256 * 5120 * 4) == 0
     assert dense(xr=5120, wr=5120, M=256, N=5120, K=5120) == native.EINVAL and "workspace" in native.last_error()
     # whole tiles for the chip: none; an odd row: its operand's copy
-    assert lib.wf_dense_workspace(p, 5120, 1, p, 5120, 1, 1, 4096, 5120, 5120, 1, ctypes.byref(need)) == native.OK
+    assert lib.wf_dense_workspace(p, 5120, 1, p, 5120, 1, 1, 4096, 5120, 5120, 0, ctypes.byref(need)) == native.OK
     assert need.value == 0
-    assert lib.wf_dense_workspace(p, 5121, 1, p, 5120, 1, 1, 4096, 5120, 5120, 1, ctypes.byref(need)) == native.OK
+    assert lib.wf_dense_workspace(p, 5121, 1, p, 5120, 1, 1, 4096, 5120, 5120, 0, ctypes.byref(need)) == native.OK
     assert need.value == 4096 * 5120 * 2
     # across K both operands are read as they lie; a fuller epilogue then goes through float32 sums
     across = (p, 1, 4096, p, 1, 5120, 1, 4096, 5120, 5120)
-    assert lib.wf_dense_workspace(*across, 1, ctypes.byref(need)) == native.OK and need.value == 0
-    assert lib.wf_dense_workspace(*across, 0, ctypes.byref(need)) == native.OK and need.value == 4096 * 5120 * 4
+    assert lib.wf_dense_workspace(*across, 0, ctypes.byref(need)) == native.OK and need.value == 0
+    assert lib.wf_dense_workspace(*across, 1, ctypes.byref(need)) == native.OK and need.value == 4096 * 5120 * 4
+    assert lib.wf_dense_workspace(*across, 8, ctypes.byref(need)) == native.EINVAL
 
     def bwd(M=4, N=8, K=64, act=0, gate=None, h=None, dy=p, dx=None, dw=None, db=None, dg=None, ws=None, n=0, rpg=4, dt=1):
         return lib.wf_dense_bwd(p, 64, p, 64, 1, dy, 8, h, dt, act, gate, 1, rpg, M, N, K, dx, dw, db, 1, dg, ws, n, None)
