@@ -6,7 +6,8 @@ At import it installs the GGUF dequantisation patch when ComfyUI-GGUF is loaded,
 name (__init__.py:104-132).
 
 Sub-modules (the reference's names): enhancers.gguf_dequant, enhancers.fused_int8, enhancers.int8_block,
-enhancers.fused_state, enhancers.fused_gguf (dequant + GEMM in one kernel), streaming.{common,state,profiler,
+enhancers.fused_state, enhancers.fused_gguf (dequant + GEMM in one kernel), enhancers.{fused_norm,fused_dense,
+fused_adamw} (a training step's operators; examples.finetune_mlp runs them together), streaming.{common,state,profiler,
 load_steps,dit_node,node}, core.tiers.{pinned,sources,plan,gguf_file}, core.env, utils.logging; the kernels live in
 lib/libweightferry_hip.so
 (csrc/, C ABI in include/weightferry.h).
