@@ -12,8 +12,10 @@ _grad_enabled = torch.is_grad_enabled
 
 
 def plain(device, *tensors):
-    """Whether each of ``tensors`` is None or an ordinary tensor on ``device``."""
-    deep = _level() is not None or forward_ad._current_level >= 0    # functorch or forward mode is at work somewhere
+    """Whether each of ``tensors`` is None or an ordinary tensor on ``device``, outside functorch's transforms."""
+    if _level() is not None:
+        return False
+    deep = forward_ad._current_level >= 0                            # forward mode is at work somewhere
     for t in tensors:
         if t is None:
             continue

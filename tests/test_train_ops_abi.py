@@ -107,3 +107,18 @@ def test_cpu_tensors_are_not_the_kernels_case():
     fa = sub("enhancers.fused_adamw")
     with pytest.raises(ValueError, match="GPU"):
         fa.adamw_step([x], [x.clone()], fa.adamw_state([x]), 1)
+
+
+def test_transformed_tensors_are_not_the_kernels_case():
+    ops = sub("enhancers.operands")
+    x = torch.randn(3, 4)
+    seen = []
+    torch.func.vmap(lambda t: seen.append(ops.plain(t.device, t)) or t)(x)
+    torch.func.grad(lambda t: seen.append(ops.plain(x.device, x)) or t.sum())(x)      # a bystander inside a transform
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        seen += [ops.plain(x.device, dual), not ops.plain(x.device, x)]
+    seen += [ops.plain(x.device, torch.nn.Buffer(x) if hasattr(torch.nn, "Buffer") and type(torch.nn.Buffer(x)) is not
+                       torch.Tensor else torch._neg_view(x)), ops.plain(torch.device("meta"), x)]
+    assert seen == [False] * len(seen) and len(seen) == 6
+    assert ops.plain(x.device, x, None, torch.nn.Parameter(x))
