@@ -51,18 +51,25 @@ __global__ __launch_bounds__(256) void dense_sum(const float* __restrict__ parts
     epilogue_run<D, true>(e, v, r, m, n, N, cnt);
 }
 
-// rows of K consecutive values (of an operand, or of memory where it lies across K) as [R, KP], KP a multiple of 8, zeros
-// past K: a run of 8 values a thread, loaded at any alignment
-__global__ __launch_bounds__(256) void dense_pack_rows(const uint16_t* __restrict__ p, int64_t row, int R, int K, int KP,
-                                                       uint16_t* __restrict__ out) {
-    const int runs = KP / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / runs;
-    if (r >= R) return;
-    const int k = (int)(i - r * runs) * 8;
+// R rows of K consecutive values (of an operand, or of memory where it lies across K), `row` apart, as [R, KP], KP a multiple
+// of 8, zeros past K: a run of 8 values a thread, loaded at any alignment. One launch copies both operands (blockIdx.y).
+struct PackRows {
+    const uint16_t* p;
+    uint16_t* out;
+    int64_t row, runs;                                             // runs: R KP / 8
+    int K, KP;
+};
+__global__ __launch_bounds__(256) void dense_pack_rows(PackRows a, PackRows b) {
+    const PackRows q = blockIdx.y ? b : a;
+    const int across = q.KP / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= q.runs) return;
+    const int64_t r = i / across;
+    const int k = (int)(i - r * across) * 8;
     Pack<WF_BF16> v;                                               // (16 bits are moved, whatever they stand for)
     v.zero();
-    if (k < K) v.load(p + r * row + k, K - k);
-    v.store(out + r * KP + k, 8);
+    if (k < q.K) v.load(q.p + r * q.row + k, q.K - k);
+    v.store(q.out + r * q.KP + k, 8);
 }
 
 // an operand of any strides (value (r, k) at r row + k col) as such rows, KP a multiple of 64: 64 x 64 tiles through LDS, read along
@@ -228,12 +235,13 @@ static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, i
     return d;
 }
 
-// the operand as the tiles load it, copied to `out` where it has to be
-static DenseOperand dense_operand(const DenseView& v, int how, int64_t R, int64_t K, uint16_t* out, hipStream_t s) {
+// the operand as the tiles load it; where it has to be copied, to `out`: rows by the job that is filled in, others at once
+static DenseOperand dense_operand(const DenseView& v, int how, int64_t R, int64_t K, uint16_t* out, PackRows& job,
+                                  hipStream_t s) {
     const uint16_t* p = static_cast<const uint16_t*>(v.p);
     const int64_t to = dense_copy_row(how, R, K);
     auto pack_rows = [&](int64_t row, int64_t n, int64_t values) {
-        dense_pack_rows<<<dim3((uint32_t)((n * (to / 8) + 255) / 256)), 256, 0, s>>>(p, row, (int)n, (int)values, (int)to, out);
+        job = {p, out, row, n * (to / 8), (int)values, (int)to};
     };
     switch (how) {
     case LIES_ALONG: return {p, v.row, (int)(v.zeros ? up(K, 8) : K), (int)R, false};
@@ -256,8 +264,12 @@ static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w
         dense_rows_run(dt, d.rows, static_cast<const uint16_t*>(x.p), x.row, static_cast<const uint16_t*>(w.p), w.row, (int)M,
                        (int)N, (int)K, parts, e, s);
     } else {
-        const DenseOperand a = dense_operand(x, d.how_x, M, K, reinterpret_cast<uint16_t*>(ws), s);
-        const DenseOperand b = dense_operand(w, d.how_w, N, K, reinterpret_cast<uint16_t*>(ws + d.w_at), s);
+        PackRows jx = {}, jw = {};
+        const DenseOperand a = dense_operand(x, d.how_x, M, K, reinterpret_cast<uint16_t*>(ws), jx, s);
+        const DenseOperand b = dense_operand(w, d.how_w, N, K, reinterpret_cast<uint16_t*>(ws + d.w_at), jw, s);
+        if (const int64_t runs = std::max(jx.runs, jw.runs))
+            dense_pack_rows<<<dim3((uint32_t)((runs + 255) / 256), jx.runs && jw.runs ? 2 : 1), 256, 0, s>>>(
+                jx.runs ? jx : jw, jw);
         auto run = a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : !d.epilogue || parts ? dense_gemm_along : dense_gemm_along_full;
         run(dt, a, b, (int)M, (int)N, (int)K, d.tiles, parts, e, s);
     }
