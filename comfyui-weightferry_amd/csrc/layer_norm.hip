@@ -271,26 +271,30 @@ struct LnShape {
     int waves, packs, teams, parts;      // a row's waves, a lane's packs, a workgroup's teams, workgroups a group of rows
 };
 // Two packs a lane, then more waves (up to 16); teams up to team_waves waves a workgroup, fewer where that would leave CUs
-// idle; wgs workgroups over all groups.
-static LnShape ln_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt, int team_waves, int wgs) {
+// idle; workgroups over all groups: as many a CU as make cu_waves waves of it, at most per_cu.
+static LnShape ln_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt, int team_waves, int cu_waves, int per_cu) {
     const int64_t lane = 64 * (dt == WF_F32 ? 4 : 8), packs = (K + lane - 1) / lane;   // of a lane, if the row had one wave
     LnShape s;
     s.waves = (int)std::min<int64_t>(16, (packs + 1) / 2);
     s.packs = (int)((packs + s.waves - 1) / s.waves);
-    s.teams = (int)std::max<int64_t>(1, std::min<int64_t>(team_waves / s.waves, M / wgs));
+    s.teams = (int)std::max<int64_t>(1, std::min<int64_t>(team_waves / s.waves, M / 256));
+    const int64_t wgs = 256 * std::max(1, std::min(per_cu, cu_waves / (s.waves * s.teams)));
     s.parts = (int)std::min<int64_t>((rows_per_group + s.teams - 1) / s.teams,
                                      std::max<int64_t>(1, wgs * rows_per_group / std::max<int64_t>(1, M)));
     return s;
 }
-// Forward: three workgroups of up to 8 waves a CU. us at 4096 x 5120 bfloat16 (84 MB), 256 / 512 / 768 / 1024 workgroups:
-// 24 / 21.8 / 19.6 / 22.8; one row a workgroup, without loading ahead, 31. 16384 x 5120 takes 64 us, 5.2 TB/s.
+// Forward: workgroups of up to 5 waves. us at 4096 x 5120 bfloat16 (84 MB; 5 waves a workgroup) with 2 / 3 / 4 a CU: 21.8 /
+// 19.6 / 22.8; one row a workgroup, without loading ahead, 31. 5152 x 2048 in workgroups of 4 waves 11.9, of 8 waves 16.4;
+// 3000 x 8192 float32 (16 waves) with one a CU 32.8, with three 35.6. 16384 x 5120 takes 64 us, 5.2 TB/s. Rows of one pack a
+// lane use half the registers: 30000 x 256 in three workgroups of 8 waves a CU 13.0, in three of 5 14.4.
 static LnShape ln_fwd_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt) {
-    return ln_shape(M, K, rows_per_group, dt, 8, 768);
+    return K <= 64 * (dt == WF_F32 ? 4 : 8) ? ln_shape(M, K, rows_per_group, dt, 8, 24, 3)
+                                            : ln_shape(M, K, rows_per_group, dt, 5, 16, 8);
 }
 // Backward: one workgroup of up to 16 waves a CU, since every workgroup writes a row of partial sums: 4096 x 5120 takes
 // 35.7 us with 256, 37.9 with 512 of half the teams, 42.4 with 512 whole ones. 16384 x 5120: 98 us, 5.2 TB/s.
 static LnShape ln_bwd_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt) {
-    return ln_shape(M, K, rows_per_group, dt, 16, 256);
+    return ln_shape(M, K, rows_per_group, dt, 16, 16, 1);
 }
 
 // f with a lane's packs as a constant: the next of 1, 2, 3, 4, 6, 8 (a row of 32768 values over 16 waves has 4, or 8 of
