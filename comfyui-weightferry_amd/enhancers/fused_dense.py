@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from .. import _native
-from .operands import CODES, Sizes, applier, groups_of, once, plain, ptr, rows_of, wants_grad, whole
+from .operands import CODES, Sizes, applier, gradient, groups_of, once, plain, ptr, rows_of, wants_grad, whole
 
 ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "relu": 4}
 MAX_ROWS, MAX_K = 1 << 24, 1 << 20
@@ -78,6 +78,7 @@ class _Dense(torch.autograd.Function):
 
     @once
     def backward(ctx, dy):
+        dy = gradient(dy)
         x2, w, h, gate = ctx.saved_tensors
         code, act, groups, shape, bias, gshape = ctx.how
         need_x, need_w, need_b, need_r, need_g = ctx.needs_input_grad[:5]

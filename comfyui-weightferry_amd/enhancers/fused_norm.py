@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from .. import _native
-from .operands import CODES, Sizes, applier, groups_of, once, plain, ptr, rows_of, wants_grad, whole
+from .operands import CODES, Sizes, applier, gradient, groups_of, once, plain, ptr, rows_of, wants_grad, whole
 
 MAX_WIDTH = 32768
 
@@ -53,6 +53,7 @@ class _LayerNorm(torch.autograd.Function):
 
     @once
     def backward(ctx, dy):
+        dy = gradient(dy)
         x2, w, stats = ctx.saved_tensors
         code, pcode, groups, modulation, shape, wshape, bshape = ctx.how
         need_x, need_w, need_b = ctx.needs_input_grad[:3]

@@ -26,6 +26,20 @@ def plain(device, *tensors):
     return True
 
 
+def gradient(dy):
+    """``dy``, the gradient that a backward pass is given, as its kernels read it. RuntimeError for one that is more than its
+    memory -- a forward-mode tangent, a functorch wrapper, a subclass with its own operations -- whose rest the pass would
+    lose in silence: the forward pass could not know of it."""
+    if dy.is_neg():
+        dy = dy.resolve_neg()
+    if type(dy) not in _TYPES and type(dy).__torch_dispatch__ is torch.Tensor.__torch_dispatch__:
+        dy = dy.as_subclass(torch.Tensor)                            # a subclass in name only
+    if not plain(dy.device, dy):
+        raise RuntimeError(f"a gradient that is no plain tensor ({type(dy).__name__}; or it carries a forward-mode tangent, or "
+                           "a functorch transform is at work): the backward pass of this operator takes values alone")
+    return dy
+
+
 def rows_of(t, width):
     """``t`` [..., width] as a matrix whose rows are runs of values, a view where its strides allow one."""
     t2 = t if t.dim() == 2 else t.reshape(-1, width)

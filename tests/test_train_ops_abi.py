@@ -122,3 +122,25 @@ def test_transformed_tensors_are_not_the_kernels_case():
                        torch.Tensor else torch._neg_view(x)), ops.plain(torch.device("meta"), x)]
     assert seen == [False] * len(seen) and len(seen) == 6
     assert ops.plain(x.device, x, None, torch.nn.Parameter(x))
+
+
+def test_gradients_that_are_more_than_memory_are_refused():
+    ops = sub("enhancers.operands")
+    x = torch.randn(3, 4)
+    assert ops.gradient(x) is x and torch.equal(ops.gradient(torch._neg_view(x)), -x)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        assert ops.gradient(x) is x
+        with pytest.raises(RuntimeError, match="gradient"):
+            ops.gradient(dual)
+    with pytest.raises(RuntimeError, match="gradient"):
+        torch.func.vmap(lambda t: ops.gradient(t))(x)
+    named = x.as_subclass(type("Named", (torch.Tensor,), {}))
+    assert type(ops.gradient(named)) is torch.Tensor and ops.gradient(named).data_ptr() == x.data_ptr()
+
+    class Own(torch.Tensor):
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return NotImplemented
+    with pytest.raises(RuntimeError, match="Own"):
+        ops.gradient(torch.Tensor._make_wrapper_subclass(Own, (3, 4)))
