@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _native
-from .operands import CODES
+from .operands import CODES, plain
 
 BLOCK = 256
 _TYPES = frozenset((torch.Tensor, torch.nn.Parameter))
@@ -108,6 +108,8 @@ def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8
     code = CODES.get(dt)
     if code is None or dev.type != "cuda":
         raise ValueError(f"parameters of type {dt} with moments on {dev}: float32, bfloat16 or float16 on a GPU")
+    if not plain(dev):
+        raise ValueError("a step inside a functorch transform or a trace, which would not see it")
     # (questions of all tensors at once: with hundreds of adapters they are the step's host time, 0.6 us a parameter; the numbers
     # of values are compared, not the shapes: that alone would be a third more)
     both, index, sizes = params + grads, dev.index, list(map(_numel, params))

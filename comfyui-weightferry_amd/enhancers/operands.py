@@ -1,6 +1,7 @@
 """What the training-step operators (fused_norm, fused_dense, fused_adamw) ask of their tensors. The kernels read memory,
 so tensors that are more than memory (subclasses, functorch wrappers, forward-mode duals, negative views) are not their
-case. These questions run once per call, so each is asked in its cheapest form."""
+case, and neither is a call that is being traced: a kernel launched through ctypes is no operation that a trace records.
+These questions run once per call, so each is asked in its cheapest form."""
 import torch
 from torch.autograd import forward_ad
 
@@ -9,11 +10,15 @@ _TYPES = frozenset((torch.Tensor, torch.nn.Parameter))
 _level = torch._C._functorch.maybe_current_level
 _wrapped = torch._C._functorch.is_functorch_wrapped_tensor
 _grad_enabled = torch.is_grad_enabled
+_jit_traces, _modes, _mode = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode
+_TRACERS = (torch._C._TorchDispatchModeKey.PROXY, torch._C._TorchDispatchModeKey.FAKE)
 
 
 def plain(device, *tensors):
-    """Whether each of ``tensors`` is None or an ordinary tensor on ``device``, outside functorch's transforms."""
-    if _level() is not None:
+    """Whether each of ``tensors`` is None or an ordinary tensor on ``device``, outside functorch's transforms and traces."""
+    if _level() is not None or _jit_traces():
+        return False
+    if _modes() and any(_mode(k) is not None for k in _TRACERS):    # proxies or fake tensors record what runs
         return False
     deep = forward_ad._current_level >= 0                            # forward mode is at work somewhere
     for t in tensors:
@@ -36,7 +41,7 @@ def gradient(dy):
         dy = dy.as_subclass(torch.Tensor)                            # a subclass in name only
     if not plain(dy.device, dy):
         raise RuntimeError(f"a gradient that is no plain tensor ({type(dy).__name__}; or it carries a forward-mode tangent, or "
-                           "a functorch transform is at work): the backward pass of this operator takes values alone")
+                           "a functorch transform or a trace is at work): the backward pass of this operator takes values alone")
     return dy
 
 

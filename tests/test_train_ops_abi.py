@@ -144,3 +144,20 @@ def test_gradients_that_are_more_than_memory_are_refused():
             return NotImplemented
     with pytest.raises(RuntimeError, match="Own"):
         ops.gradient(torch.Tensor._make_wrapper_subclass(Own, (3, 4)))
+
+
+def test_traces_are_not_the_kernels_case():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    ops = sub("enhancers.operands")
+    x, seen = torch.randn(3, 4), []
+
+    def ask(t):
+        seen.append(ops.plain(x.device, x))
+        return t * 2
+    torch.jit.trace(ask, (x,), check_trace=False)
+    make_fx(ask)(x)
+    make_fx(ask, tracing_mode="fake")(x)
+    assert seen == [False] * 3 and ops.plain(x.device, x)
+    from torch.utils.flop_counter import FlopCounterMode       # a mode that watches, but records no program
+    with FlopCounterMode(display=False):
+        assert ops.plain(x.device, x)
