@@ -14,14 +14,16 @@ enum { ACT_NONE = 0, ACT_GELU = 1, ACT_GELU_TANH = 2, ACT_SILU = 3, ACT_RELU = 4
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float rcp_of(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// The normal distribution function by formula 7.1.26 of Abramowitz and Stegun (|error| < 1e-7), on the side where it is
-// small, and e = exp(-h^2 / 2) that it needs on the way. exp2 and the reciprocal are the hardware's, one ulp: far below the
-// 16-bit outputs' rounding.
+// The normal distribution function on the side where it is small, and e = exp(-h^2 / 2) that it needs on the way: e times a
+// polynomial of 1 / (1 + 0.3 |h|), which covers the rest's slow fall (it is the scaled complementary error function). The
+// coefficients are a weighted least-squares fit to that function over |h| <= 14, good to 3e-7 where h is small and to 2.3e-5 of
+// the value itself far out, where GELU is h times it: 0.05 of float16's rounding, so the outputs there are as good as their
+// type. exp2 and the reciprocal are the hardware's, one ulp.
 __device__ __forceinline__ float normal_cdf(float h, float& e) {
-    const float t = rcp_of(fmaf(0.23164189f, fabsf(h), 1.0f));                           // 0.3275911 |h| / sqrt(2)
+    const float t = rcp_of(fmaf(0.3f, fabsf(h), 1.0f));
     e = exp2_of(h * h * -0.7213475204444817f);
-    const float q = fmaf(fmaf(fmaf(fmaf(0.5307027145f, t, -0.7265760135f), t, 0.7107068705f), t, -0.142248368f), t,
-                         0.127414796f) * t * e;                                          // the coefficients' halves
+    const float q = fmaf(fmaf(fmaf(fmaf(fmaf(-0.0788607597f, t, 0.22041145f), t, -0.0207132176f), t, 0.145473763f), t,
+                              0.113620818f), t, 0.120067716f) * t * e;
     return h < 0.0f ? q : 1.0f - q;
 }
 // GELU's tanh form is h times the logistic of 2 z, z = sqrt(2 / pi) (h + 0.044715 h^3), since (1 + tanh z) / 2 is that
