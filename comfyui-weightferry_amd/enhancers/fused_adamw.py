@@ -89,11 +89,9 @@ def _odd_one(params, grads, dt, dev):
     return "parameters and gradients do not fit together"
 
 
-def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
-    """Step ``step`` (1 is the first) on ``params`` and ``state`` in place: decoupled weight decay, bias-corrected moments.
-    ``params`` and ``grads``: contiguous GPU tensors of one type (float32, bfloat16 or float16) on one device, a gradient as
-    many values as its parameter, in the order that ``state`` was made for. ValueError for anything else. Asynchronous on torch's current stream."""
-    params, grads = list(params), list(grads)
+def _ready(params, grads, state, step, lr, betas, eps, weight_decay):
+    """A step's launch, once everything about it has been found in order (ValueError if not): nothing has changed until it is
+    called."""
     if len(params) != len(grads):
         raise ValueError(f"{len(params)} parameters and {len(grads)} gradients")
     _check_state(state)
@@ -103,7 +101,7 @@ def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8
             and math.isfinite(weight_decay)):
         raise ValueError(f"lr={lr}, betas={tuple(betas)}, eps={eps}, weight_decay={weight_decay}")
     if not params:
-        return
+        return lambda: None
     dt, dev = params[0].dtype, state.exp_avg.device
     code = CODES.get(dt)
     if code is None or dev.type != "cuda":
@@ -120,14 +118,24 @@ def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8
     table[0::3] = array.array("q", map(_data_ptr, params))
     table[1::3] = array.array("q", map(_data_ptr, grads))
     table[2::3] = array.array("q", sizes)
-    with _native.on_device(dev):
-        _native.call("wf_adamw", table.buffer_info()[0], len(params), code, state.bits, state.exp_avg.data_ptr(),
-                     state.exp_avg_sq.data_ptr(), None if state.exp_avg_scale is None else state.exp_avg_scale.data_ptr(),
-                     None if state.exp_avg_sq_scale is None else state.exp_avg_sq_scale.data_ptr(),
-                     state.exp_avg.numel() // BLOCK, int(step), lr, betas[0], betas[1], eps, weight_decay,
-                     _native.stream_of(dev))
-    # what autograd saved of them is stale now, as after torch's own in-place operations
-    torch.autograd.graph.increment_version(params)
+
+    def launch():
+        with _native.on_device(dev):
+            _native.call("wf_adamw", table.buffer_info()[0], len(params), code, state.bits, state.exp_avg.data_ptr(),
+                         state.exp_avg_sq.data_ptr(), None if state.exp_avg_scale is None else state.exp_avg_scale.data_ptr(),
+                         None if state.exp_avg_sq_scale is None else state.exp_avg_sq_scale.data_ptr(),
+                         state.exp_avg.numel() // BLOCK, int(step), lr, betas[0], betas[1], eps, weight_decay,
+                         _native.stream_of(dev))
+        # what autograd saved of them is stale now, as after torch's own in-place operations
+        torch.autograd.graph.increment_version(params)
+    return launch
+
+
+def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    """Step ``step`` (1 is the first) on ``params`` and ``state`` in place: decoupled weight decay, bias-corrected moments.
+    ``params`` and ``grads``: contiguous GPU tensors of one type (float32, bfloat16 or float16) on one device, a gradient as
+    many values as its parameter, in the order that ``state`` was made for. ValueError for anything else. Asynchronous on torch's current stream."""
+    _ready(list(params), list(grads), state, step, lr, betas, eps, weight_decay)()
 
 
 class AdamW(torch.optim.Optimizer):
@@ -155,6 +163,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        steps = []                                       # of every group, before the first of them changes anything
         for group in self.param_groups:
             params = group["params"]
             grads = [p.grad for p in params]
@@ -163,12 +172,13 @@ class AdamW(torch.optim.Optimizer):
                 continue
             if missing:
                 raise ValueError(f"{missing} of a group's {len(grads)} parameters have no gradient")
-            held = self.state[params[0]]
-            if not held:
-                state = adamw_state(params, group["bits"])
-                held["step"] = 0
-                held.update(zip(AdamWState._fields, state))
-            held["step"] += 1
-            adamw_step(params, grads, AdamWState(*(held[f] for f in AdamWState._fields)), held["step"], group["lr"],
-                       group["betas"], group["eps"], group["weight_decay"])
+            held = self.state.get(params[0]) or {"step": 0, **adamw_state(params, group["bits"])._asdict()}
+            step = held["step"] + 1
+            launch = _ready(params, grads, AdamWState(*(held[f] for f in AdamWState._fields)), step, group["lr"],
+                            group["betas"], group["eps"], group["weight_decay"])
+            steps.append((launch, params[0], held, step))
+        for launch, first, held, step in steps:
+            launch()
+            held["step"] = step
+            self.state[first] = held
         return loss
