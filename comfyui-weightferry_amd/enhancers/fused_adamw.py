@@ -17,6 +17,7 @@ from .operands import CODES, plain
 BLOCK = 256
 _TYPES = frozenset((torch.Tensor, torch.nn.Parameter))
 _dtype, _index, _contiguous = operator.attrgetter("dtype"), torch.Tensor.get_device, torch.Tensor.is_contiguous
+_capturing = torch.cuda.is_current_stream_capturing
 _data_ptr, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
 
 
@@ -106,6 +107,9 @@ def _ready(params, grads, state, step, lr, betas, eps, weight_decay):
     code = CODES.get(dt)
     if code is None or dev.type != "cuda":
         raise ValueError(f"parameters of type {dt} with moments on {dev}: float32, bfloat16 or float16 on a GPU")
+    if _capturing():
+        raise RuntimeError("a step cannot be captured into a graph: its step count, rates and addresses are the call's, and a "
+                           "replay would repeat them")
     if not plain(dev):
         raise ValueError("a step inside a functorch transform or a trace, which would not see it")
     # (questions of all tensors at once: with hundreds of adapters they are the step's host time, 0.6 us a parameter; the numbers
@@ -134,7 +138,8 @@ def _ready(params, grads, state, step, lr, betas, eps, weight_decay):
 def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
     """Step ``step`` (1 is the first) on ``params`` and ``state`` in place: decoupled weight decay, bias-corrected moments.
     ``params`` and ``grads``: contiguous GPU tensors of one type (float32, bfloat16 or float16) on one device, a gradient as
-    many values as its parameter, in the order that ``state`` was made for. ValueError for anything else. Asynchronous on torch's current stream."""
+    many values as its parameter, in the order that ``state`` was made for. ValueError for anything else. Asynchronous on
+    torch's current stream; RuntimeError while that is captured into a graph, whose replays would repeat this very step."""
     _ready(list(params), list(grads), state, step, lr, betas, eps, weight_decay)()
 
 

@@ -225,7 +225,8 @@ int wf_dense_bwd(const void* x, int64_t x_row, const void* w, int64_t w_row, int
  * call returns: address of the parameter, address of its gradient, values, for each tensor. The moments are flat over all
  * tensors, each starting on a whole block of 256 values, `blocks` in all: bits 32: float32 [blocks * 256], scales unused;
  * bits 8: exp_avg int8, exp_avg_sq uint8 [blocks * 256] with float32 scales [blocks], m = sign(q) (q / 127)^2 s, v = ((q /
- * 255)^2 s)^2, s a block's largest |m| or sqrt(v); a v > 0 keeps a code > 0. wf_adamw_values: the float32 values that 8-bit
+ * 255)^2 s)^2, s a block's largest |m| or sqrt(v); a v > 0 keeps a code > 0. Captured into a graph, a replay repeats this
+ * step: rates, bias corrections and addresses are the launch's. wf_adamw_values: the float32 values that 8-bit
  * moments stand for. */
 int wf_adamw(const int64_t* table, int64_t count, int dt, int bits, void* exp_avg, void* exp_avg_sq, float* avg_scale,
              float* sq_scale, int64_t blocks, int64_t step, double lr, double beta1, double beta2, double eps,

@@ -1,4 +1,5 @@
-"""AdamW steps that are refused leave everything as it was: parameters, moments and the count of steps."""
+"""AdamW steps that are refused leave everything as it was: parameters, moments and the count of steps.
+A step is not captured into a graph."""
 import pytest
 import torch
 
@@ -41,3 +42,21 @@ def test_no_group_steps_when_another_is_refused(native):
     opt.step()
     assert torch.equal(p, q) and torch.equal(q, r) and float(p.detach().max()) < 1.0
     assert opt.state[p]["step"] == opt.state[q]["step"] == 1
+
+
+def test_a_step_is_not_captured(native):
+    # its step count, rates and addresses are the call's: a replay would repeat them
+    p = torch.nn.Parameter(torch.zeros(300, device="cuda"))
+    p.grad = torch.ones(300, device="cuda")
+    opt = fa.AdamW([p])
+    opt.step()
+    torch.cuda.synchronize()
+    before = p.detach().clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = p.detach() * 2
+        with pytest.raises(RuntimeError, match="graph"):
+            opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(p.detach(), before) and torch.equal(y, before * 2) and opt.state[p]["step"] == 1
