@@ -38,6 +38,8 @@ class AdamWState(NamedTuple):
             return self.exp_avg, self.exp_avg_sq
         _check_state(self)
         dev = self.exp_avg.device
+        if dev.type != "cuda":
+            raise ValueError(f"codes on {dev}: the kernel that reads them needs them on a GPU")
         m, v = (torch.empty(self.exp_avg.numel(), dtype=torch.float32, device=dev) for _ in range(2))
         with _native.on_device(dev):
             _native.call("wf_adamw_values", self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),

@@ -1,4 +1,4 @@
-"""The optimizer's bookkeeping when a step is refused (CPU only: no kernel runs)."""
+"""The optimizer's bookkeeping when a step is refused, and moments that lie on the host (CPU only: no kernel runs)."""
 import pytest
 import torch
 
@@ -36,3 +36,10 @@ def test_every_group_is_looked_at_before_the_first_step():
     q.grad = None
     opt.step()                                                  # no gradients at all: nothing to do
     assert not any(opt.state.values())
+
+
+def test_values_of_moments_on_the_host():
+    p = torch.randn(300)
+    with pytest.raises(ValueError, match="GPU"):
+        fa.adamw_state([p], 8).values()
+    assert all(t.numel() == 512 for t in fa.adamw_state([p], 32).values())     # float32: the state's own tensors
