@@ -23,10 +23,10 @@
 // lane: 278 us, 5.1 TB/s. The parameter's step uses the one-ulp forms throughout; its error is far below the parameter's own
 // rounding.
 
-#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
+#include "grids.h"
 #include "values.h"
 
 namespace wf {
@@ -261,11 +261,19 @@ extern "C" int wf_adamw(const int64_t* table, int64_t count, int dt, int bits, v
     // (3.1 GB) 525 against 577 us; 14.7 M float32 values (0.4 GB) 75 against 66. In 8 bits no difference.
     const bool stream_past = (double)blocks * kBlock * (16 + 3 * (double)size) > 1e9;
     AdamTable t;
-    t.count = 0;
-    block = 0;
-    uint32_t wgs = 0;
-    auto launch = [&] {
-        t.wg[t.count] = wgs;
+    int64_t tensor = 0, before = 0;                       // blocks of the tensors before `tensor`
+    auto values = [&](int64_t i) { return table[3 * i + 2]; };
+    auto part = [&](int c, int64_t i, int64_t done, int64_t part_blocks, uint32_t wg) {
+        for (; tensor < i; tensor++) before += (values(tensor) + kBlock - 1) / kBlock;
+        t.p[c] = reinterpret_cast<char*>(table[3 * i]) + done * kBlock * size;
+        t.g[c] = reinterpret_cast<const char*>(table[3 * i + 1]) + done * kBlock * size;
+        t.n[c] = std::min(values(i) - done * kBlock, part_blocks * kBlock);
+        t.block[c] = (uint32_t)(before + done);
+        t.wg[c] = wg;
+    };
+    auto launch = [&](int parts, uint32_t wgs) {
+        t.count = parts;
+        t.wg[parts] = wgs;
         auto go = [&](auto d) {
             constexpr int D = decltype(d)::value;
             if (bits == 8) adamw<D, true, false><<<dim3(wgs), 256, 0, s>>>(t, k, exp_avg, exp_avg_sq, avg_scale, sq_scale);
@@ -276,29 +284,8 @@ extern "C" int wf_adamw(const int64_t* table, int64_t count, int dt, int bits, v
         if (dt == WF_F16) go(std::integral_constant<int, WF_F16>{});
         else if (dt == WF_BF16) go(std::integral_constant<int, WF_BF16>{});
         else go(std::integral_constant<int, WF_F32>{});
-        t.count = 0;
-        wgs = 0;
     };
-    for (int64_t i = 0; i < count; i++) {
-        int64_t n = table[3 * i + 2], done = 0;
-        const int64_t nb = (n + kBlock - 1) / kBlock;
-        // (a tensor of more workgroups than one grid holds goes out in parts of whole blocks)
-        while (done < nb) {
-            const int64_t most = ((int64_t)(1u << 30) - wgs) * kAdamWg, part = std::min(nb - done, most);
-            const int c = t.count;
-            t.p[c] = reinterpret_cast<char*>(table[3 * i]) + done * kBlock * size;
-            t.g[c] = reinterpret_cast<const char*>(table[3 * i + 1]) + done * kBlock * size;
-            t.n[c] = std::min(n - done * kBlock, part * kBlock);
-            t.block[c] = (uint32_t)(block + done);
-            t.wg[c] = wgs;
-            wgs += (uint32_t)((part + kAdamWg - 1) / kAdamWg);
-            t.count++;
-            done += part;
-            if (t.count == kAdamTensors || wgs == (1u << 30)) launch();
-        }
-        block += nb;
-    }
-    if (t.count) launch();
+    over_tensors(count, kBlock, kAdamWg, kAdamTensors, kGridMost, values, part, launch);
     WF_LAUNCH_CHECK("wf_adamw launch");
     return WF_OK;
 }
@@ -313,9 +300,12 @@ extern "C" int wf_adamw_values(const int8_t* exp_avg, const uint8_t* exp_avg_sq,
         set_error("wf_adamw_values: null or misaligned pointer");
         return WF_EINVAL;
     }
-    const int64_t quads = blocks * 64;
-    adamw_values<<<dim3((uint32_t)((quads + 255) / 256)), 256, 0, static_cast<hipStream_t>(stream)>>>(
-        exp_avg, exp_avg_sq, avg_scale, sq_scale, reinterpret_cast<float4*>(avg), reinterpret_cast<float4*>(sq), quads);
+    over_grids((blocks + 3) / 4, kGridMost, [&](int64_t wg, uint32_t n) {              // (a workgroup reads 4 blocks)
+        const int64_t b = 4 * wg;
+        adamw_values<<<dim3(n), 256, 0, static_cast<hipStream_t>(stream)>>>(
+            exp_avg + b * kBlock, exp_avg_sq + b * kBlock, avg_scale + b, sq_scale + b,
+            reinterpret_cast<float4*>(avg + b * kBlock), reinterpret_cast<float4*>(sq + b * kBlock), (blocks - b) * 64);
+    });
     WF_LAUNCH_CHECK("wf_adamw_values launch");
     return WF_OK;
 }

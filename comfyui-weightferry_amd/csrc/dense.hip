@@ -16,15 +16,16 @@
 #include "dense_gemm.h"
 #include "dense_grad.h"
 #include "dense_rows.h"
+#include "grids.h"
 
 namespace wf {
 
-// the slices' sums in slice order, then the epilogue: one run of 8 outputs a thread
+// the slices' sums in slice order, then the epilogue: one run of 8 outputs a thread, from workgroup `wg` of the whole on
 template <int D>
-__global__ __launch_bounds__(256) void dense_sum(const float* __restrict__ parts, int slices, int M, int N,
+__global__ __launch_bounds__(256) void dense_sum(int64_t wg, const float* __restrict__ parts, int slices, int M, int N,
                                                  DenseEpilogue e) {
     const int runs = (N + 7) / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = (wg + blockIdx.x) * 256 + threadIdx.x;
     if (i >= (int64_t)M * runs) return;
     const int64_t m = i / runs;
     const int n = (int)(i - m * runs) * 8, cnt = N - n;
@@ -52,17 +53,18 @@ __global__ __launch_bounds__(256) void dense_sum(const float* __restrict__ parts
 }
 
 // R rows of K consecutive values (of an operand, or of memory where it lies across K), `row` apart, as [R, KP], KP a multiple
-// of 8, zeros past K: a run of 8 values a thread, loaded at any alignment. One launch copies both operands (blockIdx.y).
+// of 8, zeros past K: a run of 8 values a thread, loaded at any alignment. One launch copies both operands (blockIdx.y),
+// from workgroup `wg` of the whole on.
 struct PackRows {
     const uint16_t* p;
     uint16_t* out;
     int64_t row, runs;                                             // runs: R KP / 8
     int K, KP;
 };
-__global__ __launch_bounds__(256) void dense_pack_rows(PackRows a, PackRows b) {
+__global__ __launch_bounds__(256) void dense_pack_rows(int64_t wg, PackRows a, PackRows b) {
     const PackRows q = blockIdx.y ? b : a;
     const int across = q.KP / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = (wg + blockIdx.x) * 256 + threadIdx.x;
     if (i >= q.runs) return;
     const int64_t r = i / across;
     const int k = (int)(i - r * across) * 8;
@@ -267,16 +269,17 @@ static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w
         PackRows jx = {}, jw = {};
         const DenseOperand a = dense_operand(x, d.how_x, M, K, reinterpret_cast<uint16_t*>(ws), jx, s);
         const DenseOperand b = dense_operand(w, d.how_w, N, K, reinterpret_cast<uint16_t*>(ws + d.w_at), jw, s);
-        if (const int64_t runs = std::max(jx.runs, jw.runs))
-            dense_pack_rows<<<dim3((uint32_t)((runs + 255) / 256), jx.runs && jw.runs ? 2 : 1), 256, 0, s>>>(
-                jx.runs ? jx : jw, jw);
+        over_grids((std::max(jx.runs, jw.runs) + 255) / 256, kGridMost, [&](int64_t wg, uint32_t n) {
+            dense_pack_rows<<<dim3(n, jx.runs && jw.runs ? 2 : 1), 256, 0, s>>>(wg, jx.runs ? jx : jw, jw);
+        });
         auto run = a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : !d.epilogue || parts ? dense_gemm_along : dense_gemm_along_full;
         run(dt, a, b, (int)M, (int)N, (int)K, d.tiles, parts, e, s);
     }
     if (d.summed) {
-        const dim3 grid((uint32_t)((M * ((N + 7) / 8) + 255) / 256));
-        if (dt == WF_BF16) dense_sum<WF_BF16><<<grid, 256, 0, s>>>(parts, d.slices(), (int)M, (int)N, e);
-        else dense_sum<WF_F16><<<grid, 256, 0, s>>>(parts, d.slices(), (int)M, (int)N, e);
+        over_grids((M * ((N + 7) / 8) + 255) / 256, kGridMost, [&](int64_t wg, uint32_t n) {
+            if (dt == WF_BF16) dense_sum<WF_BF16><<<dim3(n), 256, 0, s>>>(wg, parts, d.slices(), (int)M, (int)N, e);
+            else dense_sum<WF_F16><<<dim3(n), 256, 0, s>>>(wg, parts, d.slices(), (int)M, (int)N, e);
+        });
     }
 }
 
