@@ -105,8 +105,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, modulation=False):
                 return None
             pcode = 2
         groups = groups_of(t, rows, width, what)
-        if first is not None and (first.dtype != t.dtype or first.numel() != t.numel()):
-            raise ValueError(f"weight {first.dtype} {tuple(first.shape)} and bias {t.dtype} {tuple(t.shape)} differ")
+        if first is not None and first.numel() != t.numel():
+            raise ValueError(f"weight {tuple(first.shape)} and bias {tuple(t.shape)} differ")
+        if first is not None and first.dtype != t.dtype:
+            return None
         first = t
     if groups > 65535 or rows >= 1 << 31:
         return None
