@@ -47,7 +47,7 @@ def gradient(dy):
 
 def rows_of(t, width):
     """``t`` [..., width] as a matrix whose rows are runs of values, a view where its strides allow one."""
-    t2 = t if t.dim() == 2 else t.reshape(-1, width)
+    t2 = t if t.dim() == 2 else t.reshape(-1 if width else t.shape[:-1].numel(), width)
     return t2 if t2.stride(1) == 1 or width == 1 else t2.contiguous()
 
 

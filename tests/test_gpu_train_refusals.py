@@ -16,3 +16,15 @@ def test_layer_norm_parameters_of_two_types(native):
     assert fn.layer_norm(x, w, b) is not None
     with pytest.raises(ValueError, match="differ"):
         fn.layer_norm(x, w, b[None].expand(2, 32))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_dense_without_outputs(native, grad):
+    x = torch.randn(2, 5, 64, device="cuda").to(torch.bfloat16).requires_grad_(grad)
+    w = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16)
+    r = torch.empty(2, 5, 0, device="cuda", dtype=torch.bfloat16)
+    y = fd.dense(x, w, residual=r)
+    assert y.shape == (2, 5, 0) and y.dtype == torch.bfloat16
+    if grad:
+        (gx,) = torch.autograd.grad(y.sum(), x)
+        assert gx.shape == x.shape and float(gx.abs().sum()) == 0.0

@@ -161,3 +161,10 @@ def test_traces_are_not_the_kernels_case():
     from torch.utils.flop_counter import FlopCounterMode       # a mode that watches, but records no program
     with FlopCounterMode(display=False):
         assert ops.plain(x.device, x)
+
+
+def test_rows_of_no_values():
+    ops = sub("enhancers.operands")
+    for shape, rows in (((2, 5, 0), 10), ((0,), 1), ((3, 0), 3), ((0, 4, 0), 0)):
+        assert ops.rows_of(torch.empty(shape), 0).shape == (rows, 0)
+    assert ops.rows_of(torch.empty(2, 5, 3), 3).shape == (10, 3) and ops.rows_of(torch.empty(0, 5, 3), 3).shape == (0, 3)
