@@ -364,7 +364,8 @@ extern "C" int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void*
         set_error("wf_dense: a workspace of %lld bytes is required", (long long)d.bytes);
         return WF_EINVAL;
     }
-    const DenseEpilogue e = {bias, gate, resid, bias_dt, gate_dt, act, gate ? rows_per_group : 1, resid_row, y, h};
+    // (the kernels divide in 32 bits: a group of more than M rows is one of M)
+    const DenseEpilogue e = {bias, gate, resid, bias_dt, gate_dt, act, gate ? std::min(rows_per_group, M) : 1, resid_row, y, h};
     dense_run(d, xv, wv, dt, M, N, K, static_cast<char*>(workspace), e, static_cast<hipStream_t>(stream));
     WF_LAUNCH_CHECK("wf_dense launch");
     return WF_OK;
