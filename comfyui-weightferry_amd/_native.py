@@ -53,6 +53,7 @@ EXPORTS = {
     "wf_layer_norm_bwd": (_int, [_p, _i64, _p, _i64, _int, _p, _int, _int, _i64, _p, _p, _p, _p, _i64, _i64, _p, _i64,
                                  _p]),
     "wf_dense_workspace": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _int, ctypes.POINTER(_i64)]),
+    "wf_dense_plan": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _int, ctypes.POINTER(_int)]),
     "wf_dense": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _p, _int, _int, _p, _int, _i64, _p, _i64,
                         _p, _p, _p, _i64, _p]),
     "wf_dense_bwd_workspace": (_int, [_p, _i64, _p, _i64, _i64, _p, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _int,

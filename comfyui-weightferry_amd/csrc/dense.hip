@@ -259,6 +259,15 @@ static DenseOperand dense_operand(const DenseView& v, int how, int64_t R, int64_
     return {out, to, (int)to, (int)R, false};
 }
 
+// the tiled kernel of a call (dense_gemm.h has one source each), as wf_dense_plan numbers them; 0 is the few-rows form
+enum { FORM_ROWS, FORM_ALONG, FORM_ALONG_FULL, FORM_B_ACROSS, FORM_ACROSS };
+static int dense_form(const DenseCall& d) {
+    if (d.few) return FORM_ROWS;
+    if (is_across(d.how_x)) return FORM_ACROSS;
+    if (is_across(d.how_w)) return FORM_B_ACROSS;
+    return d.epilogue && !d.summed ? FORM_ALONG_FULL : FORM_ALONG;
+}
+
 static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w, int dt, int64_t M, int64_t N, int64_t K,
                       char* ws, const DenseEpilogue& e, hipStream_t s) {
     float* parts = d.summed ? reinterpret_cast<float*>(ws + d.parts_at) : nullptr;
@@ -272,7 +281,9 @@ static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w
         over_grids((std::max(jx.runs, jw.runs) + 255) / 256, kGridMost, [&](int64_t wg, uint32_t n) {
             dense_pack_rows<<<dim3(n, jx.runs && jw.runs ? 2 : 1), 256, 0, s>>>(wg, jx.runs ? jx : jw, jw);
         });
-        auto run = a.x ? dense_gemm_across : b.x ? dense_gemm_b_across : !d.epilogue || parts ? dense_gemm_along : dense_gemm_along_full;
+        const int form = dense_form(d);
+        auto run = form == FORM_ACROSS ? dense_gemm_across : form == FORM_B_ACROSS ? dense_gemm_b_across
+                   : form == FORM_ALONG ? dense_gemm_along : dense_gemm_along_full;
         run(dt, a, b, (int)M, (int)N, (int)K, d.tiles, parts, e, s);
     }
     if (d.summed) {
@@ -335,6 +346,21 @@ extern "C" int wf_dense_workspace(const void* x, int64_t x_row, int64_t x_col, c
     if (!bytes || epilogue < 0 || epilogue > 7) { set_error("wf_dense_workspace: null pointer or epilogue %d", epilogue); return WF_EINVAL; }
     if (const int rc = dense_check("wf_dense_workspace", dt, M, N, K, x_row, x_col, w_row, w_col)) return rc;
     *bytes = M && N ? dense_call({x, x_row, x_col, false}, {w, w_row, w_col, false}, M, N, K, epilogue).bytes : 0;
+    return WF_OK;
+}
+
+extern "C" int wf_dense_plan(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt,
+                             int64_t M, int64_t N, int64_t K, int epilogue, int* plan) {
+    using namespace wf;
+    if (!plan || epilogue < 0 || epilogue > 7) { set_error("wf_dense_plan: null pointer or epilogue %d", epilogue); return WF_EINVAL; }
+    if (const int rc = dense_check("wf_dense_plan", dt, M, N, K, x_row, x_col, w_row, w_col)) return rc;
+    if (M == 0 || N == 0) { set_error("wf_dense_plan: no outputs"); return WF_EINVAL; }
+    const DenseCall d = dense_call({x, x_row, x_col, false}, {w, w_row, w_col, false}, M, N, K, epilogue);
+    plan[0] = dense_form(d);
+    plan[1] = d.few ? d.rows.tiles : d.tiles.tiling;
+    plan[2] = d.slices();
+    plan[3] = d.few ? LIES_ALONG : d.how_x;
+    plan[4] = d.few ? LIES_ALONG : d.how_w;
     return WF_OK;
 }
 

@@ -201,6 +201,12 @@ int wf_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldd, i
  * cleared and is free again when the call's work on the stream is done. */
 int wf_dense_workspace(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt,
                        int64_t M, int64_t N, int64_t K, int epilogue, int64_t* bytes);
+/* How wf_dense runs such a call, plan[5]: the kernel (0 few rows; tiles: 1 both operands along K, 2 the same with an
+ * activation, gate, resid or h in its epilogue, 3 w across K, 4 both across), its tiling (0-7; few rows: 16-row weight tiles a
+ * workgroup), slices of K, and how x and w get there (0 as they lie along K, 1 as they lie across, 2 and 3 copied in that
+ * order, 4 copied into rows along K). */
+int wf_dense_plan(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt, int64_t M,
+                  int64_t N, int64_t K, int epilogue, int* plan);
 int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt, int64_t M,
              int64_t N, int64_t K, const void* bias, int bias_dt, int act, const void* gate, int gate_dt,
              int64_t rows_per_group, const void* resid, int64_t resid_row, void* y, void* h, void* workspace,
