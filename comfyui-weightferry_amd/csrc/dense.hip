@@ -1,14 +1,17 @@
 // The 16-bit linear for gfx950: y = resid + gate * act(x w^T + bias) on bfloat16 or float16, float32 accumulation, one
 // rounding at the end; and the products of its backward pass, which are the same product on other operands.
 //
-// 2 M N K operations: v_mfma_f32_32x32x16 tiles fed through the two-buffer LDS ring of dense_ring.h. A product with too
-// few tiles to fill the 256 CUs runs as slices of K that write float32 partial sums; a second kernel adds them in slice
-// order and runs the epilogue. Operands whose rows are not 16-byte runs along K (odd widths, transposed views) are first
-// copied into rows that are.
+// 2 M N K operations: v_mfma_f32_32x32x16 tiles fed through the two-buffer LDS ring of dense_ring.h. Each operand is loaded as
+// it lies, along K or across it (a transposed view: the backward products read the weight, x and dh so); only one that is
+// neither in 16-byte runs (odd row lengths, other strides) is first copied into rows that are. A product with too few tiles
+// to fill the 256 CUs runs as slices of K that write float32 partial sums, and so does one with w across K that has more than
+// a plain epilogue; a second kernel adds the sums in slice order and runs the epilogue. At few rows of x the product takes a
+// form of its own (dense_rows.hip).
 //
-// The epilogue works on runs of 8 outputs of a row: the accumulators (16 rows x 1 column a lane) pass through the idle
-// stage buffers in float32, so bias, activation, gate and residual are computed on the unrounded sums and every global
-// access is 16 bytes.
+// The epilogue works on the float32 sums: bias as their start, activation and gate in the accumulators (16 rows x 1 column a
+// lane). The residual comes through the idle stage buffers into that layout, and what is stored goes out through them,
+// rounded once, in 16-byte runs. A tile that spans two of the gate's groups, and rows of no whole runs with a gate or a residual,
+// go through the stage buffers in float32 and are finished run by run (dense.h).
 
 #include <algorithm>
 #include <type_traits>

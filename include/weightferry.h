@@ -194,10 +194,10 @@ int wf_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldd, i
  * float32 accumulation, one rounding. act: 0 none, 1 GELU (erf), 2 GELU (tanh), 3 SiLU, 4 ReLU. bias, gate, resid may be
  * NULL; bias and gate have type dt or WF_F32 (bias_dt, gate_dt). An operand's value (r, k) is at r * row + k * col, so
  * transposed views need no copy by the caller; resid's rows are resid_row values apart; y is [M, N]. h (may be NULL): the
- * sums with the bias, [M, N] of type dt, what wf_dense_grad reads (float16: kept finite). M, N <= 2^24, K <= 2^20.
+ * sums with the bias, [M, N], rounded to dt, what wf_dense_bwd reads (kept finite). M, N <= 2^24, K <= 2^20.
  * The workspace (256-byte aligned, at least the bytes that wf_dense_workspace gives for the same operands; epilogue: 1 with an
  * activation, + 2 where h is kept, + 4 with a gate or resid) holds copies of operands that cannot be loaded as they are, and
- * the partial sums of products that run in slices of K; it need not be
+ * the float32 partial sums of products that run in slices of K, or with w across K and any such epilogue; it need not be
  * cleared and is free again when the call's work on the stream is done. */
 int wf_dense_workspace(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt,
                        int64_t M, int64_t N, int64_t K, int epilogue, int64_t* bytes);
@@ -217,7 +217,8 @@ int wf_dense(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t
  * of the unrounded dh (bias_dt), dgate = the sum over each group's rows of dy act(h) (gate_dt); any of the four may be NULL.
  * (resid's gradient is dy.) x: rows x_row values apart; w as in wf_dense. M, N, K <= 2^20, at most 65535 groups. The workspace
  * (256-byte aligned; wf_dense_bwd_workspace for the same operands, gated: whether there is a gate, dx, dw: whether they
- * are wanted, sums: dbias or dgate is) holds dh, partial sums and what the products need. Every sum has a fixed order. */
+ * are wanted, sums: dbias or dgate is) holds dh, partial sums (for both of dbias and dgate) and what the products need. Every
+ * sum has a fixed order. */
 int wf_dense_bwd_workspace(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, const void* dy,
                            int64_t dy_row, int dt, int act, int gated, int64_t rows_per_group, int64_t M, int64_t N,
                            int64_t K, int dx, int dw, int sums, int64_t* bytes);
