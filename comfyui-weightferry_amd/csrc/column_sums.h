@@ -12,10 +12,8 @@ struct ColumnSums {
     int dt, n;
 };
 
-// blockIdx: 64 columns, group, which of two arrays of partial sums (both with the same groups)
-static __global__ __launch_bounds__(1024) void column_sums(ColumnSums a, ColumnSums b, int K) {
-    __shared__ float red[16][64];
-    const ColumnSums q = blockIdx.z ? b : a;
+// workgroup: 64 columns (blockIdx.x) of group blockIdx.y
+__device__ __forceinline__ void column_sum(const ColumnSums& q, int K, float (&red)[16][64]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = blockIdx.x * 64 + lane;
     const int64_t g = blockIdx.y;
@@ -31,6 +29,22 @@ static __global__ __launch_bounds__(1024) void column_sums(ColumnSums a, ColumnS
         for (int i = 0; i < 16; i++) s += red[i][lane];
         store_value(q.out, g * K + col, q.dt, s);
     }
+}
+
+// blockIdx.z: which of two arrays of partial sums (both with the same groups)
+static __global__ __launch_bounds__(1024) void column_sums(ColumnSums a, ColumnSums b, int K) {
+    __shared__ float red[16][64];
+    column_sum(blockIdx.z ? b : a, K, red);
+}
+
+// the same for up to four arrays, each with groups of its own
+struct ColumnSums4 {
+    ColumnSums q[4];
+    int groups[4];
+};
+static __global__ __launch_bounds__(1024) void column_sums4(ColumnSums4 a, int K) {
+    __shared__ float red[16][64];
+    if ((int)blockIdx.y < a.groups[blockIdx.z]) column_sum(a.q[blockIdx.z], K, red);
 }
 
 }  // namespace wf

@@ -17,27 +17,9 @@
 #include <type_traits>
 
 #include "column_sums.h"
+#include "row_teams.h"
 
 namespace wf {
-
-// the sums of a and b over a team's W waves, in every lane. red: 2 x 2 floats a wave, used alternately (phase) so that one
-// barrier a call is enough
-__device__ __forceinline__ float2 team_sum2(float a, float b, int W, float* red, int phase) {
-    a = wave_sum(a);
-    b = wave_sum(b);
-    if (W > 1) {
-        const int wave = threadIdx.x >> 6, first = wave / W * W;
-        float2* r = reinterpret_cast<float2*>(red) + phase * 16;
-        if ((threadIdx.x & 63) == 0) r[wave] = make_float2(a, b);
-        __syncthreads();
-        a = b = 0.0f;
-        for (int i = 0; i < W; i++) {
-            a += r[first + i].x;
-            b += r[first + i].y;
-        }
-    }
-    return make_float2(a, b);
-}
 
 struct LnParams {
     const void* w;
@@ -267,34 +249,18 @@ __global__ __launch_bounds__(1024) void ln_bwd(const value_t<D>* __restrict__ x,
 
 constexpr int kLnMaxWidth = 32768;
 
-struct LnShape {
-    int waves, packs, teams, parts;      // a row's waves, a lane's packs, a workgroup's teams, workgroups a group of rows
-};
-// Two packs a lane, then more waves (up to 16); teams up to team_waves waves a workgroup, fewer where that would leave CUs
-// idle; workgroups over all groups: as many a CU as make cu_waves waves of it, at most per_cu.
-static LnShape ln_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt, int team_waves, int cu_waves, int per_cu) {
-    const int64_t lane = 64 * (dt == WF_F32 ? 4 : 8), packs = (K + lane - 1) / lane;   // of a lane, if the row had one wave
-    LnShape s;
-    s.waves = (int)std::min<int64_t>(16, (packs + 1) / 2);
-    s.packs = (int)((packs + s.waves - 1) / s.waves);
-    s.teams = (int)std::max<int64_t>(1, std::min<int64_t>(team_waves / s.waves, M / 256));
-    const int64_t wgs = 256 * std::max(1, std::min(per_cu, cu_waves / (s.waves * s.teams)));
-    s.parts = (int)std::min<int64_t>((rows_per_group + s.teams - 1) / s.teams,
-                                     std::max<int64_t>(1, wgs * rows_per_group / std::max<int64_t>(1, M)));
-    return s;
-}
 // Forward: workgroups of up to 5 waves. us at 4096 x 5120 bfloat16 (84 MB; 5 waves a workgroup) with 2 / 3 / 4 a CU: 21.8 /
 // 19.6 / 22.8; one row a workgroup, without loading ahead, 31. 5152 x 2048 in workgroups of 4 waves 11.9, of 8 waves 16.4;
 // 3000 x 8192 float32 (16 waves) with one a CU 32.8, with three 35.6. 16384 x 5120 takes 64 us, 5.2 TB/s. Rows of one pack a
 // lane use half the registers: 30000 x 256 in three workgroups of 8 waves a CU 13.0, in three of 5 14.4.
-static LnShape ln_fwd_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt) {
-    return K <= 64 * (dt == WF_F32 ? 4 : 8) ? ln_shape(M, K, rows_per_group, dt, 8, 24, 3)
-                                            : ln_shape(M, K, rows_per_group, dt, 5, 16, 8);
+static RowShape ln_fwd_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt) {
+    return K <= 64 * (dt == WF_F32 ? 4 : 8) ? row_shape(M, K, rows_per_group, dt, 8, 24, 3)
+                                            : row_shape(M, K, rows_per_group, dt, 5, 16, 8);
 }
 // Backward: one workgroup of up to 16 waves a CU, since every workgroup writes a row of partial sums: 4096 x 5120 takes
 // 35.7 us with 256, 37.9 with 512 of half the teams, 42.4 with 512 whole ones. 16384 x 5120: 98 us, 5.2 TB/s.
-static LnShape ln_bwd_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt) {
-    return ln_shape(M, K, rows_per_group, dt, 16, 16, 1);
+static RowShape ln_bwd_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt) {
+    return row_shape(M, K, rows_per_group, dt, 16, 16, 1);
 }
 
 // f with a lane's packs as a constant: the next of 1, 2, 3, 4, 6, 8 (a row of 32768 values over 16 waves has 4, or 8 of
@@ -308,13 +274,6 @@ static void ln_packs(int packs, F&& f) {
     else if (D != WF_F32 || packs <= 4) f(integral_constant<int, 4>{});
     else if (packs <= 6) f(integral_constant<int, D == WF_F32 ? 6 : 4>{});
     else f(integral_constant<int, D == WF_F32 ? 8 : 4>{});
-}
-
-template <typename F>
-static void by_dtype(int dt, F&& f) {
-    if (dt == WF_F16) f(std::integral_constant<int, WF_F16>{});
-    else if (dt == WF_BF16) f(std::integral_constant<int, WF_BF16>{});
-    else f(std::integral_constant<int, WF_F32>{});
 }
 
 static int ln_check(const char* who, int64_t M, int64_t K, int64_t rows_per_group, int dt, int param_dt) {
@@ -347,7 +306,7 @@ extern "C" int wf_layer_norm(const void* x, int64_t ldx, int dt, const void* w, 
     const hipStream_t s = static_cast<hipStream_t>(stream);
     by_dtype(dt, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        const LnShape p = ln_fwd_shape(M, K, rows_per_group, dt);
+        const RowShape p = ln_fwd_shape(M, K, rows_per_group, dt);
         ln_packs<D>(p.packs, [&](auto c) {
             ln_fwd<D, decltype(c)::value>
                 <<<dim3(p.parts, (uint32_t)(M / rows_per_group)), 64 * p.waves * p.teams, 0, s>>>(
@@ -381,7 +340,7 @@ extern "C" int wf_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int
         set_error("wf_layer_norm_bwd: null pointer or negative row stride");
         return WF_EINVAL;
     }
-    const LnShape p = ln_bwd_shape(M, K, rows_per_group, dt);
+    const RowShape p = ln_bwd_shape(M, K, rows_per_group, dt);
     const int n = p.parts;
     const int64_t groups = M / rows_per_group, plane = groups * n * K;
     float* parts = static_cast<float*>(workspace);

@@ -85,8 +85,8 @@ def once(backward):
     second derivative); without, as it nearly always is, the bare function."""
     wrapped = torch.autograd.function.once_differentiable(backward)
 
-    def run(ctx, dy):
-        return wrapped(ctx, dy) if _grad_enabled() else backward(ctx, dy)
+    def run(ctx, *dys):
+        return wrapped(ctx, *dys) if _grad_enabled() else backward(ctx, *dys)
     return staticmethod(run)
 
 

@@ -190,6 +190,31 @@ int wf_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldd, i
                       int plus_one, int64_t rows_per_group, const float* stats, void* dx, void* dw, void* db, int64_t M,
                       int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The norms after and before two sub-layers with the gated residual between them, rows of K values of type dt, at most 32768
+ * bytes: r = scale x + gate post_weight n(h), y = norm(r) s + bias, s = weight (plus_one 0) or 1 + weight. n: post, 0 nothing, 1
+ * RMS, h / sqrt(mean h^2 + eps), 2 LayerNorm; norm: 1 or 2. post_weight: [K]; gate: [gate_groups, K]; weight, bias:
+ * [weight_groups, K], gate_groups and weight_groups 1 or groups: the M rows are `groups` runs of consecutive rows, each with a row of
+ * those. Any of the four may be NULL; each is of type dt or WF_F32 (weight and bias of one). h may be NULL (r = scale x), and r.
+ * x, h: rows x_row, h_row values apart; r, y: [M, K]; y comes from r before its rounding. stats (may be NULL): float32 [M, 4],
+ * mean (0 for RMS) and reciprocal root of h's norm and of r's, what the backward pass reads.
+ * wf_block_norm_bwd: dx and dh [M, K] of type dt, the parameters' gradients of their types, for the gradients dr of r and dy of
+ * y (either may be NULL); any output may be NULL. The workspace (for as many parameters' gradients, `sums`, as are wanted; 4-byte
+ * aligned) holds partial sums, added in a fixed order. */
+typedef struct {
+    int32_t dt, post, norm, plus_one;
+    int32_t post_weight_dt, gate_dt, weight_dt;
+    float scale, eps;
+    int64_t groups, gate_groups, weight_groups;
+    const void *post_weight, *gate, *weight, *bias;
+} wf_block_norm;
+int wf_block_norm_fwd(const wf_block_norm* q, const void* x, int64_t x_row, const void* h, int64_t h_row, void* r, void* y,
+                      float* stats, int64_t M, int64_t K, void* stream);
+int wf_block_norm_bwd_workspace(const wf_block_norm* q, int64_t M, int64_t K, int sums, int64_t* bytes);
+int wf_block_norm_bwd(const wf_block_norm* q, const void* x, int64_t x_row, const void* h, int64_t h_row, const void* dr,
+                      int64_t dr_row, const void* dy, int64_t dy_row, const float* stats, void* dx, void* dh,
+                      void* dpost_weight, void* dgate, void* dweight, void* dbias, int64_t M, int64_t K, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
 /* y[m, n] = resid[m, n] + gate[m / rows_per_group, n] * act(sum_k x[m, k] * w[n, k] + bias[n]) in dt (WF_BF16 or WF_F16),
  * float32 accumulation, one rounding. act: 0 none, 1 GELU (erf), 2 GELU (tanh), 3 SiLU, 4 ReLU. bias, gate, resid may be
  * NULL; bias and gate have type dt or WF_F32 (bias_dt, gate_dt). An operand's value (r, k) is at r * row + k * col, so
