@@ -38,14 +38,14 @@ struct BlockNorm {
 
 // W waves a row, C packs a lane; workgroup (i, g) walks the rows of group g as in layer_norm.hip: team t takes rows i T + t, then
 // every gridDim.x T further, the next row loaded ahead. With up to 16 values a lane the parameters stay in registers.
-template <int D, int C, int NT>
-__global__ __launch_bounds__(NT) void bn_fwd(const value_t<D>* __restrict__ x, int64_t ldx,
-                                               const value_t<D>* __restrict__ h, int64_t ldh, BlockNorm q,
-                                               value_t<D>* __restrict__ r, value_t<D>* __restrict__ y,
-                                               float4* __restrict__ stats, int K, int W) {
+template <int D, int C, bool CENTER>
+__global__ __launch_bounds__(1024) void bn_fwd(const value_t<D>* __restrict__ x, int64_t ldx,
+                                             const value_t<D>* __restrict__ h, int64_t ldh, BlockNorm q,
+                                             value_t<D>* __restrict__ r, value_t<D>* __restrict__ y,
+                                             float4* __restrict__ stats, int K, int W) {
     constexpr int VEC = Pack<D>::VEC;
     __shared__ float red[64];
-    const int wave = threadIdx.x >> 6, teams = (int)blockDim.x / (64 * W), team = wave / W;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), teams = (int)blockDim.x / (64 * W), team = wave / W;
     const int t = (wave % W) * 64 + (threadIdx.x & 63);
     const int64_t g = blockIdx.y, rows = q.rows, first = g * rows, stride = (int64_t)gridDim.x * teams;
     Pack<D> nx[C], nh[C];
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(NT) void bn_fwd(const value_t<D>* __restrict__ x, i
     // mean (0 for RMS) and 1 / sqrt(mean square about it + eps) of a row's values v, zero past its end
     auto moments = [&](const float (&v)[C][VEC], int kind) {
         float mean = 0.0f, ss = 0.0f;
-        if (kind == NORM_LAYER) {
+        if (CENTER && kind == NORM_LAYER) {
             float s = 0.0f;
 #pragma unroll
             for (int c = 0; c < C; c++)
@@ -97,15 +97,20 @@ __global__ __launch_bounds__(NT) void bn_fwd(const value_t<D>* __restrict__ x, i
                 for (int i = 0; i < VEC; i++) s += v[c][i];
             mean = team_sum2(s, 0.0f, W, red, phase).x / (float)K;
             phase ^= 1;
-        }
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            const int n = K - (c * 64 * W + t) * VEC;
+            for (int c = 0; c < C; c++) {
+                const int n = K - (c * 64 * W + t) * VEC;
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                const float d = v[c][i] - mean;
-                ss += i < n ? d * d : 0.0f;
+                for (int i = 0; i < VEC; i++) {
+                    const float d = i < n ? v[c][i] - mean : 0.0f;
+                    ss = fmaf(d, d, ss);
+                }
             }
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int i = 0; i < VEC; i++) ss = fmaf(v[c][i], v[c][i], ss);
         }
         const float var = team_sum2(ss, 0.0f, W, red, phase).x / (float)K;
         phase ^= 1;
@@ -127,7 +132,8 @@ __global__ __launch_bounds__(NT) void bn_fwd(const value_t<D>* __restrict__ x, i
 #pragma unroll
         for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int i = 0; i < VEC; i++) v[c][i] = q.scale * px[c].get(i) + (v[c][i] - a.x) * a.y * gp[c][i];
+            for (int i = 0; i < VEC; i++)
+                v[c][i] = fmaf(CENTER ? (v[c][i] - a.x) * a.y : v[c][i] * a.y, gp[c][i], q.scale * px[c].get(i));
         const float2 b = moments(v, q.norm);
         if (i0 >= rows) continue;
         if (stats && t == 0) stats[first + i0] = make_float4(a.x, a.y, b.x, b.y);
@@ -142,7 +148,7 @@ __global__ __launch_bounds__(NT) void bn_fwd(const value_t<D>* __restrict__ x, i
             }
             float z[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; i++) z[i] = (v[c][i] - b.x) * b.y * sc[c][i] + sh[c][i];
+            for (int i = 0; i < VEC; i++) z[i] = fmaf(CENTER ? (v[c][i] - b.x) * b.y : v[c][i] * b.y, sc[c][i], sh[c][i]);
             o.put(z);
             o.store_streamed(y + (first + i0) * K + col, K - col);
         }
@@ -153,19 +159,19 @@ struct BlockNormSums {
     float *gate, *pw, *w, *b;              // [G * gridDim.x, K], a row a workgroup; any may be NULL
 };
 
-// The same walk. NT: threads of the largest workgroup. Up to 512 a thread has 256 registers, and the next row is loaded ahead;
-// in larger ones (rows that need them) it has 128, and neither that nor the parameters fit. Dynamic LDS: T - 1 teams' sums.
-template <int D, int C, int NT>
-__global__ __launch_bounds__(NT) void bn_bwd(const value_t<D>* __restrict__ x, int64_t ldx, const value_t<D>* __restrict__ h,
+// The same walk. One pack a lane leaves room for the parameters and the next row; two (rows of more than 16 KiB) for neither.
+// Dynamic LDS: T - 1 teams' sums.
+template <int D, int C, bool CENTER>
+__global__ __launch_bounds__(1024) void bn_bwd(const value_t<D>* __restrict__ x, int64_t ldx, const value_t<D>* __restrict__ h,
                                              int64_t ldh, const value_t<D>* __restrict__ dr, int64_t ldr,
                                              const value_t<D>* __restrict__ dy, int64_t ldy, BlockNorm q,
                                              const float4* __restrict__ stats, value_t<D>* __restrict__ dx,
                                              value_t<D>* __restrict__ dh, BlockNormSums sums, int K, int W) {
     constexpr int VEC = Pack<D>::VEC;
-    constexpr bool HOLD = NT <= 512;
+    constexpr bool HOLD = C == 1;
     extern __shared__ float others[];
     __shared__ float red[64];
-    const int wave = threadIdx.x >> 6, teams = (int)blockDim.x / (64 * W), team = wave / W;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), teams = (int)blockDim.x / (64 * W), team = wave / W;
     const int t = (wave % W) * 64 + (threadIdx.x & 63);
     const int64_t g = blockIdx.y, rows = q.rows, first = g * rows, stride = (int64_t)gridDim.x * teams;
     Pack<D> nx[C], nh[C], nr[C], ny[C];
@@ -226,7 +232,8 @@ __global__ __launch_bounds__(NT) void bn_bwd(const value_t<D>* __restrict__ x, i
         for (int c = 0; c < C; c++) px[c] = nx[c], ph[c] = nh[c], pr[c] = nr[c], py[c] = ny[c];
         const float4 st = ns;
         if (HOLD && r0 + stride < rows) fetch(i0 + stride);
-        auto hh = [&](int c, int i) { return (ph[c].get(i) - st.x) * st.y; };
+        // (a mean that is taken off comes off first; RMS has none)
+        auto hh = [&](int c, int i) { return CENTER ? (ph[c].get(i) - st.x) * st.y : ph[c].get(i) * st.y; };
         float rh[C][VEC];                                  // then dR
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
@@ -234,19 +241,26 @@ __global__ __launch_bounds__(NT) void bn_bwd(const value_t<D>* __restrict__ x, i
             if (!HOLD) params(gp[0], sc[0], c);
 #pragma unroll
             for (int i = 0; i < VEC; i++) {                // (past the row's end dy is zero, so every term is)
-                rh[c][i] = (q.scale * px[c].get(i) + hh(c, i) * gp[HOLD ? c : 0][i] - st.z) * st.w;
-                const float d = py[c].get(i), gi = d * sc[HOLD ? c : 0][i];
-                s1 += gi;
-                s2 += gi * rh[c][i];
-                if (on) {
-                    aw[c][i] += d * rh[c][i];
-                    ab[c][i] += d;
-                }
+                const float rv = fmaf(hh(c, i), gp[HOLD ? c : 0][i], q.scale * px[c].get(i));
+                rh[c][i] = CENTER ? (rv - st.z) * st.w : rv * st.w;
+                const float gi = py[c].get(i) * sc[HOLD ? c : 0][i];
+                if (CENTER) s1 += gi;
+                s2 = fmaf(gi, rh[c][i], s2);
             }
         }
+        if (on)
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    const float d = py[c].get(i);
+                    aw[c][i] = fmaf(d, rh[c][i], aw[c][i]);
+                    ab[c][i] += d;
+                }
         if (!back) continue;
         const float2 s = team_sum2(s1, s2, W, red, 0);
-        const float m1 = q.norm == NORM_LAYER ? s.x / (float)K : 0.0f, m2 = s.y / (float)K;
+        // dR = dr + w g - w m1 - w m2 rh, w = 1 / r's root
+        const float m1 = CENTER && q.norm == NORM_LAYER ? st.w * (s.x / (float)K) : 0.0f, m2 = st.w * (s.y / (float)K);
         float s3 = 0.0f, s4 = 0.0f;
 #pragma unroll
         for (int c = 0; c < C; c++) {
@@ -254,12 +268,12 @@ __global__ __launch_bounds__(NT) void bn_bwd(const value_t<D>* __restrict__ x, i
             if (!HOLD) params(gp[0], sc[0], c);
 #pragma unroll
             for (int i = 0; i < VEC; i++) {                // (past the row's end gp is zero, and nothing else is kept)
-                const float d = pr[c].get(i) + st.w * (py[c].get(i) * sc[HOLD ? c : 0][i] - m1 - rh[c][i] * m2);
-                const float z = hh(c, i), tv = d * gp[HOLD ? c : 0][i];
+                float d = fmaf(-m2, rh[c][i], fmaf(py[c].get(i) * sc[HOLD ? c : 0][i], st.w, pr[c].get(i)));
+                if (CENTER) d -= m1;
+                const float tv = d * gp[HOLD ? c : 0][i];
                 rh[c][i] = d;
-                s3 += tv;
-                s4 += tv * z;
-                if (on) ah[c][i] += d * z;
+                if (CENTER) s3 += tv;
+                s4 = fmaf(tv, hh(c, i), s4);
             }
             if (dx && on && col < K) {
                 float v[VEC];
@@ -270,11 +284,16 @@ __global__ __launch_bounds__(NT) void bn_bwd(const value_t<D>* __restrict__ x, i
                 o.store_streamed(dx + (first + i0) * K + col, K - col);
             }
         }
-        float m3 = 0.0f, m4 = 0.0f;
+        if (on)
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int i = 0; i < VEC; i++) ah[c][i] = fmaf(rh[c][i], hh(c, i), ah[c][i]);
+        float m3 = 0.0f, m4 = 0.0f;                        // (both by 1 / h's root)
         if (q.post != NORM_NONE) {
             const float2 u = team_sum2(s3, s4, W, red, 1);
-            m3 = q.post == NORM_LAYER ? u.x / (float)K : 0.0f;
-            m4 = u.y / (float)K;
+            m3 = CENTER && q.post == NORM_LAYER ? st.y * (u.x / (float)K) : 0.0f;
+            m4 = st.y * (u.y / (float)K);
         } else if (W > 1) {
             __syncthreads();                               // (red is written again before the next row's other barrier)
         }
@@ -286,7 +305,10 @@ __global__ __launch_bounds__(NT) void bn_bwd(const value_t<D>* __restrict__ x, i
             if (!HOLD) params(gp[0], sc[0], c);
             float v[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; i++) v[i] = st.y * (rh[c][i] * gp[HOLD ? c : 0][i] - m3 - hh(c, i) * m4);
+            for (int i = 0; i < VEC; i++) {
+                v[i] = fmaf(-m4, hh(c, i), st.y * (rh[c][i] * gp[HOLD ? c : 0][i]));
+                if (CENTER) v[i] -= m3;
+            }
             Pack<D> o;
             o.put(v);
             o.store_streamed(dh + (first + i0) * K + col, K - col);
@@ -344,8 +366,45 @@ __global__ __launch_bounds__(NT) void bn_bwd(const value_t<D>* __restrict__ x, i
 
 constexpr int kBlockNormRow = 32768;     // bytes
 
-static RowShape bn_fwd_shape(int64_t M, int64_t K, int64_t rows, int dt) { return row_shape(M, K, rows, dt, 5, 16, 8); }
-static RowShape bn_bwd_shape(int64_t M, int64_t K, int64_t rows, int dt) { return row_shape(M, K, rows, dt, 8, 8, 2); }
+// A row's waves for `lane_packs` packs a lane, teams up to team_waves waves a workgroup but not so many that CUs are left
+// idle, `wgs` workgroups a CU over all groups. (A lane has two packs at most: 16 waves then hold 32 KiB.)
+static RowShape bn_shape(int64_t packs, int64_t M, int64_t rows, int lane_packs, int team_waves, int cu_waves, int most) {
+    RowShape s;
+    s.waves = (int)std::min<int64_t>(16, (packs + lane_packs - 1) / lane_packs);
+    s.packs = (int)((packs + s.waves - 1) / s.waves);
+    s.teams = (int)std::max<int64_t>(1, std::min<int64_t>(team_waves / s.waves, M / 256));
+    const int64_t wgs = 256 * std::max(1, std::min(most, cu_waves / (s.waves * s.teams)));
+    s.parts = (int)std::min<int64_t>((rows + s.teams - 1) / s.teams, std::max<int64_t>(1, wgs * rows / std::max<int64_t>(1, M)));
+    return s;
+}
+static int64_t bn_packs(int64_t K, int dt) { return (K * value_bytes(dt) + 1023) / 1024; }
+// Forward. Rows up to 4 KiB: one pack a lane, 24 waves a CU; wider ones two packs, 12 waves. us (the same with the other):
+// 5152 x 2048 bfloat16 18.7 (20.3), 20000 x 1024 33.1 (33.8), 16384 x 5120 131 (134): 5.1 TB/s, 3000 x 8192 40.3 (44),
+// 2048 x 5120 float32 33.5 (34.4). Three workgroups of 5 waves a CU, of which two fit at a time: 16384 x 5120 204.
+static RowShape bn_fwd_shape(int64_t M, int64_t K, int64_t rows, int dt) {
+    const int64_t packs = bn_packs(K, dt);
+    return packs <= 4 ? bn_shape(packs, M, rows, 1, 4, 24, 6) : bn_shape(packs, M, rows, 2, 4, 12, 4);
+}
+// Backward. One pack a lane, and one workgroup of 8 waves or a row's a CU, since each writes a row of partial sums and the more of
+// its registers hold data in flight the fewer waves it takes: 16384 x 5120 bfloat16 184 us (5.5 TB/s), 192 with two packs, 197
+// with two workgroups; 5152 x 2048 35 (40, 38); 20000 x 1024 54 (59, 56). Rows of one pack: two workgroups, 30000 x 256 29.2 against
+// 31.6.
+static RowShape bn_bwd_shape(int64_t M, int64_t K, int64_t rows, int dt) {
+    const int64_t packs = bn_packs(K, dt);
+    return bn_shape(packs, M, rows, packs <= 16 ? 1 : 2, 8, packs == 1 ? 16 : 8, 2);
+}
+
+// f(packs a lane, whether a mean is taken off) as constants
+template <typename F>
+static void bn_forms(const RowShape& z, bool center, F&& f) {
+    using std::integral_constant;
+    auto by = [&](auto c) {
+        if (z.packs == 1) f(integral_constant<int, 1>{}, c);
+        else f(integral_constant<int, 2>{}, c);
+    };
+    if (center) by(std::true_type{});
+    else by(std::false_type{});
+}
 
 static int bn_check(const char* who, const wf_block_norm* q, int64_t M, int64_t K) {
     if (!q || M < 0 || K <= 0 || q->groups <= 0 || M % q->groups || (q->post < NORM_NONE || q->post > NORM_LAYER) ||
@@ -389,15 +448,12 @@ extern "C" int wf_block_norm_fwd(const wf_block_norm* q, const void* x, int64_t 
     by_dtype(q->dt, [&](auto d) {
         constexpr int D = decltype(d)::value;
         const RowShape z = bn_fwd_shape(M, K, p.rows, D);
-        auto go = [&](auto c, auto nt) {
-            bn_fwd<D, decltype(c)::value, decltype(nt)::value><<<dim3(z.parts, (uint32_t)q->groups), 64 * z.waves * z.teams, 0, s>>>(
+        auto go = [&](auto c, auto center) {
+            bn_fwd<D, decltype(c)::value, decltype(center)::value><<<dim3(z.parts, (uint32_t)q->groups), 64 * z.waves * z.teams, 0, s>>>(
                 static_cast<const value_t<D>*>(x), x_row, static_cast<const value_t<D>*>(h), h_row, p,
                 static_cast<value_t<D>*>(r), static_cast<value_t<D>*>(y), reinterpret_cast<float4*>(stats), (int)K, z.waves);
         };
-        using std::integral_constant;
-        if (z.waves * z.teams > 8) go(integral_constant<int, 2>{}, integral_constant<int, 1024>{});
-        else if (z.packs == 1) go(integral_constant<int, 1>{}, integral_constant<int, 512>{});
-        else go(integral_constant<int, 2>{}, integral_constant<int, 512>{});
+        bn_forms(z, q->post == NORM_LAYER || q->norm == NORM_LAYER, go);
     });
     WF_LAUNCH_CHECK("wf_block_norm_fwd launch");
     return WF_OK;
@@ -449,19 +505,16 @@ extern "C" int wf_block_norm_bwd(const wf_block_norm* q, const void* x, int64_t 
     const hipStream_t s = static_cast<hipStream_t>(stream);
     by_dtype(q->dt, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        auto go = [&](auto c, auto nt) {
+        auto go = [&](auto c, auto center) {
             constexpr int C = decltype(c)::value;
             const uint32_t lds = (uint32_t)(z.teams - 1) * 3 * C * Pack<D>::VEC * 64 * z.waves * 4;
-            bn_bwd<D, C, decltype(nt)::value><<<dim3(z.parts, (uint32_t)q->groups), 64 * z.waves * z.teams, count ? lds : 0, s>>>(
+            bn_bwd<D, C, decltype(center)::value><<<dim3(z.parts, (uint32_t)q->groups), 64 * z.waves * z.teams, count ? lds : 0, s>>>(
                 static_cast<const value_t<D>*>(x), x_row, static_cast<const value_t<D>*>(h), h_row,
                 static_cast<const value_t<D>*>(dr), dr_row, static_cast<const value_t<D>*>(dy), dy_row, p,
                 reinterpret_cast<const float4*>(stats), static_cast<value_t<D>*>(dx), static_cast<value_t<D>*>(dh), b, (int)K,
                 z.waves);
         };
-        using std::integral_constant;
-        if (z.waves * z.teams > 8) go(integral_constant<int, 2>{}, integral_constant<int, 1024>{});
-        else if (z.packs == 1) go(integral_constant<int, 1>{}, integral_constant<int, 512>{});
-        else go(integral_constant<int, 2>{}, integral_constant<int, 512>{});
+        bn_forms(z, q->post == NORM_LAYER || q->norm == NORM_LAYER, go);
     });
     WF_LAUNCH_CHECK("wf_block_norm_bwd launch");
     if (count) {

@@ -58,6 +58,7 @@ CASES = [
     (4, 8192, "float32", "float32", "pgwb", 2, 2), (700, 8189, "float32", "float32", "pgwb", 1, 1),
     (3000, 64, "bfloat16", "bfloat16", "pgwb", 1, 1), (2000, 513, "float32", "float32", "pgwb", 4, 4),
     (1200, 320, "float16", "float16", "pgwb", 600, 600), (1030, 4096, "bfloat16", "bfloat16", "pgwb", 1, 1),
+    (2100, 250, "bfloat16", "bfloat16", "pgwb", 3, 3), (2600, 500, "float32", "float32", "pgwb", 1, 1),
     (2100, 1000, "bfloat16", "bfloat16", "pgwb", 1, 1), (1500, 2040, "float16", "float32", "pgwb", 1, 1),
     (777, 6144, "bfloat16", "bfloat16", "pgwb", 1, 1), (530, 7168, "float16", "float16", "pw", 1, 1)]
 
