@@ -72,6 +72,13 @@ EXPORTS = {
                                       _int, _int, ctypes.POINTER(_i64)]),
     "wf_dense_bwd": (_int, [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _int, _int, _p, _int, _i64, _i64, _i64, _i64, _p, _p,
                             _p, _int, _p, _p, _i64, _p]),
+    "wf_gated_dense_plan": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _int, ctypes.POINTER(_int),
+                                   ctypes.POINTER(_i64)]),
+    "wf_gated_dense": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _p, _int, _int, _p, _p, _p, _i64, _p]),
+    "wf_gated_dense_bwd_workspace": (_int, [_p, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _int, _int, _int,
+                                            ctypes.POINTER(_i64)]),
+    "wf_gated_dense_bwd": (_int, [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _int, _int, _i64, _i64, _i64, _p, _p, _p, _int, _p,
+                                  _i64, _p]),
     "wf_adamw": (_int, [_p, _i64, _int, _int, _p, _p, _p, _p, _i64, _i64] + [ctypes.c_double] * 5 + [_p]),
     "wf_adamw_values": (_int, [_p, _p, _p, _p, _i64, _p, _p, _p]),
     "wf_host_alloc": (_int, [_sz, ctypes.POINTER(ctypes.c_void_p)]),

@@ -16,7 +16,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "dense_gemm.h"
+#include "dense_call.h"
 #include "dense_grad.h"
 #include "dense_rows.h"
 #include "grids.h"
@@ -103,32 +103,26 @@ __global__ __launch_bounds__(256) void dense_pack(const uint16_t* __restrict__ p
 // faster than a whole one, which the power limit holds back; operands stream at 4.6 TB/s, less with few workgroups; a second
 // kernel adds the slices. The way it chooses took 3 % longer than the best measured one on average over the 60 (shape,
 // order) pairs, at most 21 % (2048 x 2048 x 256, 8.0 against 6.6 us).
-struct DenseTiling {
-    int bm, bn, per_cu;
-    float fixed, stage, shared;
-};
 constexpr DenseTiling kDense[] = {{256, 320, 1, 2.2f, 1.65f, 1.65f},    {256, 256, 1, 3.0f, 1.252f, 1.252f},
                                   {256, 192, 1, 1.8f, 1.076f, 1.076f},  {128, 192, 2, 0.8f, 0.785f, 0.694f},
                                   {128, 160, 2, 1.6f, 0.72f, 0.606f},   {128, 128, 2, 1.5f, 0.634f, 0.519f},
                                   {64, 128, 3, 0.8f, 0.47f, 0.367f},    {32, 128, 3, 1.6f, 0.435f, 0.315f}};
 
-// What an epilogue adds to a workgroup's time: an activation's arithmetic, the kept pre-activations' stores, the residual's
-// loads. Eight waves hide more of it than four, and workgroups that share a CU hide each other's: 4096 x 13824 x 5120 with
+// What an epilogue adds to a workgroup's time. Eight waves hide more of it than four, and workgroups that share a CU hide each other's: 4096 x 13824 x 5120 with
 // GELU 465 us in 256 x 320 tiles, 486 in 256 x 256, which without it are as fast.
-enum { EPI_ACT = 1, EPI_KEEP = 2, EPI_MORE = 4 };
 static float dense_epilogue_time(const DenseTiling& q, int epilogue) {
     const float us = (epilogue & EPI_ACT ? 5.0f : 0.0f) + (epilogue & EPI_KEEP ? 10.0f : 0.0f) +
                      (epilogue & EPI_MORE ? 8.0f : 0.0f);
     return us * (float)(q.bm * q.bn) / 65536.0f * (q.bn == 320 ? 0.5f : q.per_cu > 1 ? 0.75f : 1.0f);
 }
 
-static DensePlan dense_plan_tiles(int64_t M, int64_t N, int64_t K, int epilogue, float& us) {
+DensePlan dense_plan_tiles(const DenseTiling* tilings, int count, int64_t M, int64_t N, int64_t K, int epilogue, float& us) {
     const int64_t stages = (K + 63) / 64;
     DensePlan best = {0, 1, (int)stages};
     us = 1e30f;
     const float bytes = (float)(M * K + N * K) * 2.0f;
-    for (int t = 0; t < (int)(sizeof(kDense) / sizeof(kDense[0])); t++) {
-        const DenseTiling& q = kDense[t];
+    for (int t = 0; t < count; t++) {
+        const DenseTiling& q = tilings[t];
         const int64_t tiles = ((M + q.bm - 1) / q.bm) * ((N + q.bn - 1) / q.bn);
         for (int want : {1, 2, 3, 4, 6, 8, 12, 16}) {
             const int64_t per = (stages + want - 1) / want, slices = (stages + per - 1) / per;
@@ -158,7 +152,7 @@ static DensePlan dense_plan_tiles(int64_t M, int64_t N, int64_t K, int epilogue,
 // nearly twice where odd row lengths put the 16-byte loads at odd places (`odd`).
 // 1 x 13824 x 5120 30 us, 16 x 2048 x 8192 12 (the tiles 19), 128 x 1000 x 1024 5.1 (8.0), 12 x 5896 x 9106 36 (75 with the
 // copies that the tiles need); 16 x 5120 x 5120 20 (17), 77 x 2607 x 1531 24 (20).
-static float dense_rows_time(int64_t M, int64_t N, int64_t K, bool odd) {
+float dense_rows_time(int64_t M, int64_t N, int64_t K, bool odd) {
     const float fill = 1.0f + 0.6f * (float)std::min<int64_t>(M - 1, 15) / 15.0f;
     const int64_t groups = (M + 15) / 16;
     return 4.0f + (float)(N * K) * 2.0f / 5.2e6f * fill * (groups > 1 ? 0.87f * (float)groups : 1.0f) * (odd ? 1.9f : 1.0f);
@@ -172,23 +166,12 @@ static DenseRowsPlan dense_plan_rows(int64_t M, int64_t N, int64_t K) {
     return K >= 4096 ? DenseRowsPlan{2, 4} : DenseRowsPlan{1, 1};
 }
 
-static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-
-struct DenseView {                                    // value (r, k) at r * row + k * col
-    const void* p;
-    int64_t row, col;
-    bool zeros;                                       // along K: rows hold zeros from K up to the next multiple of 8
-};
-
 constexpr int64_t kRowsMost = 256;
 
-// How an operand gets to the tiles: as it lies along K or across it, or copied into rows that can be loaded, which keeps
-// that order (along, across) or turns it (any strides, to rows along K).
-enum { LIES_ALONG, LIES_ACROSS, COPY_ALONG, COPY_ACROSS, COPY_TURNED };
 static bool is_across(int how) { return how == LIES_ACROSS || how == COPY_ACROSS; }
 
 // may_cross: whether the operand may lie across K
-static int dense_how(const DenseView& v, int64_t R, int64_t K, bool may_cross) {
+int dense_how(const DenseView& v, int64_t R, int64_t K, bool may_cross) {
     const bool a16 = aligned(v.p, 16);
     if (v.col == 1 && (R == 1 || v.row >= K)) {
         return v.row % 8 == 0 && (K % 8 == 0 || v.zeros) && v.row <= (1 << 20) && a16 ? LIES_ALONG : COPY_ALONG;
@@ -200,28 +183,16 @@ static int dense_how(const DenseView& v, int64_t R, int64_t K, bool may_cross) {
 static int64_t dense_copy_row(int how, int64_t R, int64_t K) {
     return how == COPY_ALONG ? up(K, 8) : how == COPY_ACROSS ? up(R, 8) : up(K, 64);
 }
-static int64_t dense_copy_bytes(int how, int64_t R, int64_t K) {
+int64_t dense_copy_bytes(int how, int64_t R, int64_t K) {
     if (how == LIES_ALONG || how == LIES_ACROSS) return 0;
     return up((how == COPY_ACROSS ? K : R) * dense_copy_row(how, R, K) * 2, 256);
 }
 
-// How a product runs: in the few-rows form, or in tiles.
-struct DenseCall {
-    bool few;
-    DenseRowsPlan rows;
-    DensePlan tiles;
-    int how_x, how_w;
-    int epilogue;                                     // 0: at most a bias
-    bool summed;                                      // float32 partial sums first: slices, or operands across K with more
-    int64_t w_at, parts_at, bytes;                    // than a plain epilogue. Offsets into the workspace, x's copy first
-    int slices() const { return few ? rows.slices : tiles.slices; }
-};
-
-static DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, int64_t N, int64_t K, int epilogue) {
+DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, int64_t N, int64_t K, int epilogue) {
     DenseCall d = {};
     d.epilogue = epilogue;
     float us;
-    d.tiles = dense_plan_tiles(M, N, K, epilogue, us);
+    d.tiles = dense_plan_tiles(kDense, (int)(sizeof(kDense) / sizeof(kDense[0])), M, N, K, epilogue, us);
     d.how_w = dense_how(w, N, K, true);
     d.how_x = dense_how(x, M, K, is_across(d.how_w));
     int64_t copies = dense_copy_bytes(d.how_x, M, K);
@@ -262,6 +233,16 @@ static DenseOperand dense_operand(const DenseView& v, int how, int64_t R, int64_
     return {out, to, (int)to, (int)R, false};
 }
 
+void dense_operands(const DenseView& x, int how_x, int64_t M, char* x_out, const DenseView& w, int how_w, int64_t N, char* w_out,
+                    int64_t K, DenseOperand& a, DenseOperand& b, hipStream_t s) {
+    PackRows jx = {}, jw = {};
+    a = dense_operand(x, how_x, M, K, reinterpret_cast<uint16_t*>(x_out), jx, s);
+    b = dense_operand(w, how_w, N, K, reinterpret_cast<uint16_t*>(w_out), jw, s);
+    over_grids((std::max(jx.runs, jw.runs) + 255) / 256, kGridMost, [&](int64_t wg, uint32_t n) {
+        dense_pack_rows<<<dim3(n, jx.runs && jw.runs ? 2 : 1), 256, 0, s>>>(wg, jx.runs ? jx : jw, jw);
+    });
+}
+
 // the tiled kernel of a call (dense_gemm.h has one source each), as wf_dense_plan numbers them; 0 is the few-rows form
 enum { FORM_ROWS, FORM_ALONG, FORM_ALONG_FULL, FORM_B_ACROSS, FORM_ACROSS };
 static int dense_form(const DenseCall& d) {
@@ -271,19 +252,15 @@ static int dense_form(const DenseCall& d) {
     return d.epilogue && !d.summed ? FORM_ALONG_FULL : FORM_ALONG;
 }
 
-static void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w, int dt, int64_t M, int64_t N, int64_t K,
+void dense_run(const DenseCall& d, const DenseView& x, const DenseView& w, int dt, int64_t M, int64_t N, int64_t K,
                       char* ws, const DenseEpilogue& e, hipStream_t s) {
     float* parts = d.summed ? reinterpret_cast<float*>(ws + d.parts_at) : nullptr;
     if (d.few) {
         dense_rows_run(dt, d.rows, static_cast<const uint16_t*>(x.p), x.row, static_cast<const uint16_t*>(w.p), w.row, (int)M,
                        (int)N, (int)K, parts, e, s);
     } else {
-        PackRows jx = {}, jw = {};
-        const DenseOperand a = dense_operand(x, d.how_x, M, K, reinterpret_cast<uint16_t*>(ws), jx, s);
-        const DenseOperand b = dense_operand(w, d.how_w, N, K, reinterpret_cast<uint16_t*>(ws + d.w_at), jw, s);
-        over_grids((std::max(jx.runs, jw.runs) + 255) / 256, kGridMost, [&](int64_t wg, uint32_t n) {
-            dense_pack_rows<<<dim3(n, jx.runs && jw.runs ? 2 : 1), 256, 0, s>>>(wg, jx.runs ? jx : jw, jw);
-        });
+        DenseOperand a, b;
+        dense_operands(x, d.how_x, M, ws, w, d.how_w, N, ws + d.w_at, K, a, b, s);
         const int form = dense_form(d);
         auto run = form == FORM_ACROSS ? dense_gemm_across : form == FORM_B_ACROSS ? dense_gemm_b_across
                    : form == FORM_ALONG ? dense_gemm_along : dense_gemm_along_full;
@@ -324,7 +301,7 @@ static DenseBackward dense_backward(const void* x, int64_t x_row, const void* w,
     return b;
 }
 
-static int dense_check(const char* who, int dt, int64_t M, int64_t N, int64_t K, int64_t x_row, int64_t x_col,
+int dense_check(const char* who, int dt, int64_t M, int64_t N, int64_t K, int64_t x_row, int64_t x_col,
                        int64_t w_row, int64_t w_col) {
     if (M < 0 || N < 0 || K <= 0 || x_row < 0 || x_col < 0 || w_row < 0 || w_col < 0) {
         set_error("%s: M, N, K = %lld, %lld, %lld or a negative stride", who, (long long)M, (long long)N, (long long)K);

@@ -139,15 +139,53 @@ struct DenseAcross {
     }
 };
 
-// acc[i][j] over the nk stages from stage s0. AX, BX: whether A and B lie across K. mma(acc, a, b) returns acc + a . b.
-template <typename S, bool AX, bool BX, typename Mma>
-__device__ __forceinline__ void dense_mainloop(const DenseTile& ta, const DenseTile& tb, int s0, int nk, int wave,
-                                               int lane, wl_frag* sb0, wl_frag* sb1, f32x16v (&acc)[S::WM][S::WN],
-                                               Mma&& mma) {
+// An operand of two matrices of the same rows, both along K, as one tile: its fragments of 32 rows come from the first and the
+// second in turn, so that a wave holds the sums of a column of both (the gated linear's gate and its other half).
+struct DensePair {
+    __amdgpu_buffer_rsrc_t r[2];
+    uint32_t row, k;
+};
+template <int B, int NW, int LW, int W>
+struct DenseAlongPair {
+    __amdgpu_buffer_rsrc_t r[2];
+    uint32_t lane_at, tail, step;
+    int base, last;
+
+    // load q covers rows 8 wave .. 8 wave + 7 of fragment q of the tile, rows 32 (q / 2) on of matrix q % 2
+    __device__ __forceinline__ void init(const DensePair& t, int lane, int wave, int t0) {
+        static_assert(NW == 4, "a load of each wave is a fragment's rows");
+        const int row = 8 * wave + lane / 8;
+        const uint32_t c = 16u * (uint32_t)swz8(row, lane % 8);
+        r[0] = t.r[0];
+        r[1] = t.r[1];
+        lane_at = (uint32_t)row * t.row + c;
+        step = 32u * t.row;
+        last = (int)((t.k - 1) / 128);
+        tail = (uint32_t)last * 128u + c < t.k ? lane_at : 0x80000000u;      // past every buffer's end: zeros
+        const int lr = lane & 31;
+        base = (t0 * 32 + lr) * 8 + swz8(lr, lane >> 5);
+    }
+    __device__ __forceinline__ void begin(int kt) {
+        if (kt >= last) lane_at = tail;
+    }
+    template <int Q>
+    __device__ __forceinline__ void load(wl_frag* st, int wave, int kt) const {
+        lds_dma16(r[Q & 1], st + 64 * (Q * NW + wave), lane_at + (uint32_t)(Q >> 1) * step + (uint32_t)kt * 128u);
+    }
+    template <int I>
+    __device__ __forceinline__ wl_frag read(const wl_frag* st, int ks) const {
+        return (st + (base ^ (2 * ks)))[I * 256];
+    }
+};
+
+// acc[i][j] over the nk stages from stage s0; LA, LB load A's and B's tiles ta and tb. mma(acc, a, b) returns acc + a . b.
+template <typename S, typename LA, typename LB, typename TA, typename TB, typename Mma>
+__device__ __forceinline__ void dense_loop(const TA& ta, const TB& tb, int s0, int nk, int wave, int lane, wl_frag* sb0,
+                                           wl_frag* sb1, f32x16v (&acc)[S::WM][S::WN], Mma&& mma) {
     constexpr int WM = S::WM, WN = S::WN, AW = S::AW, BW = S::BW, IPW = AW + BW;
     constexpr int READS = WM + WN, MFMAS = WM * WN;
-    std::conditional_t<AX, DenseAcross<S::BM, S::NW, AW, WM>, DenseAlong<S::BM, S::NW, AW, WM>> a;
-    std::conditional_t<BX, DenseAcross<S::BN, S::NW, BW, WN>, DenseAlong<S::BN, S::NW, BW, WN>> b;
+    LA a;
+    LB b;
     a.init(ta, lane, wave, wave / S::VN * WM);
     b.init(tb, lane, wave, wave % S::VN * WN);
     auto issue = [&](wl_frag* st, int kt, auto qc) {               // load q of this wave's IPW of stage kt
@@ -234,6 +272,16 @@ __device__ __forceinline__ void dense_mainloop(const DenseTile& ta, const DenseT
     wait_vm<0>();                                        // the stage buffers are idle from here on
     __builtin_amdgcn_s_waitcnt(0xc07f);
     wave_barrier_sync();
+}
+
+// AX, BX: whether A and B lie across K
+template <typename S, bool AX, bool BX, typename Mma>
+__device__ __forceinline__ void dense_mainloop(const DenseTile& ta, const DenseTile& tb, int s0, int nk, int wave,
+                                               int lane, wl_frag* sb0, wl_frag* sb1, f32x16v (&acc)[S::WM][S::WN],
+                                               Mma&& mma) {
+    using LA = std::conditional_t<AX, DenseAcross<S::BM, S::NW, S::AW, S::WM>, DenseAlong<S::BM, S::NW, S::AW, S::WM>>;
+    using LB = std::conditional_t<BX, DenseAcross<S::BN, S::NW, S::BW, S::WN>, DenseAlong<S::BN, S::NW, S::BW, S::WN>>;
+    dense_loop<S, LA, LB>(ta, tb, s0, nk, wave, lane, sb0, sb1, acc, mma);
 }
 
 }  // namespace wf

@@ -1,0 +1,383 @@
+// The gated feed-forward layer's first half for gfx950: y = act(x wg^T + bg) * (x wu^T + bu), both projections, the activation and
+// the product in one kernel, and its backward pass. The weight is [2 N, K], the gate's N rows first.
+//
+//   g, u = the two halves of x w^T + bias,  y = act(g) u
+//   dg = dy u act'(g),  du = dy act(g),  dx = [dg du] w,  dw = [dg du]^T x,  dbias = the column sums of [dg du]
+//
+// 4 M N K operations forward. The tiles are those of the 16-bit linear (dense_gemm.h), but a tile's rows of the weight are fragments of 32
+// from the gate's half and from the other in turn, so that a wave's accumulators hold g and u of the same outputs: the epilogue
+// is arithmetic on registers, and neither g nor u goes to memory unless the backward pass will want them (gated.h has the format). A
+// product with too few tiles runs as slices of K, whose float32 sums a second kernel adds before the epilogue; few rows of x take
+// the form of dense_rows.hip with a tile of each half a workgroup.
+//
+// Backward: one element-wise kernel from dy and the kept g and u to [dg du], [M, 2 N], rounded to the operands' type because it is the
+// operand of the two products behind it, which are the 16-bit linear's own on a weight of 2 N rows.
+
+#include <algorithm>
+#include <type_traits>
+
+#include "column_sums.h"
+#include "dense_call.h"
+#include "grids.h"
+
+namespace wf {
+
+// a, b: x and the weight's first half, along K; half: values from a row of the first half to the same of the second. Workgroup
+// (tile, slice); parts: [slices, M, 2 N] float32 partial sums, or NULL: one slice, and the outputs.
+template <int D, typename S>
+__global__ __launch_bounds__(S::NT, S::WAVES) void gated_gemm(DenseOperand a, DenseOperand b, int64_t half, int M, int N, int K,
+                                                              int slice_stages, float* __restrict__ parts, GatedEpilogue e) {
+    constexpr int WM = S::WM, WN = S::WN, TC = WN * 16, BO = S::BN / 2;    // outputs of a wave's row, of a tile's
+    static_assert(WN % 2 == 0, "a fragment of each half");
+    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS];
+    const int ntm = (M + S::BM - 1) / S::BM, ntn = (N + BO - 1) / BO;
+    int tm, tn;
+    tile_order(blockIdx.x, ntm * ntn, ntm, ntn, tm, tn);
+    const int m0 = __builtin_amdgcn_readfirstlane(tm * S::BM), n0 = __builtin_amdgcn_readfirstlane(tn * BO);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int stages = (K + 63) / 64, s0 = blockIdx.y * slice_stages, nk = min(slice_stages, stages - s0);
+    const DenseTile ta = dense_tile<false>(a, m0), tg = dense_tile<false>(b, n0);
+    b.p += half;
+    const DensePair tb = {{tg.r, dense_tile<false>(b, n0).r}, tg.row, tg.k};
+    const int mw = m0 + wave / S::VN * WM * 32, nw = n0 + wave % S::VN * TC;
+    const int lr = lane & 31, lk = lane >> 5;
+    // the sums start from the bias
+    f32x16v acc[WM][WN];
+#pragma unroll
+    for (int j = 0; j < WN; j++) {
+        const int n = nw + j / 2 * 32 + lr;
+        const float bn = !parts && e.bias && n < N ? load_value(e.bias, (int64_t)(j & 1) * N + n, e.bias_dt) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < WM; i++)
+#pragma unroll
+            for (int x = 0; x < 16; x++) acc[i][j][x] = bn;
+    }
+    dense_loop<S, DenseAlong<S::BM, S::NW, S::AW, WM>, DenseAlongPair<S::BN, S::NW, S::BW, WN>>(
+        ta, tb, s0, nk, wave, lane, sb0, sb1, acc, [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<D>(c, x, y); });
+    if (parts) {                                                   // (32 lanes store 128 bytes of a row)
+        float* o = parts + (int64_t)blockIdx.y * M * 2 * N;
+#pragma unroll
+        for (int i = 0; i < WM; i++)
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+                const int m = mw + 32 * i + 8 * (x >> 2) + 4 * lk + (x & 3);
+                if (m >= M) continue;
+#pragma unroll
+                for (int j = 0; j < WN; j++) {
+                    const int n = nw + j / 2 * 32 + lr;
+                    if (n < N) o[((int64_t)m * 2 + (j & 1)) * N + n] = acc[i][j][x];
+                }
+            }
+        return;
+    }
+    uint16_t* o16 = wl_out_region<S>(sb0, sb1, wave);
+    auto store = [&](uint16_t* out, auto&& f) {
+        wl_store_tile<WM, WN / 2>(o16, out, M, N, mw, nw, lane,
+                                  [&](int i, int j, int x) { return f(acc[i][2 * j][x], acc[i][2 * j + 1][x]); });
+    };
+    if (e.kept) {
+        store(e.kept, [](float g, float) { return kept_upper(kept_bits(g)); });
+        store(e.kept + e.plane, [](float, float u) { return kept_upper(kept_bits(u)); });
+        store(e.kept + 2 * e.plane, [](float g, float u) { return kept_lower(kept_bits(g), kept_bits(u)); });
+    }
+    by_act(e.act, [&](auto k) {
+        store(static_cast<uint16_t*>(e.y), [](float g, float u) { return from_f32<D>(act_of<decltype(k)::value>(g) * u); });
+    });
+}
+
+// the slices' sums in slice order, then the epilogue: one run of 8 outputs a thread, from workgroup `wg` of the whole on
+template <int D>
+__global__ __launch_bounds__(256) void gated_sum(int64_t wg, const float* __restrict__ parts, int slices, int M, int N,
+                                                 GatedEpilogue e) {
+    const int runs = (N + 7) / 8;
+    const int64_t i = (wg + blockIdx.x) * 256 + threadIdx.x;
+    if (i >= (int64_t)M * runs) return;
+    const int64_t m = i / runs;
+    const int n = (int)(i - m * runs) * 8, cnt = N - n;
+    const float* p = parts + m * 2 * N + n;
+    const int64_t plane = (int64_t)M * 2 * N;
+    auto load = [&](float (&v)[8], const float* q) {
+        if (cnt >= 8) __builtin_memcpy(v, q, 32);
+        else
+#pragma unroll
+            for (int x = 0; x < 8; x++) v[x] = x < cnt ? q[x] : 0.0f;
+    };
+    float g[8] = {0, 0, 0, 0, 0, 0, 0, 0}, u[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int s = 0; s < slices; s += 2) {                          // two slices' loads in flight, added in order
+        float a[2][8], b[2][8];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int64_t at = min(s + k, slices - 1) * plane;
+            load(a[k], p + at);
+            load(b[k], p + at + N);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            if (s + k < slices)
+#pragma unroll
+                for (int x = 0; x < 8; x++) g[x] += a[k][x], u[x] += b[k][x];
+    }
+    gated_run<D>(e, g, u, m, n, N, cnt);
+}
+
+// The backward pass's element-wise part: workgroup (512 columns, i) walks rows 4 i + wave, + 4 gridDim.y, ...; bparts:
+// [gridDim.y, 2 N] float32 sums of the unrounded dg and du, or NULL. dh: [M, ldh], ldh a multiple of 8, zeros past 2 N, or NULL.
+template <int D>
+__global__ __launch_bounds__(256) void gated_dact(const value_t<D>* __restrict__ dy, int64_t ldd, const uint16_t* __restrict__ kept,
+                                                  int64_t plane, int act, value_t<D>* __restrict__ dh, int64_t ldh,
+                                                  float* __restrict__ bparts, int M, int N) {
+    __shared__ float red[4][2][512];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = blockIdx.x * 512 + lane * 8, cnt = N - n;
+    float sg[8], su[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) sg[i] = su[i] = 0.0f;
+    for (int64_t m = blockIdx.y * 4 + wave; m < M && cnt > 0; m += gridDim.y * 4) {
+        const int64_t at = m * N + n;
+        Pack<D> pd;
+        Pack<WF_BF16> pg, pu, pl;
+        pd.load(dy + m * ldd + n, cnt);
+        pg.load(kept + at, cnt);
+        pu.load(kept + plane + at, cnt);
+        pl.load(kept + 2 * plane + at, cnt);
+        float g[8], a[8], slope[8], dg[8], du[8];
+        auto half = [](const Pack<WF_BF16>& p, int i) { return i & 1 ? p.w[i / 2] >> 16 : p.w[i / 2] & 0xffffu; };
+#pragma unroll
+        for (int i = 0; i < 8; i++) g[i] = kept_g(half(pg, i), half(pl, i));
+        act_slope_run(act, g, a, slope);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float d = pd.get(i);
+            dg[i] = d * kept_u(half(pu, i), half(pl, i)) * slope[i];
+            du[i] = d * a[i];
+            sg[i] += dg[i];
+            su[i] += du[i];
+        }
+        if (!dh) continue;
+        Pack<D> o;
+        value_t<D>* row = dh + m * ldh;
+        o.put(dg);
+        o.store(row + n, cnt);
+        o.put(du);
+        o.store(row + N + n, cnt);
+        if (cnt <= 8)                                              // a row's last run writes its padding too
+            for (int64_t k = 2 * (int64_t)N; k < ldh; k++) row[k] = from_f32<D>(0.0f);
+    }
+    if (!bparts) return;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        red[wave][0][lane * 8 + i] = sg[i];
+        red[wave][1][lane * 8 + i] = su[i];
+    }
+    __syncthreads();
+    float* out = bparts + (int64_t)blockIdx.y * 2 * N;
+    for (int c = threadIdx.x; c < 512; c += 256) {
+        const int col = blockIdx.x * 512 + c;
+        if (col >= N) continue;
+        out[col] = red[0][0][c] + red[1][0][c] + red[2][0][c] + red[3][0][c];
+        out[N + col] = red[0][1][c] + red[1][1][c] + red[2][1][c] + red[3][1][c];
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- host side
+// rows of x and of the weight (both halves) a tile
+constexpr DenseTiling kGated[] = {{256, 256, 1, 3.0f, 1.252f, 1.252f}, {128, 256, 1, 1.8f, 0.70f, 0.70f},
+                                  {128, 128, 2, 1.5f, 0.634f, 0.519f}, {64, 256, 2, 1.2f, 0.60f, 0.50f},
+                                  {32, 256, 2, 1.6f, 0.55f, 0.42f}};
+
+template <int D>
+static void gated_tiling(const DenseOperand& a, const DenseOperand& b, int64_t half, int M, int N, int K, const DensePlan& p,
+                         float* parts, const GatedEpilogue& e, hipStream_t s) {
+    auto go = [&](auto shape) {
+        using S = decltype(shape);
+        const int tiles = ((M + S::BM - 1) / S::BM) * ((N + S::BN / 2 - 1) / (S::BN / 2));
+        gated_gemm<D, S><<<dim3(tiles, p.slices), S::NT, 0, s>>>(a, b, half, M, N, K, p.slice_stages, parts, e);
+    };
+    switch (p.tiling) {
+    case 0: go(DenseShape<2, 2, 4, 4>{}); break;
+    case 1: go(DenseShape<2, 2, 2, 4>{}); break;
+    case 2: go(DenseShape<2, 2, 2, 2>{}); break;
+    case 3: go(DenseShape<1, 4, 2, 2>{}); break;
+    default: go(DenseShape<1, 4, 1, 2>{}); break;
+    }
+}
+
+// How a call runs: few rows, or tiles in slices of K; where the copies of operands that cannot be loaded as they lie and the
+// partial sums are in the workspace.
+struct GatedCall {
+    bool few;
+    int slices;
+    DensePlan tiles;
+    int how_x, how_w;
+    int64_t w_at, parts_at, bytes;
+};
+static GatedCall gated_call(const DenseView& x, const DenseView& w, int64_t M, int64_t N, int64_t K, bool keep) {
+    GatedCall c = {};
+    float us;
+    c.tiles = dense_plan_tiles(kGated, (int)(sizeof(kGated) / sizeof(kGated[0])), M, 2 * N, K, EPI_ACT | (keep ? EPI_KEEP : 0), us);
+    c.slices = c.tiles.slices;
+    c.how_x = dense_how(x, M, K, false);
+    c.how_w = dense_how(w, 2 * N, K, false);
+    c.w_at = dense_copy_bytes(c.how_x, M, K);
+    c.parts_at = c.w_at + dense_copy_bytes(c.how_w, 2 * N, K);
+    if (c.w_at) us += 3.0f + (float)c.w_at * 0.5e-6f;
+    if (c.parts_at > c.w_at) us += 3.0f + (float)(c.parts_at - c.w_at) * 0.5e-6f;
+    if (M <= 256 && x.col == 1 && w.col == 1 && dense_rows_time(M, 2 * N, K, ((x.row | w.row) & 1) != 0) < us) {
+        c.few = true;
+        c.slices = (N + 15) / 16 * ((M + 15) / 16) < 128 && K >= 4096 ? 4 : 1;
+        c.w_at = c.parts_at = 0;
+    }
+    c.bytes = c.parts_at + (c.slices > 1 ? (int64_t)c.slices * M * 2 * N * 4 : 0);
+    return c;
+}
+
+struct GatedBackward {
+    int64_t dh_row, sums_at, product_at, bytes;
+    int rows;                                          // of partial sums
+    DenseView dh_along, w_turned, dh_turned, x_turned;
+    DenseCall dx, dw;
+};
+static GatedBackward gated_backward(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, int64_t M,
+                                    int64_t N, int64_t K, bool dx, bool dw, bool db, char* ws) {
+    GatedBackward b = {};
+    b.dh_row = up(2 * N, 8);
+    b.rows = (int)std::min<int64_t>((M + 3) / 4, std::max<int64_t>(1, 2048 / ((N + 511) / 512)));
+    b.sums_at = dx || dw ? up(M * b.dh_row * 2, 256) : 0;
+    b.product_at = b.sums_at + (db ? up((int64_t)b.rows * 2 * N * 4, 256) : 0);
+    b.dh_along = {ws, b.dh_row, 1, true};              // (a workspace not yet there is as aligned as it will be)
+    b.w_turned = {w, w_col, w_row, false};
+    b.dh_turned = {ws, 1, b.dh_row, false};
+    b.x_turned = {x, 1, x_row, false};
+    if (dx) b.dx = dense_call(b.dh_along, b.w_turned, M, K, 2 * N, 0);
+    if (dw) b.dw = dense_call(b.dh_turned, b.x_turned, 2 * N, K, M, 0);
+    b.bytes = b.product_at + std::max(b.dx.bytes, b.dw.bytes);
+    return b;
+}
+
+static int gated_check(const char* who, int dt, int act, int64_t M, int64_t N, int64_t K, int64_t x_row, int64_t x_col,
+                       int64_t w_row, int64_t w_col) {
+    if (const int rc = dense_check(who, dt, M, N, K, x_row, x_col, w_row, w_col)) return rc;
+    if (act < ACT_NONE || act > ACT_RELU) { set_error("%s: activation %d", who, act); return WF_EINVAL; }
+    if (M > (1 << 20) || N > (1 << 19)) {
+        set_error("%s: M above 2^20 or N above 2^19", who);
+        return WF_EUNSUPPORTED;
+    }
+    return WF_OK;
+}
+
+}  // namespace wf
+
+extern "C" int wf_gated_dense_plan(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col,
+                                   int dt, int64_t M, int64_t N, int64_t K, int keep, int* plan, int64_t* bytes) {
+    using namespace wf;
+    if (!plan || !bytes) { set_error("wf_gated_dense_plan: null pointer"); return WF_EINVAL; }
+    if (const int rc = gated_check("wf_gated_dense_plan", dt, 0, M, N, K, x_row, x_col, w_row, w_col)) return rc;
+    *bytes = 0;
+    plan[0] = plan[1] = plan[2] = plan[3] = plan[4] = 0;
+    if (M == 0 || N == 0) return WF_OK;
+    const GatedCall c = gated_call({x, x_row, x_col, false}, {w, w_row, w_col, false}, M, N, K, keep);
+    plan[0] = c.few ? 0 : 1;
+    plan[1] = c.few ? 0 : c.tiles.tiling;
+    plan[2] = c.slices;
+    plan[3] = c.few ? LIES_ALONG : c.how_x;
+    plan[4] = c.few ? LIES_ALONG : c.how_w;
+    *bytes = c.bytes;
+    return WF_OK;
+}
+
+extern "C" int wf_gated_dense(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt,
+                              int64_t M, int64_t N, int64_t K, const void* bias, int bias_dt, int act, void* y, void* kept,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace wf;
+    if (const int rc = gated_check("wf_gated_dense", dt, act, M, N, K, x_row, x_col, w_row, w_col)) return rc;
+    if (bias && bias_dt != dt && bias_dt != WF_F32) { set_error("wf_gated_dense: dtype code %d of the bias", bias_dt); return WF_EINVAL; }
+    if (M == 0 || N == 0) return WF_OK;
+    if (!x || !w || !y) { set_error("wf_gated_dense: null pointer"); return WF_EINVAL; }
+    if (!aligned(x, 2) || !aligned(w, 2) || !aligned(y, 2) || !aligned(kept, 2) || !aligned(bias, bias_dt == WF_F32 ? 4 : 2)) {
+        set_error("wf_gated_dense: a pointer is not aligned to its values");
+        return WF_EINVAL;
+    }
+    const DenseView xv = {x, x_row, x_col, false}, wv = {w, w_row, w_col, false};
+    const GatedCall c = gated_call(xv, wv, M, N, K, kept != nullptr);
+    char* ws = static_cast<char*>(workspace);
+    if (c.bytes && (!ws || workspace_bytes < c.bytes || !aligned(ws, 256))) {
+        set_error("wf_gated_dense: a workspace of %lld bytes is required", (long long)c.bytes);
+        return WF_EINVAL;
+    }
+    const GatedEpilogue e = {bias, bias_dt, act, y, static_cast<uint16_t*>(kept), M * N};
+    float* parts = c.slices > 1 ? reinterpret_cast<float*>(ws + c.parts_at) : nullptr;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (c.few) {
+        gated_rows_run(dt, c.slices, static_cast<const uint16_t*>(x), x_row, static_cast<const uint16_t*>(w), w_row, (int)M, (int)N,
+                       (int)K, parts, e, s);
+    } else {
+        DenseOperand a, b;
+        dense_operands(xv, c.how_x, M, ws, wv, c.how_w, 2 * N, ws + c.w_at, K, a, b, s);
+        b.rows = (int)N;
+        if (dt == WF_BF16) gated_tiling<WF_BF16>(a, b, N * b.row, (int)M, (int)N, (int)K, c.tiles, parts, e, s);
+        else gated_tiling<WF_F16>(a, b, N * b.row, (int)M, (int)N, (int)K, c.tiles, parts, e, s);
+    }
+    if (parts) {
+        over_grids((M * ((N + 7) / 8) + 255) / 256, kGridMost, [&](int64_t wg, uint32_t n) {
+            if (dt == WF_BF16) gated_sum<WF_BF16><<<dim3(n), 256, 0, s>>>(wg, parts, c.slices, (int)M, (int)N, e);
+            else gated_sum<WF_F16><<<dim3(n), 256, 0, s>>>(wg, parts, c.slices, (int)M, (int)N, e);
+        });
+    }
+    WF_LAUNCH_CHECK("wf_gated_dense launch");
+    return WF_OK;
+}
+
+extern "C" int wf_gated_dense_bwd_workspace(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, int dt,
+                                            int64_t M, int64_t N, int64_t K, int dx, int dw, int db, int64_t* bytes) {
+    using namespace wf;
+    if (!bytes) { set_error("wf_gated_dense_bwd_workspace: null pointer"); return WF_EINVAL; }
+    if (const int rc = gated_check("wf_gated_dense_bwd_workspace", dt, 0, M, N, K, x_row, 1, w_row, w_col)) return rc;
+    *bytes = M && N ? gated_backward(x, x_row, w, w_row, w_col, M, N, K, dx, dw, db, nullptr).bytes : 0;
+    return WF_OK;
+}
+
+extern "C" int wf_gated_dense_bwd(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, const void* dy,
+                                  int64_t dy_row, const void* kept, int dt, int act, int64_t M, int64_t N, int64_t K, void* dx,
+                                  void* dw, void* dbias, int bias_dt, void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace wf;
+    if (const int rc = gated_check("wf_gated_dense_bwd", dt, act, M, N, K, x_row, dy_row, w_row, w_col)) return rc;
+    if (dbias && bias_dt != dt && bias_dt != WF_F32) { set_error("wf_gated_dense_bwd: dtype code %d of the bias", bias_dt); return WF_EINVAL; }
+    if (M == 0 || N == 0) return WF_OK;                            // (the caller's empty or zero gradients)
+    if (!dy || !kept || (dx && !w) || (dw && !x)) { set_error("wf_gated_dense_bwd: null pointer"); return WF_EINVAL; }
+    if (!aligned(x, 2) || !aligned(w, 2) || !aligned(dy, 2) || !aligned(kept, 2) || !aligned(dx, 2) || !aligned(dw, 2) ||
+        !aligned(dbias, bias_dt == WF_F32 ? 4 : 2)) {
+        set_error("wf_gated_dense_bwd: a pointer is not aligned to its values");
+        return WF_EINVAL;
+    }
+    char* ws = static_cast<char*>(workspace);
+    const GatedBackward b = gated_backward(x, x_row, w, w_row, w_col, M, N, K, dx, dw, dbias, ws);
+    if (b.bytes && (!ws || workspace_bytes < b.bytes || !aligned(ws, 256))) {
+        set_error("wf_gated_dense_bwd: a workspace of %lld bytes is required", (long long)b.bytes);
+        return WF_EINVAL;
+    }
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    float* sums = dbias ? reinterpret_cast<float*>(ws + b.sums_at) : nullptr;
+    if (dx || dw || dbias) {
+        auto go = [&](auto d) {
+            constexpr int D = decltype(d)::value;
+            gated_dact<D><<<dim3((uint32_t)((N + 511) / 512), b.rows), 256, 0, s>>>(
+                static_cast<const value_t<D>*>(dy), dy_row, static_cast<const uint16_t*>(kept), M * N, act,
+                dx || dw ? reinterpret_cast<value_t<D>*>(ws) : nullptr, b.dh_row, sums, (int)M, (int)N);
+        };
+        if (dt == WF_BF16) go(std::integral_constant<int, WF_BF16>{});
+        else go(std::integral_constant<int, WF_F16>{});
+    }
+    if (dbias) {
+        const ColumnSums q = {sums, dbias, bias_dt, b.rows};
+        column_sums<<<dim3((uint32_t)((2 * N + 63) / 64), 1, 1), 1024, 0, s>>>(q, q, (int)(2 * N));
+    }
+    DenseEpilogue e = {};
+    e.rows_per_group = 1;
+    e.y = dx;
+    if (dx) dense_run(b.dx, b.dh_along, b.w_turned, dt, M, K, 2 * N, ws + b.product_at, e, s);
+    e.y = dw;
+    if (dw) dense_run(b.dw, b.dh_turned, b.x_turned, dt, 2 * N, K, M, ws + b.product_at, e, s);
+    WF_LAUNCH_CHECK("wf_gated_dense_bwd launch");
+    return WF_OK;
+}

@@ -252,6 +252,26 @@ int wf_dense_bwd(const void* x, int64_t x_row, const void* w, int64_t w_row, int
                  int64_t N, int64_t K, void* dx, void* dw, void* dbias, int bias_dt, void* dgate, void* workspace,
                  int64_t workspace_bytes, void* stream);
 
+/* The gated feed-forward layer's first half: g, u = the halves of x w^T + bias, y[m, n] = act(g[m, n]) u[m, n] in dt (WF_BF16 or
+ * WF_F16), float32 accumulation, one rounding. w: [2 N, K], the gate's rows first; bias (may be NULL): [2 N] of type dt or
+ * WF_F32; y: [M, N]; operands and act as in wf_dense. kept (may be NULL): 6 M N bytes, g and u in 24 bits for wf_gated_dense_bwd.
+ * M <= 2^20, N <= 2^19, K <= 2^20. wf_gated_dense_plan: the workspace's bytes (256-byte aligned; it need not be cleared) and how
+ * such a call runs, plan[5]: 0 few rows or 1 tiles, the tiling (0-4), slices of K, and how x and w get there as in wf_dense_plan. */
+int wf_gated_dense_plan(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt,
+                        int64_t M, int64_t N, int64_t K, int keep, int* plan, int64_t* bytes);
+int wf_gated_dense(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt, int64_t M,
+                   int64_t N, int64_t K, const void* bias, int bias_dt, int act, void* y, void* kept, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* Its backward pass for the gradient dy of y (rows dy_row values apart): dg = dy u act'(g), du = dy act(g), dh = [dg du] rounded to
+ * dt, dx = dh w [M, K], dw = dh^T x [2 N, K], dbias the sums over rows of the unrounded dh [2 N]; any of the three may be NULL. Every
+ * sum has a fixed order. */
+int wf_gated_dense_bwd_workspace(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, int dt, int64_t M,
+                                 int64_t N, int64_t K, int dx, int dw, int db, int64_t* bytes);
+int wf_gated_dense_bwd(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, const void* dy, int64_t dy_row,
+                       const void* kept, int dt, int act, int64_t M, int64_t N, int64_t K, void* dx, void* dw, void* dbias,
+                       int bias_dt, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* One AdamW step (step >= 1) of `count` tensors of type dt, in place: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
  * p = (1 - lr decay) p - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps). table: host memory, read before the
  * call returns: address of the parameter, address of its gradient, values, for each tensor. The moments are flat over all
