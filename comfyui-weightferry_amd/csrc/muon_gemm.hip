@@ -1,0 +1,316 @@
+// The products of a Newton-Schulz step on a batch of float16 matrices, for gfx950, in the tiles of the 16-bit linear (dense_ring.h):
+//
+//   A = X X^T (or X^T X, whichever is the smaller),  B = b A + c A A,  X = a X + B X (or X B)
+//
+// A and B are symmetric, so only the tiles on and below the diagonal are computed, half the operations, and each is stored twice, as
+// it is and turned: a lane's accumulators are four consecutive rows of a column, which turned are four consecutive values of
+// a row. X is read as it lies, along or across the sum.
+//
+// Where a batch's tiles do not fill the chip a symmetric product runs in slices of K: the accumulators go to memory as they are
+// in the registers, and a second launch of the same kernel starts from their sum, in slice order.
+//
+// X is kept with the remainder of its rounding (lo) while small singular values grow, and a X is taken from both: a X is what they live
+// from, and an error in the first X is multiplied by a^5 = 485 there. The products see X itself, 11 bits.
+
+#include <algorithm>
+#include <type_traits>
+
+#include "dense_gemm.h"
+#include "muon.h"
+
+namespace wf {
+
+// a wave's part of the idle stage buffers (four waves)
+template <typename S>
+__device__ __forceinline__ char* muon_region(wl_frag* sb0, wl_frag* sb1, int wave) {
+    static_assert(S::NW == 4, "two waves a buffer");
+    return reinterpret_cast<char*>(wave < 2 ? sb0 : sb1) + (wave & 1) * (S::SLOTS * 8);
+}
+
+__device__ __forceinline__ int muon_spread(int w, int T) {        // XCD w % 8 takes consecutive tiles
+    return w < (T & ~7) ? (w & 7) * (T >> 3) + (w >> 3) : w;
+}
+
+__device__ __forceinline__ float f16_at(uint64_t v, int i) { return f16_bits_to_f32((uint32_t)(v >> (16 * i)) & 0xffffu); }
+
+// Workgroup (tile, slice, matrix). parts: [batch, slices, tiles, accumulators of a workgroup], NULL without slices. SUM: the second
+// launch, its slice the only one.
+template <bool X, typename S, bool SUM>
+__global__ __launch_bounds__(S::NT, S::WAVES) void muon_sym(DenseOperand o, int64_t o_step, MuonSymmetric q, int64_t s_step, int side,
+                                                            int sld, int stages, int slice_stages, int slices,
+                                                            float* __restrict__ parts) {
+    constexpr int WM = S::WM, WN = S::WN, LANES = WM * WN * 16 * S::NT;
+    static_assert(S::BM == S::BN && WM == WN, "tiles that turn into tiles");
+    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS];
+    const int T = gridDim.x, tile = __builtin_amdgcn_readfirstlane(muon_spread(blockIdx.x, T));
+    int tm = (int)((sqrtf(8.0f * (float)tile + 1.0f) - 1.0f) * 0.5f);
+    while (tm * (tm + 1) / 2 > tile) tm--;
+    while ((tm + 1) * (tm + 2) / 2 <= tile) tm++;
+    const int m0 = __builtin_amdgcn_readfirstlane(tm * S::BM), n0 = __builtin_amdgcn_readfirstlane((tile - tm * (tm + 1) / 2) * S::BN);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t b = blockIdx.z;
+    f32x16v acc[WM][WN];
+#pragma unroll
+    for (int i = 0; i < WM; i++)
+#pragma unroll
+        for (int j = 0; j < WN; j++)
+#pragma unroll
+            for (int x = 0; x < 16; x++) acc[i][j][x] = 0.0f;
+    auto at = [&](int s) { return parts + ((b * slices + s) * T + tile) * LANES + threadIdx.x; };
+    if constexpr (SUM) {
+        for (int s = 0; s < slices; s++) {
+            const float* p = at(s);
+#pragma unroll
+            for (int i = 0; i < WM; i++)
+#pragma unroll
+                for (int j = 0; j < WN; j++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) acc[i][j][x] += p[((i * WN + j) * 16 + x) * S::NT];
+        }
+    } else {
+        o.p += b * o_step;
+        const int s0 = blockIdx.y * slice_stages, nk = min(slice_stages, stages - s0);
+        const DenseTile ta = dense_tile<X>(o, m0), tb = dense_tile<X>(o, n0);
+        dense_mainloop<S, X, X>(ta, tb, s0, nk, wave, lane, sb0, sb1, acc,
+                                [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<WF_F16>(c, x, y); });
+        if (parts) {
+            float* p = at(blockIdx.y);
+#pragma unroll
+            for (int i = 0; i < WM; i++)
+#pragma unroll
+                for (int j = 0; j < WN; j++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) p[((i * WN + j) * 16 + x) * S::NT] = acc[i][j][x];
+            return;
+        }
+    }
+    const int mw = m0 + wave / S::VN * WM * 32, nw = n0 + wave % S::VN * WN * 32;
+    const int lr = lane & 31, lk = lane >> 5;
+    uint16_t* out = q.out + b * s_step;
+    const uint16_t* in = q.in ? q.in + b * s_step : nullptr;
+    // the outputs, rounded, in the accumulators' places: four rows' values in 64 bits
+    uint64_t v[WM][WN][4];
+#pragma unroll
+    for (int i = 0; i < WM; i++)
+#pragma unroll
+        for (int j = 0; j < WN; j++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const int m = mw + 32 * i + 8 * y + 4 * lk, n = nw + 32 * j + lr;
+                uint64_t c = 0;                                    // (in is symmetric: its row n holds column n)
+                if (in && n < side && m < sld) __builtin_memcpy(&c, in + (int64_t)n * sld + m, 8);
+                float r[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    r[x] = q.alpha * acc[i][j][4 * y + x];
+                    if (in) r[x] = fmaf(q.beta, f16_at(c, x), r[x]);
+                    if (m + x == n && n < side) r[x] += q.gamma;
+                }
+                v[i][j][y] = pack_f16(r[0], r[1]) | (uint64_t)pack_f16(r[2], r[3]) << 32;
+            }
+    uint16_t* lds = reinterpret_cast<uint16_t*>(muon_region<S>(sb0, sb1, wave));
+    wl_store_tile<WM, WN>(lds, out, side, sld, mw, nw, lane,
+                          [&](int i, int j, int x) { return (uint16_t)(v[i][j][x >> 2] >> (16 * (x & 3))); });
+    if (m0 == n0) return;
+    // turned: 32 columns at a time are rows of WM 32 values (8 more apart: the lanes' 8-byte writes then share banks by twos)
+    constexpr int ROW = WM * 32 + 8, RUNS = WM * 4;
+    static_assert(32 * ROW * 2 <= S::SLOTS * 8, "the turned rows fit a wave's region");
+#pragma unroll
+    for (int j = 0; j < WN; j++) {
+#pragma unroll
+        for (int i = 0; i < WM; i++)
+#pragma unroll
+            for (int y = 0; y < 4; y++)
+                __builtin_memcpy(__builtin_assume_aligned(lds + lr * ROW + 32 * i + 8 * y + 4 * lk, 8), &v[i][j][y], 8);
+#pragma unroll
+        for (int it = 0; it < 32 * RUNS / 64; it++) {
+            const int p = it * 64 + lane, n = nw + 32 * j + p / RUNS, m = mw + 8 * (p % RUNS);
+            Pack<WF_F16> w;
+            __builtin_memcpy(w.w, __builtin_assume_aligned(lds + p / RUNS * ROW + 8 * (p % RUNS), 16), 16);
+            if (n < side && m < sld) w.store(out + (int64_t)n * sld + m, 8);
+        }
+    }
+}
+
+// Workgroup (tile, matrix) of the outputs [rows, cols]; BX: b lies across K.
+template <bool BX, typename S>
+__global__ __launch_bounds__(S::NT, S::WAVES) void muon_upd(DenseOperand a, int64_t a_step, DenseOperand bo, int64_t b_step, MuonUpdate q,
+                                                            int64_t x_step, int rows, int cols, int ld, int K, MuonTensors t) {
+    constexpr int WM = S::WM, WN = S::WN, TC = WN * 32;
+    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS];
+    const int ntm = (rows + S::BM - 1) / S::BM, ntn = (cols + S::BN - 1) / S::BN;
+    int tm, tn;
+    tile_order(blockIdx.x, ntm * ntn, ntm, ntn, tm, tn);
+    const int m0 = __builtin_amdgcn_readfirstlane(tm * S::BM), n0 = __builtin_amdgcn_readfirstlane(tn * S::BN);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.y;
+    a.p += b * a_step;
+    bo.p += b * b_step;
+    f32x16v acc[WM][WN];
+#pragma unroll
+    for (int i = 0; i < WM; i++)
+#pragma unroll
+        for (int j = 0; j < WN; j++)
+#pragma unroll
+            for (int x = 0; x < 16; x++) acc[i][j][x] = 0.0f;
+    const DenseTile ta = dense_tile<false>(a, m0), tb = dense_tile<BX>(bo, n0);
+    dense_mainloop<S, false, BX>(ta, tb, 0, (K + 63) / 64, wave, lane, sb0, sb1, acc,
+                                 [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<WF_F16>(c, x, y); });
+    const int mw = m0 + wave / S::VN * WM * 32, nw = n0 + wave % S::VN * TC;
+    const int lr = lane & 31, lk = lane >> 5;
+    // 16 rows at a time through LDS in float32, then runs of 8 outputs
+    static_assert(16 * TC * 4 <= S::SLOTS * 8, "the rows fit a wave's region");
+    float* lds = reinterpret_cast<float*>(muon_region<S>(sb0, sb1, wave));
+    constexpr int RUNS = TC / 8;
+#pragma unroll
+    for (int half = 0; half < 2 * WM; half++) {
+        if (mw + half * 16 >= rows) break;
+#pragma unroll
+        for (int x = 0; x < 8; x++)
+#pragma unroll
+            for (int j = 0; j < WN; j++)
+                lds[(8 * (x >> 2) + 4 * lk + (x & 3)) * TC + j * 32 + lr] = acc[half / 2][j][8 * (half & 1) + x];
+#pragma unroll 1
+        for (int it = 0; it < (16 * RUNS + 63) / 64; it++) {
+            const int p = it * 64 + lane, m = mw + half * 16 + p / RUNS, n = nw + 8 * (p % RUNS);
+            if (p >= 16 * RUNS || m >= rows || n >= (q.next ? ld : cols)) continue;
+            const float4 lo4 = reinterpret_cast<const float4*>(lds)[2 * p], hi4 = reinterpret_cast<const float4*>(lds)[2 * p + 1];
+            float v[8] = {lo4.x, lo4.y, lo4.z, lo4.w, hi4.x, hi4.y, hi4.z, hi4.w};
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] *= q.alpha;
+            const int64_t at = b * x_step + (int64_t)m * ld + n;
+            if (q.lo) {
+                Pack<WF_F16> x, r;
+                x.load(q.x + at, 8);
+                r.load(q.lo + at, 8);
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = fmaf(q.a, fmaf(r.get(i), 1.0f / 2048.0f, x.get(i)), v[i]);
+            }
+            if (!q.next) {
+                muon_apply(t, b, (int64_t)m * cols + n, v, cols - n);
+                continue;
+            }
+            Pack<WF_F16> o;
+            o.put(v);
+            o.store(q.next + at, 8);
+            if (q.lo) {
+                float w[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[i] = (v[i] - o.get(i)) * 2048.0f;
+                Pack<WF_F16> r;
+                r.put(w);
+                r.store(q.lo + at, 8);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- host side
+// us of a workgroup, of each 64 values of K, and that where per_cu of them share a CU
+struct MuonTile {
+    int bm, bn, per_cu;
+    float fixed, stage, shared;
+};
+static float muon_time(const MuonTile& q, int64_t wgs, int64_t stages) {
+    const int64_t on = (wgs + 255) / 256, full = on / q.per_cu;
+    const int rest = (int)(on % q.per_cu);
+    auto together = [&](int n) {
+        if (n == 0) return 0.0f;
+        const float more = q.per_cu > 1 ? (q.shared * q.per_cu - q.stage) * (n - 1) / (q.per_cu - 1) : 0.0f;
+        return q.fixed + (float)stages * (q.stage + more);
+    };
+    return (float)full * together(q.per_cu) + together(rest);
+}
+
+constexpr MuonTile kSymmetric[] = {{256, 256, 1, 5.0f, 1.252f, 1.252f}, {128, 128, 2, 2.5f, 0.634f, 0.519f}, {64, 64, 4, 2.0f, 0.42f, 0.20f}};
+struct MuonSlices {
+    int tiling, tiles, slices, slice_stages;
+};
+static MuonSlices muon_symmetric_plan(const MuonShape& s, int64_t K) {
+    const int64_t stages = (K + 63) / 64;
+    MuonSlices best = {};
+    float least = 1e30f;
+    for (int t = 0; t < 3; t++) {
+        const MuonTile& q = kSymmetric[t];
+        const int64_t across = (s.side + q.bm - 1) / q.bm, tiles = across * (across + 1) / 2;
+        for (int want : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            const int64_t per = (stages + want - 1) / want, slices = (stages + per - 1) / per, wgs = tiles * s.batch * slices;
+            if (want > 1 && (slices != want || per < 3 || wgs > 1600)) continue;
+            float c = muon_time(q, wgs, per);
+            if (want > 1) c += 5.0f + 0.8e-6f * (float)(tiles * s.batch) * (float)(q.bm * q.bn) * (float)(slices + 1);
+            if (c < least) least = c, best = {t, (int)tiles, (int)slices, (int)per};
+        }
+    }
+    return best;
+}
+static int muon_symmetric_k(const MuonShape& s, bool square) { return square ? s.sld : s.tall ? s.rows : s.ld; }
+
+int64_t muon_symmetric_bytes(const MuonShape& s, bool square) {
+    const MuonSlices p = muon_symmetric_plan(s, muon_symmetric_k(s, square));
+    const int64_t bm = kSymmetric[p.tiling].bm;
+    return p.slices > 1 ? (int64_t)s.batch * p.slices * p.tiles * bm * bm * 4 : 0;
+}
+
+void muon_symmetric(const MuonShape& s, const MuonSymmetric& q, float* parts, hipStream_t st) {
+    const int K = muon_symmetric_k(s, q.square);
+    const MuonSlices p = muon_symmetric_plan(s, K);
+    const bool across = !q.square && s.tall;
+    const DenseOperand o = q.square ? DenseOperand{q.x, s.sld, s.sld, s.side, false}
+                           : s.tall ? DenseOperand{q.x, s.ld, s.rows, s.cols, true}
+                                    : DenseOperand{q.x, s.ld, s.ld, s.rows, false};
+    const int64_t s_step = (int64_t)s.side * s.sld, o_step = q.square ? s_step : (int64_t)s.rows * s.ld;
+    auto go = [&](auto x, auto shape) {
+        constexpr bool X = decltype(x)::value;
+        using S = decltype(shape);
+        float* w = p.slices > 1 ? parts : nullptr;
+        muon_sym<X, S, false><<<dim3(p.tiles, p.slices, s.batch), S::NT, 0, st>>>(o, o_step, q, s_step, s.side, s.sld, (K + 63) / 64,
+                                                                                 p.slice_stages, p.slices, w);
+        if (w)
+            muon_sym<X, S, true><<<dim3(p.tiles, 1, s.batch), S::NT, 0, st>>>(o, o_step, q, s_step, s.side, s.sld, 0, 0, p.slices, w);
+    };
+    auto by = [&](auto x) {
+        if (p.tiling == 0) go(x, DenseShape<2, 2, 4, 4>{});
+        else if (p.tiling == 1) go(x, DenseShape<2, 2, 2, 2>{});
+        else go(x, DenseShape<2, 2, 1, 1>{});
+    };
+    if (across) by(std::true_type{});
+    else by(std::false_type{});
+}
+
+constexpr MuonTile kUpdate[] = {{256, 256, 1, 6.0f, 1.252f, 1.252f}, {256, 192, 1, 4.5f, 1.076f, 1.076f},
+                                {128, 128, 2, 2.5f, 0.634f, 0.519f}, {64, 128, 3, 1.5f, 0.47f, 0.367f}};
+
+void muon_update(const MuonShape& s, const MuonUpdate& q, const MuonTensors& t, hipStream_t st) {
+    int tiling = 0;
+    float least = 1e30f;
+    for (int i = 0; i < 4; i++) {
+        const MuonTile& z = kUpdate[i];
+        const int64_t wgs = (int64_t)((s.rows + z.bm - 1) / z.bm) * ((s.cols + z.bn - 1) / z.bn) * s.batch;
+        const float c = muon_time(z, wgs, (s.side + 63) / 64);
+        if (c < least) least = c, tiling = i;
+    }
+    const int64_t x_step = (int64_t)s.rows * s.ld, q_step = (int64_t)s.side * s.sld;
+    const DenseOperand q_along = {q.q, s.sld, s.sld, s.side, false};
+    auto go = [&](auto bx, auto shape) {
+        constexpr bool BX = decltype(bx)::value;
+        using S = decltype(shape);
+        const dim3 grid(((s.rows + S::BM - 1) / S::BM) * ((s.cols + S::BN - 1) / S::BN), s.batch);
+        if constexpr (BX) {                                        // q x: x's columns are rows that lie across the sum
+            const DenseOperand x = {q.x, s.ld, s.rows, s.cols, true};
+            muon_upd<true, S><<<grid, S::NT, 0, st>>>(q_along, q_step, x, x_step, q, x_step, s.rows, s.cols, s.ld, s.side, t);
+        } else {
+            const DenseOperand x = {q.x, s.ld, s.ld, s.rows, false};
+            muon_upd<false, S><<<grid, S::NT, 0, st>>>(x, x_step, q_along, q_step, q, x_step, s.rows, s.cols, s.ld, s.side, t);
+        }
+    };
+    auto by = [&](auto bx) {
+        if (tiling == 0) go(bx, DenseShape<2, 2, 4, 4>{});
+        else if (tiling == 1) go(bx, DenseShape<2, 2, 4, 3>{});
+        else if (tiling == 2) go(bx, DenseShape<2, 2, 2, 2>{});
+        else go(bx, DenseShape<1, 4, 2, 1>{});
+    };
+    if (s.tall) by(std::false_type{});
+    else by(std::true_type{});
+}
+
+}  // namespace wf

@@ -286,6 +286,19 @@ int wf_adamw(const int64_t* table, int64_t count, int dt, int bits, void* exp_av
 int wf_adamw_values(const int8_t* exp_avg, const uint8_t* exp_avg_sq, const float* avg_scale, const float* sq_scale,
                     int64_t blocks, float* avg, float* sq, void* stream);
 
+/* Orthogonalised updates of `count` matrices [rows, cols] of type dt, row-major and contiguous: m = mu m + (1 - mu) g, u = (1 - mu) g + mu
+ * m (nesterov) or m, X = u / max(|u|, eps) with the Frobenius norm, `steps` times (1 to 32) X = a X + (b A + c A A) X, A = X X^T; then p =
+ * keep p - rate X, in place (p and m). table: host memory, read before the call returns: addresses of p, g and m of each matrix; m
+ * (float32) may be 0: u = g. coefficients: a, b, c; WF_EINVAL for ones that take singular values from [0, 1] past 1.9. The shorter side
+ * <= 16384, the longer <= 2^20, (rows + 128) (cols + 8) < 2^30. No matrix may be there twice. With a shorter side up to 64 everything
+ * is float32 or more; above, the products' operands are float16 and X is good to 1e-3 of its norm. wf_orthogonalize: out = X, table:
+ * addresses of out, g and 0. The workspace (256-byte aligned) need not be cleared. */
+int wf_muon_workspace(int64_t count, int64_t rows, int64_t cols, int64_t* bytes);
+int wf_muon(const int64_t* table, int64_t count, int64_t rows, int64_t cols, int dt, double momentum, int nesterov, double keep,
+            double rate, int steps, const double* coefficients, double eps, void* workspace, int64_t workspace_bytes, void* stream);
+int wf_orthogonalize(const int64_t* table, int64_t count, int64_t rows, int64_t cols, int dt, int steps, const double* coefficients,
+                     double eps, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------------------- block streaming
  * Exact-size page-locked host memory: replaces PinnedHost's cudaHostRegister / cudaHostUnregister
  * (core/tiers/pinned.py:84-129); allocated page-locked (hipHostMalloc) instead of registered after the fact. */
