@@ -29,11 +29,10 @@ class I8Plan(ctypes.Structure):
 
 
 class BlockNorm(ctypes.Structure):
-    """wf_block_norm: the parameters of the norms around a gated residual (wf_block_norm_fwd)."""
+    """wf_block_norm: the kinds, types and groups of the norms around a gated residual (wf_block_norm_fwd)."""
     _fields_ = [(f, ctypes.c_int32) for f in ("dt", "post", "norm", "plus_one", "post_weight_dt", "gate_dt", "weight_dt")] + \
                [("scale", ctypes.c_float), ("eps", ctypes.c_float)] + \
-               [(f, _i64) for f in ("groups", "gate_groups", "weight_groups")] + \
-               [(f, _p) for f in ("post_weight", "gate", "weight", "bias")]
+               [(f, _i64) for f in ("groups", "gate_groups", "weight_groups")]
 
 
 # every symbol of include/weightferry.h: name -> (restype, argtypes)
@@ -60,9 +59,9 @@ EXPORTS = {
     "wf_layer_norm_bwd_workspace": (_int, [_i64, _i64, _i64, _int, ctypes.POINTER(_i64)]),
     "wf_layer_norm_bwd": (_int, [_p, _i64, _p, _i64, _int, _p, _int, _int, _i64, _p, _p, _p, _p, _i64, _i64, _p, _i64,
                                  _p]),
-    "wf_block_norm_fwd": (_int, [ctypes.POINTER(BlockNorm), _p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _p]),
-    "wf_block_norm_bwd_workspace": (_int, [ctypes.POINTER(BlockNorm), _i64, _i64, _int, ctypes.POINTER(_i64)]),
-    "wf_block_norm_bwd": (_int, [ctypes.POINTER(BlockNorm), _p, _i64, _p, _i64, _p, _i64, _p, _i64] + [_p] * 7 +
+    "wf_block_norm_fwd": (_int, [_p, _p, _i64, _p, _i64] + [_p] * 7 + [_i64, _i64, _p]),
+    "wf_block_norm_bwd_workspace": (_int, [_p, _i64, _i64, _int, ctypes.POINTER(_i64)]),
+    "wf_block_norm_bwd": (_int, [_p, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _p, _i64] + [_p] * 7 +
                           [_i64, _i64, _p, _i64, _p]),
     "wf_dense_workspace": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _int, ctypes.POINTER(_i64)]),
     "wf_dense_plan": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _int, ctypes.POINTER(_int)]),

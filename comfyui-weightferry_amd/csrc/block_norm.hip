@@ -412,9 +412,8 @@ static int bn_check(const char* who, const wf_block_norm* q, int64_t M, int64_t 
         set_error("%s: M, K = %lld, %lld, or no parameters, groups or norms that fit", who, (long long)M, (long long)K);
         return WF_EINVAL;
     }
-    auto other = [&](const void* p, int dt) { return p && dt != q->dt && dt != WF_F32; };
-    if (!known_dtype(q->dt) || other(q->post_weight, q->post_weight_dt) || other(q->gate, q->gate_dt) ||
-        other(q->weight, q->weight_dt) || other(q->bias, q->weight_dt)) {
+    auto other = [&](int dt) { return dt != q->dt && dt != WF_F32; };
+    if (!known_dtype(q->dt) || other(q->post_weight_dt) || other(q->gate_dt) || other(q->weight_dt)) {
         set_error("%s: dtype codes %d, %d, %d, %d", who, q->dt, q->post_weight_dt, q->gate_dt, q->weight_dt);
         return WF_EUNSUPPORTED;
     }
@@ -425,15 +424,16 @@ static int bn_check(const char* who, const wf_block_norm* q, int64_t M, int64_t 
     return WF_OK;
 }
 
-static BlockNorm bn_of(const wf_block_norm* q, int64_t M, int64_t K) {
-    return {q->post_weight, q->gate, q->weight, q->bias, q->post_weight_dt, q->gate_dt, q->weight_dt, q->post, q->norm,
+static BlockNorm bn_of(const wf_block_norm* q, const void* pw, const void* gate, const void* w, const void* b, int64_t M, int64_t K) {
+    return {pw, gate, w, b, q->post_weight_dt, q->gate_dt, q->weight_dt, q->post, q->norm,
             q->plus_one ? 1.0f : 0.0f, q->scale, q->eps, M / q->groups, q->gate_groups > 1 ? K : 0, q->weight_groups > 1 ? K : 0};
 }
 
 }  // namespace wf
 
-extern "C" int wf_block_norm_fwd(const wf_block_norm* q, const void* x, int64_t x_row, const void* h, int64_t h_row, void* r,
-                                 void* y, float* stats, int64_t M, int64_t K, void* stream) {
+extern "C" int wf_block_norm_fwd(const wf_block_norm* q, const void* x, int64_t x_row, const void* h, int64_t h_row,
+                                 const void* post_weight, const void* gate, const void* weight, const void* bias, void* r, void* y,
+                                 float* stats, int64_t M, int64_t K, void* stream) {
     using namespace wf;
     if (const int rc = bn_check("wf_block_norm_fwd", q, M, K)) return rc;
     auto one_or_all = [&](int64_t n) { return n == 1 || n == q->groups; };
@@ -443,7 +443,7 @@ extern "C" int wf_block_norm_fwd(const wf_block_norm* q, const void* x, int64_t 
     }
     if (M == 0) return WF_OK;
     if (!x || !y) { set_error("wf_block_norm_fwd: null pointer"); return WF_EINVAL; }
-    const BlockNorm p = bn_of(q, M, K);
+    const BlockNorm p = bn_of(q, post_weight, gate, weight, bias, M, K);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     by_dtype(q->dt, [&](auto d) {
         constexpr int D = decltype(d)::value;
@@ -468,8 +468,8 @@ extern "C" int wf_block_norm_bwd_workspace(const wf_block_norm* q, int64_t M, in
 }
 
 extern "C" int wf_block_norm_bwd(const wf_block_norm* q, const void* x, int64_t x_row, const void* h, int64_t h_row,
-                                 const void* dr, int64_t dr_row, const void* dy, int64_t dy_row, const float* stats, void* dx,
-                                 void* dh, void* dpost_weight, void* dgate, void* dweight, void* dbias, int64_t M, int64_t K,
+                                 const void* post_weight, const void* gate, const void* weight, const void* dr, int64_t dr_row,
+                                 const void* dy, int64_t dy_row, const float* stats, void* dx, void* dh, void* dpost_weight, void* dgate, void* dweight, void* dbias, int64_t M, int64_t K,
                                  void* workspace, int64_t workspace_bytes, void* stream) {
     using namespace wf;
     if (const int rc = bn_check("wf_block_norm_bwd", q, M, K)) return rc;
@@ -480,7 +480,7 @@ extern "C" int wf_block_norm_bwd(const wf_block_norm* q, const void* x, int64_t 
     }
     if (M == 0) return WF_OK;                                   // (no rows: the caller's empty or zero gradients)
     if (!x || !stats || (!dr && !dy)) { set_error("wf_block_norm_bwd: null pointer"); return WF_EINVAL; }
-    const BlockNorm p = bn_of(q, M, K);
+    const BlockNorm p = bn_of(q, post_weight, gate, weight, nullptr, M, K);
     const RowShape z = bn_bwd_shape(M, K, p.rows, q->dt);
     const int64_t plane = q->groups * z.parts * K;
     const int count = (dpost_weight ? 1 : 0) + (dgate ? 1 : 0) + (dweight ? 1 : 0) + (dbias ? 1 : 0);

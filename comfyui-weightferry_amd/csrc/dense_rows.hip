@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256) void dense_rows(const uint16_t* __restrict__ x
             sum(g, m, c);
             sum(u, m, 16 + c);
             if (!parts) {
-                gated_run<D>(e, g, u, m0 + m, n, N, cnt);
+                gated_run<D, true>(e, g, u, m0 + m, n, N, cnt);
                 return;
             }
             float* o = parts + ((int64_t)blockIdx.y * M + m0 + m) * 2 * N + n;

@@ -19,16 +19,21 @@ struct GatedEpilogue {
     int64_t plane;                         // M N
 };
 
-// float32 rounded to 24 bits, finite as keep_finite; NaN stays NaN
-__device__ __forceinline__ uint32_t kept_bits(float v) {
-    return v != v ? 0x7fc00000u : __float_as_uint(keep_finite<WF_BF16>(v)) + 0x80u;
+// float32 rounded to 24 bits, which are the upper ones; NaN stays NaN
+__device__ __forceinline__ uint32_t kept_bits(float v) { return v != v ? 0x7fc00000u : __float_as_uint(v) + 0x80u; }
+// two places' upper halves, and their lower 8 bits of g and u, as 32 bits each
+__device__ __forceinline__ uint32_t kept_uppers(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
+__device__ __forceinline__ uint32_t kept_lowers(uint32_t g0, uint32_t u0, uint32_t g1, uint32_t u1) {
+    const uint32_t lo = __builtin_amdgcn_perm(u0, g0, 0x0c0c0501), hi = __builtin_amdgcn_perm(u1, g1, 0x05010c0c);
+    return lo | hi;
 }
-__device__ __forceinline__ uint16_t kept_upper(uint32_t b) { return (uint16_t)(b >> 16); }
-__device__ __forceinline__ uint16_t kept_lower(uint32_t g, uint32_t u) {
-    return (uint16_t)((g >> 8 & 0xffu) | (u & 0xff00u));
+// back to float32, and finite (keep_finite's reason)
+__device__ __forceinline__ float kept_g(uint32_t upper, uint32_t lower) {
+    return keep_finite<WF_BF16>(__uint_as_float(upper << 16 | (lower & 0xffu) << 8));
 }
-__device__ __forceinline__ float kept_g(uint32_t upper, uint32_t lower) { return __uint_as_float(upper << 16 | (lower & 0xffu) << 8); }
-__device__ __forceinline__ float kept_u(uint32_t upper, uint32_t lower) { return __uint_as_float(upper << 16 | (lower & 0xff00u)); }
+__device__ __forceinline__ float kept_u(uint32_t upper, uint32_t lower) {
+    return keep_finite<WF_BF16>(__uint_as_float(upper << 16 | (lower & 0xff00u)));
+}
 
 // the first cnt of 8 values
 __device__ __forceinline__ void store_run(float* o, const float (&v)[8], int cnt) {
@@ -39,10 +44,10 @@ __device__ __forceinline__ void store_run(float* o, const float (&v)[8], int cnt
             if (k < cnt) o[k] = v[k];
 }
 
-// g, u: a run's sums without the bias
-template <int D>
+// g, u: a run's sums, without the bias when BIAS is set
+template <int D, bool BIAS>
 __device__ __forceinline__ void gated_run(const GatedEpilogue& e, float (&g)[8], float (&u)[8], int64_t m, int n, int N, int cnt) {
-    if (e.bias) {
+    if (BIAS && e.bias) {
         float b[8];
         load_params<8>(b, e.bias, n, cnt, e.bias_dt);
 #pragma unroll
@@ -59,9 +64,9 @@ __device__ __forceinline__ void gated_run(const GatedEpilogue& e, float (&g)[8],
         Pack<WF_BF16> pg, pu, pl;                                  // (16 bits are moved, whatever they stand for)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            pg.w[i] = kept_upper(bg[2 * i]) | (uint32_t)kept_upper(bg[2 * i + 1]) << 16;
-            pu.w[i] = kept_upper(bu[2 * i]) | (uint32_t)kept_upper(bu[2 * i + 1]) << 16;
-            pl.w[i] = kept_lower(bg[2 * i], bu[2 * i]) | (uint32_t)kept_lower(bg[2 * i + 1], bu[2 * i + 1]) << 16;
+            pg.w[i] = kept_uppers(bg[2 * i], bg[2 * i + 1]);
+            pu.w[i] = kept_uppers(bu[2 * i], bu[2 * i + 1]);
+            pl.w[i] = kept_lowers(bg[2 * i], bu[2 * i], bg[2 * i + 1], bu[2 * i + 1]);
         }
         pg.store(e.kept + at, cnt);
         pu.store(e.kept + e.plane + at, cnt);

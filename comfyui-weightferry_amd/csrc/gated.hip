@@ -19,6 +19,7 @@
 #include "column_sums.h"
 #include "dense_call.h"
 #include "grids.h"
+#include "tile_stage.h"
 
 namespace wf {
 
@@ -71,18 +72,22 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void gated_gemm(DenseOperand a, De
             }
         return;
     }
-    uint16_t* o16 = wl_out_region<S>(sb0, sb1, wave);
-    auto store = [&](uint16_t* out, auto&& f) {
-        wl_store_tile<WM, WN / 2>(o16, out, M, N, mw, nw, lane,
-                                  [&](int i, int j, int x) { return f(acc[i][2 * j][x], acc[i][2 * j + 1][x]); });
-    };
-    if (e.kept) {
-        store(e.kept, [](float g, float) { return kept_upper(kept_bits(g)); });
-        store(e.kept + e.plane, [](float, float u) { return kept_upper(kept_bits(u)); });
-        store(e.kept + 2 * e.plane, [](float g, float u) { return kept_lower(kept_bits(g), kept_bits(u)); });
-    }
-    by_act(e.act, [&](auto k) {
-        store(static_cast<uint16_t*>(e.y), [](float g, float u) { return from_f32<D>(act_of<decltype(k)::value>(g) * u); });
+    using Stage = TileStage<S>;
+    constexpr int RUNS = TC / 8;
+    float* t = Stage::region(sb0, sb1, wave);
+    static_for<Stage::PHASES>([&](auto pc) {
+        constexpr int P = decltype(pc)::value;
+        if (mw + P * Stage::ROWS >= M) return;
+        Stage::template put<P>(t, acc, lane);
+#pragma unroll 1
+        for (int it = 0; it < Stage::ROWS * RUNS / 64; it++) {
+            const int q = it * 64 + lane, r = q / RUNS, c = 8 * (q % RUNS), m = mw + P * Stage::ROWS + r, n = nw + c;
+            const float* p = t + r * Stage::TC + (c & ~31) * 2 + (c & 31);
+            float g[8], u[8];
+            staged_run(g, p);
+            staged_run(u, p + 32);
+            if (m < M && n < N) gated_run<D, false>(e, g, u, m, n, N, N - n);
+        }
     });
 }
 
@@ -118,7 +123,7 @@ __global__ __launch_bounds__(256) void gated_sum(int64_t wg, const float* __rest
 #pragma unroll
                 for (int x = 0; x < 8; x++) g[x] += a[k][x], u[x] += b[k][x];
     }
-    gated_run<D>(e, g, u, m, n, N, cnt);
+    gated_run<D, true>(e, g, u, m, n, N, cnt);
 }
 
 // The backward pass's element-wise part: workgroup (512 columns, i) walks rows 4 i + wave, + 4 gridDim.y, ...; bparts:

@@ -416,7 +416,7 @@ static int muon_check(const char* who, int64_t count, int64_t rows, int64_t cols
         return WF_EINVAL;
     }
     if (!known_dtype(dt)) { set_error("%s: dtype code %d", who, dt); return WF_EUNSUPPORTED; }
-    if (std::min(rows, cols) > 16384 || std::max(rows, cols) > (1 << 20) || (rows + 128) * (cols + 8) >= (1LL << 30)) {
+    if (std::min(rows, cols) > 16384 || std::max(rows, cols) > (1 << 20) || (rows + 256) * (cols + 8) >= (1LL << 30)) {
         set_error("%s: the shorter side above 16384, the longer above 2^20 or 2^30 values", who);
         return WF_EUNSUPPORTED;
     }

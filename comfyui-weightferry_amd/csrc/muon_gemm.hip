@@ -13,42 +13,77 @@
 // from, and an error in the first X is multiplied by a^5 = 485 there. The products see X itself, 11 bits.
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
+#include "deep_ring.h"
 #include "dense_gemm.h"
 #include "muon.h"
+#include "tile_stage.h"
 
 namespace wf {
 
-// a wave's part of the idle stage buffers (four waves)
-template <typename S>
-__device__ __forceinline__ char* muon_region(wl_frag* sb0, wl_frag* sb1, int wave) {
-    static_assert(S::NW == 4, "two waves a buffer");
-    return reinterpret_cast<char*>(wave < 2 ? sb0 : sb1) + (wave & 1) * (S::SLOTS * 8);
-}
-
-__device__ __forceinline__ int muon_spread(int w, int T) {        // XCD w % 8 takes consecutive tiles
-    return w < (T & ~7) ? (w & 7) * (T >> 3) + (w >> 3) : w;
-}
-
 __device__ __forceinline__ float f16_at(uint64_t v, int i) { return f16_bits_to_f32((uint32_t)(v >> (16 * i)) & 0xffffu); }
 
-// Workgroup (tile, slice, matrix). parts: [batch, slices, tiles, accumulators of a workgroup], NULL without slices. SUM: the second
+// Workgroup w of W runs on XCD w % 8: which of the W pieces of work, in an order whose neighbours share operands, it takes so that an XCD
+// takes neighbours. The pieces are all matrices' tiles, one matrix after the other: an XCD's L2 then sees one matrix of a batch, or few.
+__device__ __forceinline__ int muon_spread(int w, int W) {
+    return w < (W & ~7) ? (w & 7) * (W >> 3) + (w >> 3) : w;
+}
+// tile t of an nt x nt lower triangle: bands of `band` rows, a band's columns one after the other
+__device__ __forceinline__ void triangle_tile(int t, int nt, int band, int& tm, int& tn) {
+    int r0 = 0, rows = min(band, nt);
+    for (;; r0 += rows, rows = min(band, nt - r0)) {
+        const int here = rows * r0 + rows * (rows + 1) / 2;
+        if (t < here) break;
+        t -= here;
+    }
+    if (t < rows * (r0 + 1)) {                                     // columns left of the diagonal, and its first
+        tn = t / rows;
+        tm = r0 + t % rows;
+        return;
+    }
+    t -= rows * (r0 + 1);
+    for (tn = r0 + 1; t >= rows - (tn - r0); tn++) t -= rows - (tn - r0);
+    tm = tn + t;
+}
+
+// acc over stages s0 .. s0 + nk of a . b in one of the two main loops: four stage buffers for the small tiles, else two
+template <typename S, bool AX, bool BX>
+struct MuonLoop {
+    static constexpr bool DEEP = S::BM * S::BN <= 64 * 64;
+    static constexpr int MORE = DEEP ? S::SLOTS : 1;              // of the third and fourth buffer
+    static constexpr int WAVES = DEEP ? 2 : S::WAVES;             // a SIMD
+    __device__ __forceinline__ static void run(const DenseTile& ta, const DenseTile& tb, int s0, int nk, int wave, int lane, wl_frag* sb0,
+                                               wl_frag* sb1, wl_frag* sb2, wl_frag* sb3, f32x16v (&acc)[S::WM][S::WN]) {
+        auto mma = [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<WF_F16>(c, x, y); };
+        if constexpr (DEEP) {
+            using LA = std::conditional_t<AX, DenseAcross<S::BM, S::NW, S::AW, S::WM>, DenseAlong<S::BM, S::NW, S::AW, S::WM>>;
+            using LB = std::conditional_t<BX, DenseAcross<S::BN, S::NW, S::BW, S::WN>, DenseAlong<S::BN, S::NW, S::BW, S::WN>>;
+            wl_frag* const sb[kDeep] = {sb0, sb1, sb2, sb3};
+            deep_loop<S, LA, LB>(ta, tb, s0, nk, wave, lane, sb, acc, mma);
+        } else {
+            dense_mainloop<S, AX, BX>(ta, tb, s0, nk, wave, lane, sb0, sb1, acc, mma);
+        }
+    }
+};
+
+// Workgroup (tile of a matrix, slice). parts: [batch, slices, tiles, accumulators of a workgroup], NULL without slices. SUM: the second
 // launch, its slice the only one.
 template <bool X, typename S, bool SUM>
-__global__ __launch_bounds__(S::NT, S::WAVES) void muon_sym(DenseOperand o, int64_t o_step, MuonSymmetric q, int64_t s_step, int side,
-                                                            int sld, int stages, int slice_stages, int slices,
+__global__ __launch_bounds__(S::NT, (MuonLoop<S, X, X>::WAVES)) void muon_sym(DenseOperand o, int64_t o_step, MuonSymmetric q, int64_t s_step, int side,
+                                                            int sld, int stages, int slice_stages, int slices, int T, int band,
                                                             float* __restrict__ parts) {
     constexpr int WM = S::WM, WN = S::WN, LANES = WM * WN * 16 * S::NT;
     static_assert(S::BM == S::BN && WM == WN, "tiles that turn into tiles");
-    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS];
-    const int T = gridDim.x, tile = __builtin_amdgcn_readfirstlane(muon_spread(blockIdx.x, T));
-    int tm = (int)((sqrtf(8.0f * (float)tile + 1.0f) - 1.0f) * 0.5f);
-    while (tm * (tm + 1) / 2 > tile) tm--;
-    while ((tm + 1) * (tm + 2) / 2 <= tile) tm++;
-    const int m0 = __builtin_amdgcn_readfirstlane(tm * S::BM), n0 = __builtin_amdgcn_readfirstlane((tile - tm * (tm + 1) / 2) * S::BN);
+    using Loop = MuonLoop<S, X, X>;
+    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS], sb2[SUM ? 1 : Loop::MORE], sb3[SUM ? 1 : Loop::MORE];
+    const int piece = __builtin_amdgcn_readfirstlane(muon_spread(blockIdx.x, gridDim.x)), tile = piece % T;
+    const int64_t b = piece / T;
+    int tm, tn;
+    triangle_tile(tile, (side + S::BM - 1) / S::BM, band, tm, tn);
+    const int m0 = __builtin_amdgcn_readfirstlane(tm * S::BM), n0 = __builtin_amdgcn_readfirstlane(tn * S::BN);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t b = blockIdx.z;
     f32x16v acc[WM][WN];
 #pragma unroll
     for (int i = 0; i < WM; i++)
@@ -71,8 +106,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void muon_sym(DenseOperand o, int6
         o.p += b * o_step;
         const int s0 = blockIdx.y * slice_stages, nk = min(slice_stages, stages - s0);
         const DenseTile ta = dense_tile<X>(o, m0), tb = dense_tile<X>(o, n0);
-        dense_mainloop<S, X, X>(ta, tb, s0, nk, wave, lane, sb0, sb1, acc,
-                                [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<WF_F16>(c, x, y); });
+        Loop::run(ta, tb, s0, nk, wave, lane, sb0, sb1, sb2, sb3, acc);
         if (parts) {
             float* p = at(blockIdx.y);
 #pragma unroll
@@ -104,11 +138,11 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void muon_sym(DenseOperand o, int6
                 for (int x = 0; x < 4; x++) {
                     r[x] = q.alpha * acc[i][j][4 * y + x];
                     if (in) r[x] = fmaf(q.beta, f16_at(c, x), r[x]);
-                    if (m + x == n && n < side) r[x] += q.gamma;
+                    if (m0 == n0 && m + x == n && n < side) r[x] += q.gamma;
                 }
                 v[i][j][y] = pack_f16(r[0], r[1]) | (uint64_t)pack_f16(r[2], r[3]) << 32;
             }
-    uint16_t* lds = reinterpret_cast<uint16_t*>(muon_region<S>(sb0, sb1, wave));
+    uint16_t* lds = reinterpret_cast<uint16_t*>(TileStage<S>::region(sb0, sb1, wave));
     wl_store_tile<WM, WN>(lds, out, side, sld, mw, nw, lane,
                           [&](int i, int j, int x) { return (uint16_t)(v[i][j][x >> 2] >> (16 * (x & 3))); });
     if (m0 == n0) return;
@@ -132,18 +166,18 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void muon_sym(DenseOperand o, int6
     }
 }
 
-// Workgroup (tile, matrix) of the outputs [rows, cols]; BX: b lies across K.
+// Workgroup: a tile of a matrix's outputs [rows, cols]; BX: b lies across K.
 template <bool BX, typename S>
-__global__ __launch_bounds__(S::NT, S::WAVES) void muon_upd(DenseOperand a, int64_t a_step, DenseOperand bo, int64_t b_step, MuonUpdate q,
+__global__ __launch_bounds__(S::NT, (MuonLoop<S, false, BX>::WAVES)) void muon_upd(DenseOperand a, int64_t a_step, DenseOperand bo, int64_t b_step, MuonUpdate q,
                                                             int64_t x_step, int rows, int cols, int ld, int K, MuonTensors t) {
     constexpr int WM = S::WM, WN = S::WN, TC = WN * 32;
-    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS];
+    using Loop = MuonLoop<S, false, BX>;
+    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS], sb2[Loop::MORE], sb3[Loop::MORE];
     const int ntm = (rows + S::BM - 1) / S::BM, ntn = (cols + S::BN - 1) / S::BN;
-    int tm, tn;
-    tile_order(blockIdx.x, ntm * ntn, ntm, ntn, tm, tn);
-    const int m0 = __builtin_amdgcn_readfirstlane(tm * S::BM), n0 = __builtin_amdgcn_readfirstlane(tn * S::BN);
+    const int T = ntm * ntn, piece = __builtin_amdgcn_readfirstlane(muon_spread(blockIdx.x, gridDim.x)), b = piece / T, t0 = piece % T;
+    const int first = t0 / (8 * ntn) * 8, high = min(ntm - first, 8);      // bands of 8 rows of tiles, column by column
+    const int m0 = (first + (t0 - first * ntn) % high) * S::BM, n0 = (t0 - first * ntn) / high * S::BN;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.y;
     a.p += b * a_step;
     bo.p += b * b_step;
     f32x16v acc[WM][WN];
@@ -154,59 +188,83 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void muon_upd(DenseOperand a, int6
 #pragma unroll
             for (int x = 0; x < 16; x++) acc[i][j][x] = 0.0f;
     const DenseTile ta = dense_tile<false>(a, m0), tb = dense_tile<BX>(bo, n0);
-    dense_mainloop<S, false, BX>(ta, tb, 0, (K + 63) / 64, wave, lane, sb0, sb1, acc,
-                                 [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<WF_F16>(c, x, y); });
+    Loop::run(ta, tb, 0, (K + 63) / 64, wave, lane, sb0, sb1, sb2, sb3, acc);
     const int mw = m0 + wave / S::VN * WM * 32, nw = n0 + wave % S::VN * TC;
-    const int lr = lane & 31, lk = lane >> 5;
-    // 16 rows at a time through LDS in float32, then runs of 8 outputs
-    static_assert(16 * TC * 4 <= S::SLOTS * 8, "the rows fit a wave's region");
-    float* lds = reinterpret_cast<float*>(muon_region<S>(sb0, sb1, wave));
-    constexpr int RUNS = TC / 8;
+    using Stage = TileStage<S>;
+    float* st = Stage::region(sb0, sb1, wave);
+    if (q.next && !q.lo) {
+        wl_store_tile<WM, WN>(reinterpret_cast<uint16_t*>(st), q.next + b * x_step, rows, ld, mw, nw, lane,
+                              [&](int i, int j, int x) { return from_f32<WF_F16>(q.alpha * acc[i][j][x]); });
+        return;
+    }
+    constexpr int ROWS = Stage::ROWS, RUNS = ROWS * TC / 8 / 64, U = RUNS % 4 == 0 ? 4 : RUNS;
+    // U runs' loads in flight together
+    static_for<Stage::PHASES>([&](auto pc) {
+        constexpr int P = decltype(pc)::value;
+        const int mp = mw + P * ROWS;
+        if (mp >= rows) return;
+        auto at = [&](int it, int& m, int& n) {
+            const int p = it * 64 + lane;
+            m = mp + p / (TC / 8);
+            n = nw + 8 * (p % (TC / 8));
+            return m < rows && n < (q.next ? ld : cols);
+        };
+        Pack<WF_F16> x[U], r[U];
+        auto fetch = [&](int it) {
 #pragma unroll
-    for (int half = 0; half < 2 * WM; half++) {
-        if (mw + half * 16 >= rows) break;
-#pragma unroll
-        for (int x = 0; x < 8; x++)
-#pragma unroll
-            for (int j = 0; j < WN; j++)
-                lds[(8 * (x >> 2) + 4 * lk + (x & 3)) * TC + j * 32 + lr] = acc[half / 2][j][8 * (half & 1) + x];
+            for (int u = 0; u < U; u++) {
+                int m, n;
+                x[u].zero();
+                r[u].zero();
+                if (at(it + u, m, n)) {
+                    x[u].load(q.x + b * x_step + (int64_t)m * ld + n, 8);
+                    r[u].load(q.lo + b * x_step + (int64_t)m * ld + n, 8);
+                }
+            }
+        };
+        if (q.lo) fetch(0);
+        Stage::template put<P>(st, acc, lane);
 #pragma unroll 1
-        for (int it = 0; it < (16 * RUNS + 63) / 64; it++) {
-            const int p = it * 64 + lane, m = mw + half * 16 + p / RUNS, n = nw + 8 * (p % RUNS);
-            if (p >= 16 * RUNS || m >= rows || n >= (q.next ? ld : cols)) continue;
-            const float4 lo4 = reinterpret_cast<const float4*>(lds)[2 * p], hi4 = reinterpret_cast<const float4*>(lds)[2 * p + 1];
-            float v[8] = {lo4.x, lo4.y, lo4.z, lo4.w, hi4.x, hi4.y, hi4.z, hi4.w};
+        for (int it = 0; it < RUNS; it += U) {
+            Pack<WF_F16> xc[U], rc[U];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] *= q.alpha;
-            const int64_t at = b * x_step + (int64_t)m * ld + n;
-            if (q.lo) {
-                Pack<WF_F16> x, r;
-                x.load(q.x + at, 8);
-                r.load(q.lo + at, 8);
+            for (int u = 0; u < U; u++) xc[u] = x[u], rc[u] = r[u];
+            if (q.lo && it + U < RUNS) fetch(it + U);
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = fmaf(q.a, fmaf(r.get(i), 1.0f / 2048.0f, x.get(i)), v[i]);
-            }
-            if (!q.next) {
-                muon_apply(t, b, (int64_t)m * cols + n, v, cols - n);
-                continue;
-            }
-            Pack<WF_F16> o;
-            o.put(v);
-            o.store(q.next + at, 8);
-            if (q.lo) {
-                float w[8];
+            for (int u = 0; u < U; u++) {
+                int m, n;
+                if (!at(it + u, m, n)) continue;
+                float v[8];
+                staged_run(v, st + ((it + u) * 64 + lane) * 8);
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = (v[i] - o.get(i)) * 2048.0f;
-                Pack<WF_F16> r;
-                r.put(w);
-                r.store(q.lo + at, 8);
+                for (int i = 0; i < 8; i++) v[i] *= q.alpha;
+                const int64_t to = b * x_step + (int64_t)m * ld + n;
+                if (q.lo)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = fmaf(q.a, fmaf(rc[u].get(i), 1.0f / 2048.0f, xc[u].get(i)), v[i]);
+                if (!q.next) {
+                    muon_apply(t, b, (int64_t)m * cols + n, v, cols - n);
+                    continue;
+                }
+                Pack<WF_F16> o;
+                o.put(v);
+                o.store(q.next + to, 8);
+                if (q.lo) {
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) w[i] = (v[i] - o.get(i)) * 2048.0f;
+                    o.put(w);
+                    o.store(q.lo + to, 8);
+                }
             }
         }
-    }
+    });
 }
 
 // ------------------------------------------------------------------------------------------------- host side
-// us of a workgroup, of each 64 values of K, and that where per_cu of them share a CU
+// The times that choose a tiling, in us: of a workgroup, of each 64 values of K, and that where per_cu of them share a CU; least-squares
+// fits to 268 measured launches of 17 shapes (64 x 128 x 512 to 13824 x 5120), off by 13 % on average for the symmetric product and by 9 %
+// for the update.
 struct MuonTile {
     int bm, bn, per_cu;
     float fixed, stage, shared;
@@ -222,7 +280,7 @@ static float muon_time(const MuonTile& q, int64_t wgs, int64_t stages) {
     return (float)full * together(q.per_cu) + together(rest);
 }
 
-constexpr MuonTile kSymmetric[] = {{256, 256, 1, 5.0f, 1.252f, 1.252f}, {128, 128, 2, 2.5f, 0.634f, 0.519f}, {64, 64, 4, 2.0f, 0.42f, 0.20f}};
+constexpr MuonTile kSymmetric[] = {{256, 256, 1, 14.5f, 1.10f, 1.10f}, {128, 128, 2, 4.0f, 0.53f, 0.52f}, {64, 64, 2, 1.75f, 0.20f, 0.25f}};
 struct MuonSlices {
     int tiling, tiles, slices, slice_stages;
 };
@@ -235,9 +293,10 @@ static MuonSlices muon_symmetric_plan(const MuonShape& s, int64_t K) {
         const int64_t across = (s.side + q.bm - 1) / q.bm, tiles = across * (across + 1) / 2;
         for (int want : {1, 2, 3, 4, 6, 8, 12, 16}) {
             const int64_t per = (stages + want - 1) / want, slices = (stages + per - 1) / per, wgs = tiles * s.batch * slices;
-            if (want > 1 && (slices != want || per < 3 || wgs > 1600)) continue;
+            if (want > 1 && (t == 0 || slices != want || per < 3 || wgs > 1600)) continue;
             float c = muon_time(q, wgs, per);
-            if (want > 1) c += 5.0f + 0.8e-6f * (float)(tiles * s.batch) * (float)(q.bm * q.bn) * (float)(slices + 1);
+            // the sum's launch: 64 x 64 tiles 4 to 8 us, 128 x 128 7 to 20; 256 x 256 up to 150, and they never gain
+            if (want > 1) c += 2.0f + (t == 2 ? 3.8f : 7.0f) + 0.8e-6f * (float)(tiles * s.batch * slices) * (float)(q.bm * q.bn);
             if (c < least) least = c, best = {t, (int)tiles, (int)slices, (int)per};
         }
     }
@@ -263,10 +322,12 @@ void muon_symmetric(const MuonShape& s, const MuonSymmetric& q, float* parts, hi
         constexpr bool X = decltype(x)::value;
         using S = decltype(shape);
         float* w = p.slices > 1 ? parts : nullptr;
-        muon_sym<X, S, false><<<dim3(p.tiles, p.slices, s.batch), S::NT, 0, st>>>(o, o_step, q, s_step, s.side, s.sld, (K + 63) / 64,
-                                                                                 p.slice_stages, p.slices, w);
-        if (w)
-            muon_sym<X, S, true><<<dim3(p.tiles, 1, s.batch), S::NT, 0, st>>>(o, o_step, q, s_step, s.side, s.sld, 0, 0, p.slices, w);
+        // (bands about as high as an XCD's share of the tiles is wide)
+        const int band = std::max(1, std::min(8, (int)std::sqrt((double)p.tiles * s.batch / 8.0)));
+        const dim3 grid(p.tiles * s.batch, p.slices), one(p.tiles * s.batch);
+        muon_sym<X, S, false><<<grid, S::NT, 0, st>>>(o, o_step, q, s_step, s.side, s.sld, (K + 63) / 64, p.slice_stages, p.slices,
+                                                      p.tiles, band, w);
+        if (w) muon_sym<X, S, true><<<one, S::NT, 0, st>>>(o, o_step, q, s_step, s.side, s.sld, 0, 0, p.slices, p.tiles, band, w);
     };
     auto by = [&](auto x) {
         if (p.tiling == 0) go(x, DenseShape<2, 2, 4, 4>{});
@@ -277,8 +338,8 @@ void muon_symmetric(const MuonShape& s, const MuonSymmetric& q, float* parts, hi
     else by(std::false_type{});
 }
 
-constexpr MuonTile kUpdate[] = {{256, 256, 1, 6.0f, 1.252f, 1.252f}, {256, 192, 1, 4.5f, 1.076f, 1.076f},
-                                {128, 128, 2, 2.5f, 0.634f, 0.519f}, {64, 128, 3, 1.5f, 0.47f, 0.367f}};
+constexpr MuonTile kUpdate[] = {{256, 320, 1, 12.3f, 1.70f, 1.70f}, {256, 192, 1, 13.3f, 1.12f, 1.12f},
+                                {128, 128, 2, 5.5f, 0.57f, 0.50f}, {64, 64, 2, 2.7f, 0.20f, 0.19f}};
 
 void muon_update(const MuonShape& s, const MuonUpdate& q, const MuonTensors& t, hipStream_t st) {
     int tiling = 0;
@@ -294,7 +355,7 @@ void muon_update(const MuonShape& s, const MuonUpdate& q, const MuonTensors& t, 
     auto go = [&](auto bx, auto shape) {
         constexpr bool BX = decltype(bx)::value;
         using S = decltype(shape);
-        const dim3 grid(((s.rows + S::BM - 1) / S::BM) * ((s.cols + S::BN - 1) / S::BN), s.batch);
+        const dim3 grid(((s.rows + S::BM - 1) / S::BM) * ((s.cols + S::BN - 1) / S::BN) * s.batch);
         if constexpr (BX) {                                        // q x: x's columns are rows that lie across the sum
             const DenseOperand x = {q.x, s.ld, s.rows, s.cols, true};
             muon_upd<true, S><<<grid, S::NT, 0, st>>>(q_along, q_step, x, x_step, q, x_step, s.rows, s.cols, s.ld, s.side, t);
@@ -304,10 +365,10 @@ void muon_update(const MuonShape& s, const MuonUpdate& q, const MuonTensors& t, 
         }
     };
     auto by = [&](auto bx) {
-        if (tiling == 0) go(bx, DenseShape<2, 2, 4, 4>{});
+        if (tiling == 0) go(bx, DenseShape<4, 2, 2, 5>{});
         else if (tiling == 1) go(bx, DenseShape<2, 2, 4, 3>{});
         else if (tiling == 2) go(bx, DenseShape<2, 2, 2, 2>{});
-        else go(bx, DenseShape<1, 4, 2, 1>{});
+        else go(bx, DenseShape<2, 2, 1, 1>{});
     };
     if (s.tall) by(std::false_type{});
     else by(std::true_type{});

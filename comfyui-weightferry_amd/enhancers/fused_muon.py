@@ -17,7 +17,7 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)     # steep at zero: small singular val
 _TYPES = frozenset((torch.Tensor, torch.nn.Parameter))
 _dtype, _index, _contiguous = operator.attrgetter("dtype"), torch.Tensor.get_device, torch.Tensor.is_contiguous
 _capturing = torch.cuda.is_current_stream_capturing
-_data_ptr = torch.Tensor.data_ptr
+_data_ptr, _numel, _shape = torch.Tensor.data_ptr, torch.Tensor.numel, operator.attrgetter("shape")
 MAX_SHORT, MAX_LONG, MAX_VALUES = 16384, 1 << 20, 1 << 30
 
 
@@ -31,7 +31,7 @@ _bytes = Sizes(_ask)
 
 
 def _fits(rows, cols):
-    return min(rows, cols) <= MAX_SHORT and max(rows, cols) <= MAX_LONG and (rows + 128) * (cols + 8) < MAX_VALUES
+    return min(rows, cols) <= MAX_SHORT and max(rows, cols) <= MAX_LONG and (rows + 256) * (cols + 8) < MAX_VALUES
 
 
 _known = {}
@@ -103,11 +103,11 @@ def _odd_one(params, grads, momenta, dt, dev):
         if p.dim() != 2:
             return f"parameter {tuple(p.shape)}: matrices are wanted (fused_adamw steps the others)"
         for t, want in ((p, dt), (g, dt), (m, torch.float32)):
-            if t.dtype != want or t.device != dev or not t.is_contiguous() or t.shape != p.shape or type(t) not in _TYPES:
+            if t.dtype != want or t.device != dev or not t.is_contiguous() or t.numel() != p.numel() or type(t) not in _TYPES:
                 return (f"parameter {tuple(p.shape)} {p.dtype} on {p.device}, gradient {tuple(g.shape)} {g.dtype} on {g.device}, "
                         f"momentum {tuple(m.shape)} {m.dtype} on {m.device}: plain contiguous matrices of one shape, {dt} and "
                         f"float32 momenta on {dev}, are wanted")
-    return "parameters, gradients and momenta do not fit together"
+    return "a gradient has another shape than its parameter"
 
 
 def _ready(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, coefficients, eps, adjust):
@@ -130,34 +130,40 @@ def _ready(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, 
                            "repeat them")
     if not plain(dev):
         raise ValueError("a step inside a functorch transform or a trace, which would not see it")
-    both, every = params + grads, params + grads + momenta
-    shapes = [p.shape for p in params]
-    if (set(map(_dtype, both)) != {dt} or set(map(_dtype, momenta)) != {torch.float32} or set(map(_index, every)) != {dev.index}
-            or not all(map(_contiguous, every)) or not _TYPES.issuperset(map(type, every)) or set(map(len, shapes)) != {2}
-            or shapes != [g.shape for g in grads] or shapes != [m.shape for m in momenta]):
+    # (questions of all tensors at once: with hundreds of adapters they are the step's host time, a microsecond a matrix)
+    every = params + grads + momenta
+    shapes, many = list(map(_shape, params)), len(params)
+    if (set(map(_dtype, params + grads)) != {dt} or set(map(_dtype, momenta)) != {torch.float32}
+            or set(map(_index, every)) != {dev.index} or not all(map(_contiguous, every))
+            or not _TYPES.issuperset(map(type, every)) or set(map(len, shapes)) != {2} or shapes != list(map(_shape, grads))
+            or list(map(_numel, params)) != list(map(_numel, momenta))):
         raise ValueError(_odd_one(params, grads, momenta, dt, dev))
-    if any(t.is_neg() for t in every):
-        raise ValueError("a negative view: what it stands for is not in its memory")
-    at = [list(map(_data_ptr, ts)) for ts in (params, grads, momenta)]
-    by_shape, need = {}, 0
+    by_shape = {}
     for i, shape in enumerate(shapes):
-        if shape.numel():
-            by_shape.setdefault(tuple(shape), []).append(i)
+        which = by_shape.get(shape)
+        if which is None:
+            by_shape[shape] = [i]
+        else:
+            which.append(i)
+    at, need, order, calls = list(map(_data_ptr, every)), 0, [], []
     for (rows, cols), which in by_shape.items():
-        if not _fits(rows, cols):
-            raise ValueError(f"a matrix of {rows} x {cols}: the shorter side is at most {MAX_SHORT}, the longer {MAX_LONG}")
-        need = max(need, _bytes((len(which), rows, cols)))
-    changed = [a for a, s in zip(at[0], shapes) if s.numel()] + [a for a, s in zip(at[2], shapes) if s.numel()]
+        if rows and cols:
+            if not _fits(rows, cols):
+                raise ValueError(f"a matrix of {rows} x {cols}: the shorter side is at most {MAX_SHORT}, the longer {MAX_LONG}, "
+                                 f"and there are fewer than {MAX_VALUES} values")
+            # (contiguous, but not what its memory holds: only a single value can be both without a private call)
+            if rows * cols == 1 and any(t[i].is_neg() for t in (params, grads, momenta) for i in which):
+                raise ValueError("a negative view: what it stands for is not in its memory")
+            need = max(need, _bytes((len(which), rows, cols)))
+            calls.append((24 * len(order), len(which), rows, cols, lr * _size(adjust, rows, cols)))
+            order += which
+    changed = at[:many] + at[2 * many:] if len(order) == many else [at[i + k] for i in order for k in (0, 2 * many)]
     if len(set(changed)) != len(changed):
         raise ValueError("a parameter or a momentum is there twice: each is stepped on its own")
-    table = array.array("q", [0]) * (3 * sum(map(len, by_shape.values())))
-    calls, first = [], 0
-    for (rows, cols), which in by_shape.items():
-        end = first + 3 * len(which)
-        for k in range(3):
-            table[first + k:end:3] = array.array("q", [at[k][i] for i in which])
-        calls.append((8 * first, len(which), rows, cols, lr * _size(adjust, rows, cols)))
-        first = end
+    table = array.array("q", bytes(24 * len(order)))
+    for k in range(3):
+        column = at[k * many:(k + 1) * many]
+        table[k::3] = array.array("q", map(column.__getitem__, order))
 
     def launch():
         if not calls:
@@ -179,7 +185,8 @@ def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, wei
     """A step on ``params`` and ``momenta`` in place: m = momentum m + (1 - momentum) g; the update is m, or with ``nesterov``
     momentum m + (1 - momentum) g, orthogonalised as by ``orthogonalize``; p = (1 - lr weight_decay) p - lr s update, s =
     sqrt(max(1, rows / cols)) ("spectral") or 0.2 sqrt(max(rows, cols)) ("rms": updates as large as AdamW's). ``params`` and ``grads``:
-    contiguous GPU matrices of one type (float32, bfloat16 or float16), ``momenta`` float32 (``muon_momenta``), all on one device, none twice.
+    contiguous GPU matrices of one type (float32, bfloat16 or float16); ``momenta``: contiguous, float32, as many values
+    (``muon_momenta``); all on one device, no parameter or momentum twice.
     ValueError for anything else. Asynchronous on torch's current stream; RuntimeError while that is captured into a graph."""
     _ready(list(params), list(grads), list(momenta), lr, momentum, nesterov, weight_decay, steps, coefficients, eps, adjust)()
 

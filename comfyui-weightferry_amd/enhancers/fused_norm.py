@@ -124,38 +124,38 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, modulation=False):
 
 # ------------------------------------------------------------------------- the norms around a gated residual
 NORMS = {"rms": 1, "layer": 2}
+_POSTS = {None: 0, **NORMS}
 MAX_ROW_BYTES = 32768
 
 
-def _ask_block(code, rows, width, groups, sums):
-    q, need = _native.BlockNorm(dt=code, norm=1, groups=groups), ctypes.c_int64()
-    _native.call("wf_block_norm_bwd_workspace", ctypes.byref(q), rows, width, sums, ctypes.byref(need))
+def _block(*how):
+    """A call's kinds, types and groups as the library takes them: its address, and what keeps that valid."""
+    q = _native.BlockNorm(*how)
+    return ctypes.addressof(q), q
+
+
+def _ask_block(q, rows, width, sums):
+    need = ctypes.c_int64()
+    _native.call("wf_block_norm_bwd_workspace", q, rows, width, sums, ctypes.byref(need))
     return need.value
 
 
-_bytes_block = Sizes(_ask_block)
+_blocks = Sizes(_block)
+_bytes_block = Sizes(lambda how, rows, width, sums: _ask_block(_blocks(how)[0], rows, width, sums))
 
 
-def _block(how, post_weight, gate, weight, bias):
-    """The call's parameters as the library takes them."""
-    code, post, norm, plus_one, scale, eps, groups, gate_groups, weight_groups = how
-    wcode = code if weight is None and bias is None else CODES[(bias if weight is None else weight).dtype]
-    return _native.BlockNorm(code, post, norm, plus_one, code if post_weight is None else CODES[post_weight.dtype],
-                             code if gate is None else CODES[gate.dtype], wcode, scale, eps, groups, gate_groups,
-                             weight_groups, ptr(post_weight), ptr(gate), ptr(weight), ptr(bias))
-
-
-def _launch_block(x2, h2, params, how, stats):
+def _launch_block(x2, h2, post_weight, gate, weight, bias, how, stats):
     """(r, or None without a branch, and y)"""
     rows, width = x2.shape
     dev = x2.device
     y = torch.empty((rows, width), dtype=x2.dtype, device=dev)
     r = None if h2 is None else torch.empty_like(y)
     if rows:
+        q = _blocks(how)
         with _native.on_device(dev):
-            rc = _native.lib().wf_block_norm_fwd(ctypes.byref(_block(how, *params)), x2.data_ptr(), x2.stride(0), ptr(h2),
-                                                 0 if h2 is None else h2.stride(0), ptr(r), y.data_ptr(), ptr(stats), rows,
-                                                 width, _native.stream_of(dev))
+            rc = _native.lib().wf_block_norm_fwd(q[0], x2.data_ptr(), x2.stride(0), ptr(h2), 0 if h2 is None else h2.stride(0),
+                                                 ptr(post_weight), ptr(gate), ptr(weight), ptr(bias), ptr(r), y.data_ptr(),
+                                                 ptr(stats), rows, width, _native.stream_of(dev))
         if rc:
             _native.must(rc, "wf_block_norm_fwd")
     return r, y
@@ -165,18 +165,20 @@ class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, branch, post_weight, gate, weight, bias, how):
         ctx.set_materialize_grads(False)
-        width = x.shape[-1]
+        shape = x.shape
+        width = shape[-1]
         x2, h2 = rows_of(x, width), None if branch is None else rows_of(branch, width)
-        params = whole(post_weight), whole(gate), whole(weight), whole(bias)
+        pw, g, w = whole(post_weight), whole(gate), whole(weight)
         stats = torch.empty((x2.shape[0], 4), dtype=torch.float32, device=x2.device)
-        r, y = _launch_block(x2, h2, params, how, stats)
-        ctx.how = how, x.shape, tuple(None if t is None else (t.shape, t.dtype) for t in (post_weight, gate, weight, bias))
-        ctx.save_for_backward(x2, h2, *params[:3], stats)
-        return y.view(x.shape) if r is None else (r.view(x.shape), y.view(x.shape))
+        r, y = _launch_block(x2, h2, pw, g, w, whole(bias), how, stats)
+        ctx.how = how, shape, tuple(None if t is None else (t.shape, t.dtype) for t in (post_weight, gate, weight, bias))
+        ctx.save_for_backward(x2, h2, pw, g, w, stats)
+        if len(shape) == 2:
+            return y if r is None else (r, y)
+        return y.view(shape) if r is None else (r.view(shape), y.view(shape))
 
     @once
     def backward(ctx, *grads):
-        grads = [None if d is None else gradient(d) for d in grads]
         dr, dy = grads if len(grads) == 2 else (None, grads[0])
         if dr is None and dy is None:
             return (None,) * 7
@@ -184,25 +186,25 @@ class _BlockNorm(torch.autograd.Function):
         how, shape, specs = ctx.how
         need = ctx.needs_input_grad
         rows, width = x2.shape
-        dev = x2.device
+        dt, dev = x2.dtype, x2.device
+        dr = None if dr is None else rows_of(gradient(dr), width)
+        dy = None if dy is None else rows_of(gradient(dy), width)
         new = torch.empty if rows else torch.zeros
-        dx = new(shape, dtype=x2.dtype, device=dev) if need[0] else None
-        dh = new(shape, dtype=x2.dtype, device=dev) if need[1] else None
-        dparams = [new(spec[0], dtype=spec[1], device=dev) if want else None for want, spec in zip(need[2:6], specs)]
+        dx = new(shape, dtype=dt, device=dev) if need[0] else None
+        dh = new(shape, dtype=dt, device=dev) if need[1] else None
+        dparams, sums = [], 0
+        for want, spec in zip(need[2:6], specs):
+            dparams.append(new(spec[0], dtype=spec[1], device=dev) if want else None)
+            sums += want
         if rows:
-            q = _block(how, post_weight, gate, weight, None)
-            if specs[3] is not None:
-                q.weight_dt = CODES[specs[3][1]]
-            d2 = [None if d is None else rows_of(d, width) for d in (dr, dy)]
-            sums = sum(t is not None for t in dparams)
-            size = _bytes_block((how[0], rows, width, how[6], sums)) if sums else 0
+            size = _bytes_block((how, rows, width, sums)) if sums else 0
             ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+            q = _blocks(how)
             with _native.on_device(dev):
                 rc = _native.lib().wf_block_norm_bwd(
-                    ctypes.byref(q), x2.data_ptr(), x2.stride(0), ptr(h2), 0 if h2 is None else h2.stride(0), ptr(d2[0]),
-                    0 if d2[0] is None else d2[0].stride(0), ptr(d2[1]), 0 if d2[1] is None else d2[1].stride(0),
-                    stats.data_ptr(), ptr(dx), ptr(dh), *map(ptr, dparams), rows, width, ptr(ws), size,
-                    _native.stream_of(dev))
+                    q[0], x2.data_ptr(), x2.stride(0), ptr(h2), 0 if h2 is None else h2.stride(0), ptr(post_weight), ptr(gate),
+                    ptr(weight), ptr(dr), 0 if dr is None else dr.stride(0), ptr(dy), 0 if dy is None else dy.stride(0),
+                    stats.data_ptr(), ptr(dx), ptr(dh), *map(ptr, dparams), rows, width, ptr(ws), size, _native.stream_of(dev))
             if rc:
                 _native.must(rc, "wf_block_norm_bwd")
         return (dx, dh, *dparams, None)
@@ -212,47 +214,58 @@ _apply_block = applier(_BlockNorm)
 
 
 def _block_norm(x, branch, gate, post_weight, weight, bias, eps, modulation, norm, post, scale):
-    if norm not in NORMS or (post is not None and post not in NORMS):
+    norm_code, post_code = NORMS.get(norm), _POSTS.get(post)
+    if norm_code is None or post_code is None:
         raise ValueError(f"norm={norm!r}, post={post!r}: one of {', '.join(map(repr, NORMS))}; post may be None")
-    if post is None and post_weight is not None:
-        raise ValueError("post_weight without the norm that it scales (post)")
-    dt, dev, dims = x.dtype, x.device, x.dim()
+    dt, dev, shape = x.dtype, x.device, x.shape
     code = CODES.get(dt)
-    if code is None or dims == 0 or dev.type != "cuda" or not plain(dev, x, branch, gate, post_weight, weight, bias):
+    if code is None or not shape or dev.type != "cuda" or not plain(dev, x, branch, gate, post_weight, weight, bias):
         return None
     if branch is not None:
-        if branch.shape != x.shape:
-            raise ValueError(f"branch has shape {tuple(branch.shape)}: {tuple(x.shape)} is wanted")
+        if branch.shape != shape:
+            raise ValueError(f"branch has shape {tuple(branch.shape)}: {tuple(shape)} is wanted")
         if branch.dtype != dt:
             return None
-    width = x.shape[-1]
-    if not 0 < width * x.element_size() <= MAX_ROW_BYTES:
+    width = shape[-1]
+    if not 0 < width * (4 if code == 2 else 2) <= MAX_ROW_BYTES:
         return None
-    rows = x.numel() // width
-    if any(t is not None and t.dtype != dt and t.dtype != torch.float32 for t in (gate, post_weight, weight, bias)):
-        return None
-    if post_weight is not None and tuple(post_weight.shape) != (width,):
-        raise ValueError(f"post_weight has shape {tuple(post_weight.shape)}: ({width},) is wanted")
-    gate_groups = 1 if gate is None else groups_of(gate, rows, width, "gate")
-    weight_groups = 1
-    for t, what in ((weight, "weight"), (bias, "bias")):
-        if t is not None:
-            weight_groups = groups_of(t, rows, width, what)
-    if weight is not None and bias is not None:
-        if weight.numel() != bias.numel():
-            raise ValueError(f"weight {tuple(weight.shape)} and bias {tuple(bias.shape)} differ")
-        if weight.dtype != bias.dtype:
+    dims = len(shape)
+    rows = shape[0] if dims == 2 else x.numel() // width
+    gate_code = post_weight_code = weight_code = code
+    gate_groups = weight_groups = 1
+    if post_weight is not None:
+        if not post_code:
+            raise ValueError("post_weight without the norm that it scales (post)")
+        if post_weight.shape != (width,):
+            raise ValueError(f"post_weight has shape {tuple(post_weight.shape)}: ({width},) is wanted")
+        post_weight_code = CODES.get(post_weight.dtype)
+    if gate is not None:
+        gate_groups, gate_code = groups_of(gate, rows, width, "gate"), CODES.get(gate.dtype)
+    if weight is not None:
+        weight_groups, weight_code = groups_of(weight, rows, width, "weight"), CODES.get(weight.dtype)
+    if bias is not None:
+        groups = groups_of(bias, rows, width, "bias")
+        if weight is not None:
+            if groups != weight_groups:
+                raise ValueError(f"weight {tuple(weight.shape)} and bias {tuple(bias.shape)} differ")
+            if bias.dtype != weight.dtype:
+                return None
+        weight_groups, weight_code = groups, CODES.get(bias.dtype)
+    for c in (post_weight_code, gate_code, weight_code):
+        if c != code and c != 2:
             return None
-    groups = max(gate_groups, weight_groups)
-    if min(gate_groups, weight_groups) not in (1, groups) or groups > 65535 or rows >= 1 << 31:
+    groups = gate_groups if gate_groups > weight_groups else weight_groups
+    if groups > 1 and (gate_groups not in (1, groups) or weight_groups not in (1, groups) or groups > 65535) or rows >= 1 << 31:
         return None
-    how = (code, 0 if post is None else NORMS[post], NORMS[norm], 1 if modulation else 0, float(scale), float(eps), groups,
-           gate_groups, weight_groups)
+    how = (code, post_code, norm_code, 1 if modulation else 0, post_weight_code, gate_code, weight_code, float(scale), float(eps),
+           groups, gate_groups, weight_groups)
     if wants_grad(x, branch, post_weight, gate, weight, bias):
         return _apply_block(x, branch, post_weight, gate, weight, bias, how)
-    r, y = _launch_block(rows_of(x, width), None if branch is None else rows_of(branch, width),
-                         (whole(post_weight), whole(gate), whole(weight), whole(bias)), how, None)
-    return y.view(x.shape) if r is None else (r.view(x.shape), y.view(x.shape))
+    r, y = _launch_block(rows_of(x, width), None if branch is None else rows_of(branch, width), whole(post_weight), whole(gate),
+                         whole(weight), whole(bias), how, None)
+    if dims == 2:
+        return y if r is None else (r, y)
+    return y.view(shape) if r is None else (r.view(shape), y.view(shape))
 
 
 def residual_norm(x, branch, gate=None, post_weight=None, weight=None, bias=None, eps=1e-6, modulation=False, norm="rms",

@@ -198,22 +198,22 @@ int wf_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldd, i
  * x, h: rows x_row, h_row values apart; r, y: [M, K]; y comes from r before its rounding. stats (may be NULL): float32 [M, 4],
  * mean (0 for RMS) and reciprocal root of h's norm and of r's, what the backward pass reads.
  * wf_block_norm_bwd: dx and dh [M, K] of type dt, the parameters' gradients of their types, for the gradients dr of r and dy of
- * y (either may be NULL); any output may be NULL. The workspace (for as many parameters' gradients, `sums`, as are wanted; 4-byte
- * aligned) holds partial sums, added in a fixed order. */
+ * y (either may be NULL); any output may be NULL; bias is not read. The workspace (for as many parameters' gradients, `sums`, as are
+ * wanted; 4-byte aligned) holds partial sums, added in a fixed order. */
 typedef struct {
     int32_t dt, post, norm, plus_one;
     int32_t post_weight_dt, gate_dt, weight_dt;
     float scale, eps;
     int64_t groups, gate_groups, weight_groups;
-    const void *post_weight, *gate, *weight, *bias;
 } wf_block_norm;
-int wf_block_norm_fwd(const wf_block_norm* q, const void* x, int64_t x_row, const void* h, int64_t h_row, void* r, void* y,
-                      float* stats, int64_t M, int64_t K, void* stream);
+int wf_block_norm_fwd(const wf_block_norm* q, const void* x, int64_t x_row, const void* h, int64_t h_row, const void* post_weight,
+                      const void* gate, const void* weight, const void* bias, void* r, void* y, float* stats, int64_t M, int64_t K,
+                      void* stream);
 int wf_block_norm_bwd_workspace(const wf_block_norm* q, int64_t M, int64_t K, int sums, int64_t* bytes);
-int wf_block_norm_bwd(const wf_block_norm* q, const void* x, int64_t x_row, const void* h, int64_t h_row, const void* dr,
-                      int64_t dr_row, const void* dy, int64_t dy_row, const float* stats, void* dx, void* dh,
-                      void* dpost_weight, void* dgate, void* dweight, void* dbias, int64_t M, int64_t K, void* workspace,
-                      int64_t workspace_bytes, void* stream);
+int wf_block_norm_bwd(const wf_block_norm* q, const void* x, int64_t x_row, const void* h, int64_t h_row, const void* post_weight,
+                      const void* gate, const void* weight, const void* dr, int64_t dr_row, const void* dy, int64_t dy_row,
+                      const float* stats, void* dx, void* dh, void* dpost_weight, void* dgate, void* dweight, void* dbias, int64_t M,
+                      int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* y[m, n] = resid[m, n] + gate[m / rows_per_group, n] * act(sum_k x[m, k] * w[n, k] + bias[n]) in dt (WF_BF16 or WF_F16),
  * float32 accumulation, one rounding. act: 0 none, 1 GELU (erf), 2 GELU (tanh), 3 SiLU, 4 ReLU. bias, gate, resid may be
@@ -290,7 +290,7 @@ int wf_adamw_values(const int8_t* exp_avg, const uint8_t* exp_avg_sq, const floa
  * m (nesterov) or m, X = u / max(|u|, eps) with the Frobenius norm, `steps` times (1 to 32) X = a X + (b A + c A A) X, A = X X^T; then p =
  * keep p - rate X, in place (p and m). table: host memory, read before the call returns: addresses of p, g and m of each matrix; m
  * (float32) may be 0: u = g. coefficients: a, b, c; WF_EINVAL for ones that take singular values from [0, 1] past 1.9. The shorter side
- * <= 16384, the longer <= 2^20, (rows + 128) (cols + 8) < 2^30. No matrix may be there twice. With a shorter side up to 64 everything
+ * <= 16384, the longer <= 2^20, (rows + 256) (cols + 8) < 2^30. No matrix may be there twice. With a shorter side up to 64 everything
  * is float32 or more; above, the products' operands are float16 and X is good to 1e-3 of its norm. wf_orthogonalize: out = X, table:
  * addresses of out, g and 0. The workspace (256-byte aligned) need not be cleared. */
 int wf_muon_workspace(int64_t count, int64_t rows, int64_t cols, int64_t* bytes);
