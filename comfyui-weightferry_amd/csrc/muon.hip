@@ -28,29 +28,37 @@
 namespace wf {
 
 // -------------------------------------------------------------------------------------------------- a matrix's update u
-// 8 values of type D from i on, the first cnt (zeros for the others)
-__device__ __forceinline__ void muon_load(float (&v)[8], const void* p, int64_t i, int cnt, int dt) { load_params<8>(v, p, i, cnt, dt); }
-
-// u from g and m; STEP: m is stepped first, and stored
+// 8 places of a matrix's g and m from i on, the first cnt of them (zeros for the others)
+struct MuonRun {
+    float g[8], m[8];
+    __device__ __forceinline__ void load(const MuonTensors& t, int b, int64_t i, int cnt) {
+        load_params<8>(g, t.g[b], i, cnt, t.dt);
+        if (t.m[b]) load_params<8>(m, t.m[b], i, cnt, WF_F32);
+    }
+    // u; STEP: m is stepped first, and stored
+    template <bool STEP>
+    __device__ __forceinline__ void finish(float (&u)[8], const MuonTensors& t, int b, int64_t i, int cnt) const {
+        float* p = t.m[b];
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float d = t.nu * g[k];
+            v[k] = STEP ? fmaf(t.mu, m[k], d) : m[k];
+            u[k] = !p ? g[k] : t.nesterov ? fmaf(t.mu, v[k], d) : v[k];
+        }
+        if (!STEP || !p) return;
+        if (cnt >= 8) __builtin_memcpy(p + i, v, 32);
+        else
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (k < cnt) p[i + k] = v[k];
+    }
+};
 template <bool STEP>
 __device__ __forceinline__ void muon_u(float (&u)[8], const MuonTensors& t, int b, int64_t i, int cnt) {
-    muon_load(u, t.g[b], i, cnt, t.dt);
-    float* m = t.m[b];
-    if (!m) return;
-    float v[8];
-    load_params<8>(v, m, i, cnt, WF_F32);
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-        const float g = t.nu * u[k];
-        if (STEP) v[k] = fmaf(t.mu, v[k], g);
-        u[k] = t.nesterov ? fmaf(t.mu, v[k], g) : v[k];
-    }
-    if (!STEP) return;
-    if (cnt >= 8) __builtin_memcpy(m + i, v, 32);
-    else
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (k < cnt) m[i + k] = v[k];
+    MuonRun r;
+    r.load(t, b, i, cnt);
+    r.finish<STEP>(u, t, b, i, cnt);
 }
 
 __device__ __forceinline__ double wave_sum_f64(double v) {         // by halves: a fixed order
@@ -112,36 +120,73 @@ __global__ __launch_bounds__(256) void muon_scale(MuonTensors t, int rows, int c
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 constexpr int kNarrow = 64, kStretch = 256;                        // the longer side in stretches
 
-// Element (i of the shorter side, k of the longer) of a matrix is at i * si + k * sk, one of them 1. u[i][k] of the stretch from k0 on,
-// zeros past n and past the matrix's m rows, rows 4 banks apart (16 rows x 4 k of a matrix instruction's operand: all 64 banks).
+// Element (i of the shorter side, k of the longer) of a matrix is at i n + k, or where it is tall at k m + i. In LDS a stretch is
+// u[i][k], zeros past n and past the matrix's m rows, rows 4 banks apart (16 rows x 4 k of a matrix instruction's operand: all 64 banks).
 constexpr int kStretchRow = kStretch + 4;
-template <int MT, bool STEP>
-__device__ __forceinline__ void narrow_load(float* us, const MuonTensors& t, int b, int m, int64_t n, bool tall, int64_t k0) {
-    const int len = (int)min<int64_t>(kStretch, n - k0);
-    for (int i = threadIdx.x; i < 16 * MT * kStretchRow; i += 256) us[i] = 0.0f;
-    __syncthreads();
-    if (tall) {                                                    // the stretch is one run of values
-        const int64_t first = k0 * m;
-        const int size = len * m;
-        for (int i = threadIdx.x * 8; i < size; i += 2048) {
-            float u[8];
-            muon_u<STEP>(u, t, b, first + i, min(8, size - i));
-            int k = i / m, r = i - k * m;
-#pragma unroll
-            for (int x = 0; x < 8; x++) {
-                if (i + x < size) us[r * kStretchRow + k] = u[x];
-                if (++r == m) r = 0, k++;
-            }
+
+// The runs of 8 consecutive values of a stretch's memory, f(place in LDS of the first, offset in the matrix, count, u) each: G runs' loads
+// go out together, whatever load() does, before finish() does anything.
+struct NarrowRuns {
+    int m, len, runs;
+    int64_t n, k0;
+    bool tall;
+    __device__ __forceinline__ NarrowRuns(int m_, int64_t n_, bool tall_, int64_t k0_)
+        : m(m_), len((int)min<int64_t>(kStretch, n_ - k0_)), n(n_), k0(k0_), tall(tall_) {
+        runs = tall ? (len * m + 7) / 8 : m * (kStretch / 8);
+    }
+    // run i: its offset in the matrix, values (0: none), and its first value's place (r, k)
+    __device__ __forceinline__ int at(int i, int64_t& offset, int& r, int& k) const {
+        if (i >= runs) return 0;
+        if (tall) {                                                // (the stretch is one run of values)
+            offset = k0 * m + i * 8;
+            k = i * 8 / m;
+            r = i * 8 - k * m;
+            return min(8, len * m - i * 8);
         }
-    } else {
-        for (int i = threadIdx.x; i < m * (kStretch / 8); i += 256) {
-            const int r = i / (kStretch / 8), k = i % (kStretch / 8) * 8;
-            if (k >= len) continue;
-            float u[8];
-            muon_u<STEP>(u, t, b, r * n + k0 + k, min(8, len - k));
+        r = i / (kStretch / 8);
+        k = i % (kStretch / 8) * 8;
+        offset = r * n + k0 + k;
+        return min(8, len - k);
+    }
+    // f(x, place) for the run's 8 places from (r, k) on
+    template <typename F>
+    __device__ __forceinline__ void places(int r, int k, F&& f) const {
 #pragma unroll
-            for (int x = 0; x < 8; x++)
-                if (k + x < len) us[r * kStretchRow + k + x] = u[x];
+        for (int x = 0; x < 8; x++) {
+            f(x, r * kStretchRow + k);
+            if (!tall) k++;
+            else if (++r == m) r = 0, k++;
+        }
+    }
+};
+constexpr int kRunsAhead = 4;
+
+template <int MT, bool STEP>
+__device__ __forceinline__ void narrow_load(float* us, const MuonTensors& t, int b, const NarrowRuns& q) {
+    if (q.m != 16 * MT || q.len != kStretch) {
+        for (int i = threadIdx.x; i < 16 * MT * kStretchRow; i += 256) us[i] = 0.0f;
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < q.runs; i += 256 * kRunsAhead) {
+        MuonRun v[kRunsAhead];
+#pragma unroll
+        for (int h = 0; h < kRunsAhead; h++) {
+            int64_t offset;
+            int r, k;
+            const int cnt = q.at(i + 256 * h, offset, r, k);
+            if (cnt > 0) v[h].load(t, b, offset, cnt);
+        }
+#pragma unroll
+        for (int h = 0; h < kRunsAhead; h++) {
+            int64_t offset;
+            int r, k;
+            const int cnt = q.at(i + 256 * h, offset, r, k);
+            if (cnt <= 0) continue;
+            float u[8];
+            v[h].template finish<STEP>(u, t, b, offset, cnt);
+            q.places(r, k, [&](int x, int place) {
+                if (x < cnt) us[place] = u[x];
+            });
         }
     }
     __syncthreads();
@@ -150,12 +195,12 @@ __device__ __forceinline__ void narrow_load(float* us, const MuonTensors& t, int
 // Steps m and sums u u^T over a stretch: workgroup (stretch, matrix). parts: [batch, stretches, tiles, 64 lanes, 4], the 16 x 16 tiles on and
 // below the diagonal.
 template <int MT>
-__global__ __launch_bounds__(256) void narrow_gram(MuonTensors t, int m, int64_t n, int tall, f64x4* __restrict__ parts) {
+__global__ __launch_bounds__(256, (MT <= 2 ? 4 : 2)) void narrow_gram(MuonTensors t, int m, int64_t n, int tall, f64x4* __restrict__ parts) {
     constexpr int TILES = MT * (MT + 1) / 2;
     __shared__ float us[16 * MT * kStretchRow];
     __shared__ f64x4 red[3][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    narrow_load<MT, true>(us, t, blockIdx.y, m, n, tall != 0, (int64_t)blockIdx.x * kStretch);
+    narrow_load<MT, true>(us, t, blockIdx.y, NarrowRuns(m, n, tall != 0, (int64_t)blockIdx.x * kStretch));
     f64x4 acc[TILES];
 #pragma unroll
     for (int i = 0; i < TILES; i++) acc[i] = f64x4{0.0, 0.0, 0.0, 0.0};
@@ -180,26 +225,53 @@ __global__ __launch_bounds__(256) void narrow_gram(MuonTensors t, int m, int64_t
     }
 }
 
-// D = alpha A B + beta C + gamma I of [16 MT]^2 float64 matrices in LDS (rows ROW apart), A symmetric and all of them polynomials of one
-// matrix; tiles over the workgroup's 16 waves. C may be NULL or any of the others but D.
-template <int MT, int ROW>
-__device__ __forceinline__ void narrow_product(const double* A, const double* B, const double* C, double* D, double alpha, double beta,
-                                               double gamma) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (wave < MT * MT) {
-        const int i0 = wave / MT * 16, j0 = wave % MT * 16, c = lane & 15, q = lane >> 4;
-        f64x4 acc = {0.0, 0.0, 0.0, 0.0};
-        for (int k = 0; k < 16 * MT; k += 4)                       // (A's column k is its row k)
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64(A[(k + q) * ROW + i0 + c], B[(k + q) * ROW + j0 + c], acc, 0, 0, 0);
+// D = alpha A B + beta C + gamma I of [16 MT]^2 float64 matrices in LDS (rows ROW apart), all of them polynomials of one symmetric matrix:
+// they commute and are symmetric, so the tiles on and below the diagonal are computed and stored twice. C may be NULL; D may be any of
+// them: everything is read before anything is written. The jobs' tiles go over the workgroup's 16 waves.
+struct NarrowJob {
+    const double *A, *B, *C;
+    double* D;
+    double alpha, beta, gamma;
+};
+template <int MT, int ROW, int JOBS>
+__device__ __forceinline__ void narrow_products(const NarrowJob (&jobs)[JOBS]) {
+    constexpr int TILES = MT * (MT + 1) / 2, EACH = (TILES * JOBS + 15) / 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    f64x4 d[EACH];
+    auto each = [&](auto&& f) {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int job = wave + 16 * e, tile = job % TILES;
+            if (job >= TILES * JOBS) continue;
+            int ti = 0;
+            while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
+            f(jobs[JOBS > 1 && job >= TILES ? JOBS - 1 : 0], d[e], 16 * ti, 16 * (tile - ti * (ti + 1) / 2));
+        }
+    };
+    each([&](const NarrowJob& q, f64x4& d, int i0, int j0) {
+        f64x4 acc[2] = {};                                         // (two chains: each product waits for the one before)
+#pragma unroll
+        for (int k = 0; k < 4 * MT; k++) {                         // (A's column k is its row k)
+            const int at = (4 * k + g) * ROW + c;
+            acc[k & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64(q.A[at + i0], q.B[at + j0], acc[k & 1], 0, 0, 0);
+        }
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-            const int at = (i0 + 4 * v + q) * ROW + j0 + c;
-            double d = alpha * acc[v];
-            if (C) d += beta * C[at];
-            if (i0 + 4 * v + q == j0 + c) d += gamma;
-            D[at] = d;
+            const int r = i0 + 4 * v + g, s = j0 + c;
+            d[v] = q.alpha * (acc[0][v] + acc[1][v]);
+            if (q.C) d[v] += q.beta * q.C[r * ROW + s];
+            if (r == s) d[v] += q.gamma;
         }
-    }
+    });
+    __syncthreads();
+    each([&](const NarrowJob& q, f64x4& d, int i0, int j0) {
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const int r = i0 + 4 * v + g, s = j0 + c;
+            q.D[r * ROW + s] = d[v];
+            if (i0 != j0) q.D[s * ROW + r] = d[v];
+        }
+    });
     __syncthreads();
 }
 
@@ -212,9 +284,7 @@ struct MuonSteps {
 template <int MT>
 __global__ __launch_bounds__(1024) void narrow_steps(const f64x4* __restrict__ parts, int stretches, MuonSteps s, double* __restrict__ out) {
     constexpr int TILES = MT * (MT + 1) / 2, M = 16 * MT, ROW = M + 2;      // (two rows' lanes then lie in different banks)
-    __shared__ double buf[4][M * ROW];
-    __shared__ double trace;
-    double *A = buf[0], *Q = buf[1], *P = buf[2], *T = buf[3];
+    __shared__ double A[M * ROW], Q[M * ROW], P[M * ROW], trace;
     const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int tile = wave; tile < TILES; tile += 16) {
         f64x4 g = {0.0, 0.0, 0.0, 0.0};
@@ -246,34 +316,32 @@ __global__ __launch_bounds__(1024) void narrow_steps(const f64x4* __restrict__ p
     }
     __syncthreads();
     for (int k = 0; k < s.steps; k++) {
-        narrow_product<MT, ROW>(A, A, A, Q, s.c, s.b, s.a);        // Q = a + b A + c A^2
-        narrow_product<MT, ROW>(Q, P, nullptr, T, 1.0, 0.0, 0.0);  // P = Q P
-        double* swap = P;
-        P = T;
-        T = swap;
-        if (k + 1 == s.steps) break;
-        narrow_product<MT, ROW>(Q, A, nullptr, T, 1.0, 0.0, 0.0);  // A = Q A Q
-        narrow_product<MT, ROW>(Q, T, nullptr, A, 1.0, 0.0, 0.0);
+        narrow_products<MT, ROW>({{A, A, A, Q, s.c, s.b, s.a}});   // Q = a + b A + c A^2
+        if (k + 1 == s.steps) {
+            narrow_products<MT, ROW>({{Q, P, nullptr, P, 1.0, 0.0, 0.0}});
+        } else {                                                   // P = Q P; A = Q A Q
+            narrow_products<MT, ROW>({{Q, P, nullptr, P, 1.0, 0.0, 0.0}, {Q, A, nullptr, A, 1.0, 0.0, 0.0}});
+            narrow_products<MT, ROW>({{Q, A, nullptr, A, 1.0, 0.0, 0.0}});
+        }
     }
     for (int i = threadIdx.x; i < M * M; i += 1024) out[(int64_t)b * M * M + i] = P[i / M * ROW + i % M];
 }
 
 // O = P u over a stretch, and the parameter's step: workgroup (stretch, matrix).
 template <int MT>
-__global__ __launch_bounds__(256) void narrow_apply(MuonTensors t, int m, int64_t n, int tall, const double* __restrict__ parts) {
+__global__ __launch_bounds__(256, (MT <= 2 ? 4 : 2)) void narrow_apply(MuonTensors t, int m, int64_t n, int tall, const double* __restrict__ parts) {
     constexpr int M = 16 * MT;
     __shared__ float us[M * kStretchRow];
     const int b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, q = lane >> 4;
-    const int64_t k0 = (int64_t)blockIdx.x * kStretch;
-    const int len = (int)min<int64_t>(kStretch, n - k0);
     double p[MT][4 * MT];                                          // P's operands: P is symmetric, so row 16 i + c is column
     const double* pp = parts + (int64_t)b * M * M;
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int k = 0; k < 4 * MT; k++) p[i][k] = pp[(4 * k + q) * M + 16 * i + c];
-    narrow_load<MT, false>(us, t, b, m, n, tall != 0, k0);
+    const NarrowRuns runs(m, n, tall != 0, (int64_t)blockIdx.x * kStretch);
+    narrow_load<MT, false>(us, t, b, runs);
     // a wave's 64 columns, 16 at a time; its outputs take their place (no other wave reads them)
 #pragma unroll 1
     for (int j = wave * 64; j < wave * 64 + 64; j += 16) {
@@ -293,27 +361,24 @@ __global__ __launch_bounds__(256) void narrow_apply(MuonTensors t, int m, int64_
             for (int v = 0; v < 4; v++) us[(16 * i + 4 * v + q) * kStretchRow + j + c] = (float)acc[i][v];
     }
     __syncthreads();
-    if (tall) {
-        const int64_t first = k0 * m;
-        const int size = len * m;
-        for (int i = threadIdx.x * 8; i < size; i += 2048) {
-            float v[8];
-            int k = i / m, r = i - k * m;
+    for (int i = threadIdx.x; i < runs.runs; i += 256 * kRunsAhead) {
+        float old[kRunsAhead][8];
 #pragma unroll
-            for (int x = 0; x < 8; x++) {
-                v[x] = i + x < size ? us[r * kStretchRow + k] : 0.0f;
-                if (++r == m) r = 0, k++;
-            }
-            muon_apply(t, b, first + i, v, size - i);
+        for (int h = 0; h < kRunsAhead; h++) {
+            int64_t offset;
+            int r, k;
+            const int cnt = runs.at(i + 256 * h, offset, r, k);
+            if (cnt > 0 && t.keep != 0.0f) load_params<8>(old[h], t.p[b], offset, cnt, t.dt);
         }
-    } else {
-        for (int i = threadIdx.x; i < m * (kStretch / 8); i += 256) {
-            const int r = i / (kStretch / 8), k = i % (kStretch / 8) * 8;
-            if (k >= len) continue;
-            float v[8];
 #pragma unroll
-            for (int x = 0; x < 8; x++) v[x] = us[r * kStretchRow + k + x];
-            muon_apply(t, b, r * n + k0 + k, v, len - k);
+        for (int h = 0; h < kRunsAhead; h++) {
+            int64_t offset;
+            int r, k;
+            const int cnt = runs.at(i + 256 * h, offset, r, k);
+            if (cnt <= 0) continue;
+            float v[8];
+            runs.places(r, k, [&](int x, int place) { v[x] = x < cnt ? us[place] : 0.0f; });
+            muon_store(t, b, offset, old[h], v, cnt);
         }
     }
 }
@@ -336,7 +401,7 @@ static MuonPlan muon_plan(int64_t rows, int64_t cols, int64_t count) {
     p.narrow = side <= kNarrow;
     if (p.narrow) {
         p.batch = (int)std::min<int64_t>(count, kMuonBatch);
-        p.mt = side <= 16 ? 1 : side <= 32 ? 2 : 4;
+        p.mt = (int)(side + 15) / 16;
         p.stretches = (int)((n + kStretch - 1) / kStretch);
         p.sums_at = up_to((int64_t)p.batch * p.stretches * p.mt * (p.mt + 1) / 2 * 64 * 32, 256);
         p.bytes = p.sums_at + (int64_t)p.batch * 256 * p.mt * p.mt * 8;
@@ -380,6 +445,7 @@ static void muon_narrow(const MuonPlan& p, int batch, int64_t rows, int64_t cols
     };
     if (p.mt == 1) go(std::integral_constant<int, 1>{});
     else if (p.mt == 2) go(std::integral_constant<int, 2>{});
+    else if (p.mt == 3) go(std::integral_constant<int, 3>{});
     else go(std::integral_constant<int, 4>{});
 }
 

@@ -209,27 +209,30 @@ __global__ __launch_bounds__(S::NT, (MuonLoop<S, false, BX>::WAVES)) void muon_u
             n = nw + 8 * (p % (TC / 8));
             return m < rows && n < (q.next ? ld : cols);
         };
-        Pack<WF_F16> x[U], r[U];
+        Pack<WF_F16> x[U], r[U];                                   // of X and its remainder, or of the parameter (float32: both)
         auto fetch = [&](int it) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 int m, n;
                 x[u].zero();
                 r[u].zero();
-                if (at(it + u, m, n)) {
+                if (!at(it + u, m, n)) continue;
+                if (q.next) {
                     x[u].load(q.x + b * x_step + (int64_t)m * ld + n, 8);
                     r[u].load(q.lo + b * x_step + (int64_t)m * ld + n, 8);
+                } else if (t.keep != 0.0f) {
+                    muon_raw(t, b, (int64_t)m * cols + n, cols - n, x[u], r[u]);
                 }
             }
         };
-        if (q.lo) fetch(0);
+        fetch(0);
         Stage::template put<P>(st, acc, lane);
 #pragma unroll 1
         for (int it = 0; it < RUNS; it += U) {
             Pack<WF_F16> xc[U], rc[U];
 #pragma unroll
             for (int u = 0; u < U; u++) xc[u] = x[u], rc[u] = r[u];
-            if (q.lo && it + U < RUNS) fetch(it + U);
+            if (it + U < RUNS) fetch(it + U);
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 int m, n;
@@ -239,23 +242,22 @@ __global__ __launch_bounds__(S::NT, (MuonLoop<S, false, BX>::WAVES)) void muon_u
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[i] *= q.alpha;
                 const int64_t to = b * x_step + (int64_t)m * ld + n;
-                if (q.lo)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = fmaf(q.a, fmaf(rc[u].get(i), 1.0f / 2048.0f, xc[u].get(i)), v[i]);
                 if (!q.next) {
-                    muon_apply(t, b, (int64_t)m * cols + n, v, cols - n);
+                    float old[8];
+                    muon_values(t, xc[u], rc[u], old);
+                    muon_store(t, b, (int64_t)m * cols + n, old, v, cols - n);
                     continue;
                 }
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = fmaf(q.a, fmaf(rc[u].get(i), 1.0f / 2048.0f, xc[u].get(i)), v[i]);
                 Pack<WF_F16> o;
                 o.put(v);
                 o.store(q.next + to, 8);
-                if (q.lo) {
-                    float w[8];
+                float w[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) w[i] = (v[i] - o.get(i)) * 2048.0f;
-                    o.put(w);
-                    o.store(q.lo + to, 8);
-                }
+                for (int i = 0; i < 8; i++) w[i] = (v[i] - o.get(i)) * 2048.0f;
+                o.put(w);
+                o.store(q.lo + to, 8);
             }
         }
     });
