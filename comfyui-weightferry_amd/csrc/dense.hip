@@ -108,15 +108,16 @@ constexpr DenseTiling kDense[] = {{256, 320, 1, 2.2f, 1.65f, 1.65f},    {256, 25
                                   {128, 160, 2, 1.6f, 0.72f, 0.606f},   {128, 128, 2, 1.5f, 0.634f, 0.519f},
                                   {64, 128, 3, 0.8f, 0.47f, 0.367f},    {32, 128, 3, 1.6f, 0.435f, 0.315f}};
 
-// What an epilogue adds to a workgroup's time. Eight waves hide more of it than four, and workgroups that share a CU hide each other's: 4096 x 13824 x 5120 with
-// GELU 465 us in 256 x 320 tiles, 486 in 256 x 256, which without it are as fast.
+// What an epilogue adds to a workgroup's time. Eight waves hide more of it than four, and workgroups that share a CU hide each
+// other's: 4096 x 13824 x 5120 with GELU 465 us in 256 x 320 tiles, 486 in 256 x 256, which without it are as fast.
 static float dense_epilogue_time(const DenseTiling& q, int epilogue) {
     const float us = (epilogue & EPI_ACT ? 5.0f : 0.0f) + (epilogue & EPI_KEEP ? 10.0f : 0.0f) +
                      (epilogue & EPI_MORE ? 8.0f : 0.0f);
     return us * (float)(q.bm * q.bn) / 65536.0f * (q.bn == 320 ? 0.5f : q.per_cu > 1 ? 0.75f : 1.0f);
 }
 
-DensePlan dense_plan_tiles(const DenseTiling* tilings, int count, int64_t M, int64_t N, int64_t K, int epilogue, float& us) {
+DensePlan dense_plan_tiles(const DenseTiling* tilings, int count, int64_t M, int64_t N, int64_t K, int epilogue, float sum_us,
+                           float& us) {
     const int64_t stages = (K + 63) / 64;
     DensePlan best = {0, 1, (int)stages};
     us = 1e30f;
@@ -141,7 +142,7 @@ DensePlan dense_plan_tiles(const DenseTiling* tilings, int count, int64_t M, int
             const float mem = bytes / 4.6e6f * (1.0f + 0.12f * 256.0f / (float)wgs);
             const float hi = std::max(busy, mem), r = std::min(busy, mem) / hi;
             float c = 4.4f + hi * (1.0f + 0.26f * r * r * r);
-            if (want > 1) c += 1.3f + 1.5e-6f * (float)(M * N) * (float)(slices + 1);
+            if (want > 1) c += sum_us + 1.5e-6f * (float)(M * N) * (float)(slices + 1);
             if (c < us) us = c, best = {t, (int)slices, (int)per};
         }
     }
@@ -192,7 +193,7 @@ DenseCall dense_call(const DenseView& x, const DenseView& w, int64_t M, int64_t 
     DenseCall d = {};
     d.epilogue = epilogue;
     float us;
-    d.tiles = dense_plan_tiles(kDense, (int)(sizeof(kDense) / sizeof(kDense[0])), M, N, K, epilogue, us);
+    d.tiles = dense_plan_tiles(kDense, (int)(sizeof(kDense) / sizeof(kDense[0])), M, N, K, epilogue, 1.3f, us);
     d.how_w = dense_how(w, N, K, true);
     d.how_x = dense_how(x, M, K, is_across(d.how_w));
     int64_t copies = dense_copy_bytes(d.how_x, M, K);

@@ -16,8 +16,10 @@ struct DenseTiling {
 
 // what an epilogue adds to it: an activation's arithmetic, the kept pre-activations' stores, the residual's loads
 enum { EPI_ACT = 1, EPI_KEEP = 2, EPI_MORE = 4 };
-// the tiling and slices of K that the model finds fastest, and its time in us
-DensePlan dense_plan_tiles(const DenseTiling* tilings, int count, int64_t M, int64_t N, int64_t K, int epilogue, float& us);
+// the tiling and slices of K that the model finds fastest, and its time in us; sum_us: of the second launch that slices need, besides
+// the time of its bytes
+DensePlan dense_plan_tiles(const DenseTiling* tilings, int count, int64_t M, int64_t N, int64_t K, int epilogue, float sum_us,
+                           float& us);
 // the few-rows form's
 float dense_rows_time(int64_t M, int64_t N, int64_t K, bool odd);
 
