@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "column_sums.h"
+#include "deep_ring.h"
 #include "dense_call.h"
 #include "grids.h"
 #include "tile_stage.h"
@@ -24,13 +25,13 @@
 namespace wf {
 
 // a, b: x and the weight's first half, along K; half: values from a row of the first half to the same of the second. Workgroup
-// (tile, slice); parts: [slices, M, 2 N] float32 partial sums, or NULL: one slice, and the outputs.
-template <int D, typename S>
-__global__ __launch_bounds__(S::NT, S::WAVES) void gated_gemm(DenseOperand a, DenseOperand b, int64_t half, int M, int N, int K,
+// (tile, slice); parts: [slices, M, 2 N] float32 partial sums, or NULL: one slice, and the outputs. DEEP: four stage buffers.
+template <int D, typename S, bool DEEP>
+__global__ __launch_bounds__(S::NT, (DEEP ? 1 : S::WAVES)) void gated_gemm(DenseOperand a, DenseOperand b, int64_t half, int M, int N, int K,
                                                               int slice_stages, float* __restrict__ parts, GatedEpilogue e) {
     constexpr int WM = S::WM, WN = S::WN, TC = WN * 16, BO = S::BN / 2;    // outputs of a wave's row, of a tile's
     static_assert(WN % 2 == 0, "a fragment of each half");
-    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS];
+    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS], sb2[DEEP ? S::SLOTS : 1], sb3[DEEP ? S::SLOTS : 1];
     const int ntm = (M + S::BM - 1) / S::BM, ntn = (N + BO - 1) / BO;
     int tm, tn;
     tile_order(blockIdx.x, ntm * ntn, ntm, ntn, tm, tn);
@@ -54,8 +55,15 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void gated_gemm(DenseOperand a, De
 #pragma unroll
             for (int x = 0; x < 16; x++) acc[i][j][x] = bn;
     }
-    dense_loop<S, DenseAlong<S::BM, S::NW, S::AW, WM>, DenseAlongPair<S::BN, S::NW, S::BW, WN>>(
-        ta, tb, s0, nk, wave, lane, sb0, sb1, acc, [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<D>(c, x, y); });
+    using LA = DenseAlong<S::BM, S::NW, S::AW, WM>;
+    using LB = DenseAlongPair<S::BN, S::NW, S::BW, WN>;
+    auto mma = [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<D>(c, x, y); };
+    if constexpr (DEEP) {
+        wl_frag* const sb[kDeep] = {sb0, sb1, sb2, sb3};
+        deep_loop<S, LA, LB>(ta, tb, s0, nk, wave, lane, sb, acc, mma);
+    } else {
+        dense_loop<S, LA, LB>(ta, tb, s0, nk, wave, lane, sb0, sb1, acc, mma);
+    }
     if (parts) {                                                   // (32 lanes store 128 bytes of a row)
         float* o = parts + (int64_t)blockIdx.y * M * 2 * N;
 #pragma unroll
@@ -186,27 +194,31 @@ __global__ __launch_bounds__(256) void gated_dact(const value_t<D>* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------------- host side
-// Rows of x and of the weight (both halves) a tile, and its times, chosen so that the model picks well among 330 measured launches (20
-// shapes of 40-16384 rows, 1000-13824 outputs and K 512-8192, with and without the halves kept): what it takes is 2.3 % longer than
-// the best on average, at most 14 % (77 x 2608 x 1536 and 64 x 1024 x 1024, 15.6 and 10.5 us). 64 x 256 tiles were nowhere the best
-// by more than 8 %. us at 4096 x 13824 x 5120 in these tilings: 874 / 1232 / 1113 / 2666; 512 x 8192 x 2048 45 / 33.5 / 34.6 / 57; 300 x
-// 1000 x 1024 (one slice) 9.6 in the third, 8.9 in the last.
-constexpr DenseTiling kGated[] = {{256, 256, 1, 6.6f, 1.30f, 1.30f}, {128, 256, 1, 3.2f, 0.83f, 0.83f},
-                                  {128, 128, 2, 1.15f, 0.452f, 0.546f}, {32, 256, 2, 0.85f, 0.54f, 0.65f}};
+// Rows of x and of the weight (both halves) a tile, and its times, chosen so that the model picks well among 380 measured launches (20
+// shapes of 40-16384 rows, 1000-13824 outputs and K 512-8192, weights not in the caches, with and without the halves kept): what it takes
+// is 2 % longer than the best on average. Where a tile has a CU to itself a ring of four stages waits less than two buffers: us in 128
+// x 128 tiles, two buffers / four, 128 x 13824 x 5120 79.5 / 70.5, 700 x 2048 x 5120 43.7 (two slices) / 40.2, 77 x 2608 x 1536 16.9 /
+// 15.2; 512 x 8192 x 2048, two tiles a CU, 38.6 / 43.6. 4096 x 13824 x 5120 in these tilings: 827 / 1244 / 1092 / 1273 / 2669.
+constexpr DenseTiling kGated[] = {{256, 256, 1, 6.1f, 1.09f, 1.09f}, {128, 256, 1, 3.0f, 0.70f, 0.70f},
+                                  {128, 128, 2, 0.4f, 0.60f, 0.56f}, {128, 128, 1, 0.8f, 0.432f, 0.432f},
+                                  {32, 256, 1, 1.3f, 0.426f, 0.426f}};
 
 template <int D>
 static void gated_tiling(const DenseOperand& a, const DenseOperand& b, int64_t half, int M, int N, int K, const DensePlan& p,
                          float* parts, const GatedEpilogue& e, hipStream_t s) {
-    auto go = [&](auto shape) {
+    auto go = [&](auto shape, auto deep) {
         using S = decltype(shape);
         const int tiles = ((M + S::BM - 1) / S::BM) * ((N + S::BN / 2 - 1) / (S::BN / 2));
-        gated_gemm<D, S><<<dim3(tiles, p.slices), S::NT, 0, s>>>(a, b, half, M, N, K, p.slice_stages, parts, e);
+        gated_gemm<D, S, decltype(deep)::value><<<dim3(tiles, p.slices), S::NT, 0, s>>>(a, b, half, M, N, K, p.slice_stages, parts, e);
     };
+    const std::false_type two{};
+    const std::true_type four{};
     switch (p.tiling) {
-    case 0: go(DenseShape<2, 2, 4, 4>{}); break;
-    case 1: go(DenseShape<2, 2, 2, 4>{}); break;
-    case 2: go(DenseShape<2, 2, 2, 2>{}); break;
-    default: go(DenseShape<1, 4, 1, 2>{}); break;
+    case 0: go(DenseShape<2, 2, 4, 4>{}, two); break;
+    case 1: go(DenseShape<2, 2, 2, 4>{}, two); break;
+    case 2: go(DenseShape<2, 2, 2, 2>{}, two); break;
+    case 3: go(DenseShape<2, 2, 2, 2>{}, four); break;
+    default: go(DenseShape<1, 4, 1, 2>{}, four); break;
     }
 }
 

@@ -79,6 +79,7 @@ SHAPES = [
     (280, 5, 5760), (512, 1280, 1280), (1023, 1537, 513), (1560, 1024, 1024), (2049, 2056, 200), (4096, 2560, 320),
     (5000, 333, 96), (536, 524, 4736), (803, 3008, 455), (3880, 1560, 576), (1096, 1903, 6264), (6080, 4, 400), (8224, 165, 2),
     (256, 2560, 5120), (1881, 3424, 736), (1419, 1655, 896), (1392, 1536, 5376), (904, 1135, 7552), (262, 6, 1152), (512, 16, 928),
+    (2112, 1824, 648), (104, 1265, 3264), (3640, 1, 2934), (2225, 1295, 1744), (104, 1791, 2448), (8640, 1, 1152), (2113, 1824, 648),
     (1984, 3200, 1302), (2048, 1040, 1814), (1420, 1656, 900), (1900, 3420, 737), (905, 1136, 7553), (1393, 1537, 5376), (263, 7, 1153), (513, 17, 928)]
 
 

@@ -274,3 +274,21 @@ def test_refused_steps_change_nothing(native):
     with pytest.raises(ValueError):
         fm.Muon([torch.nn.Parameter(vector)])
     fm.muon_step([], [], [])
+
+
+def test_the_largest_shorter_side(native):
+    # 16384 x 16384: the powers of two that keep X and its products in float16's range are at their largest
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = matrix(16384, 16384, "falling", g).bfloat16()
+    x[:, 0] *= 40                                               # one column, and so one entry of X^T X, far above the others
+    got = fm.orthogonalize(x)
+    assert got.isfinite().all()
+    sv = torch.linalg.svdvals(got[:, :64].double())
+    # 64 of the columns of a matrix whose singular values all lie below 1.21 (the polynomial's largest, plus 1 % for the roundings)
+    assert float(sv[0]) < 1.22
+    a, b, c = ABC
+    want = x.float() / x.float().norm()
+    for _ in range(5):                                          # float32 products: 2^-24 against 2^-11
+        s = want @ want.T
+        want = a * want + (b * s + c * (s @ s)) @ want
+    assert float((got.float() - want).norm() / want.norm()) < 5e-3
