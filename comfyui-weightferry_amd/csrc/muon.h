@@ -18,51 +18,6 @@ struct MuonTensors {
     int nesterov;
 };
 
-// 8 places of a parameter from `at` on, the first cnt of them: keep old - rate v (keep 0: old is not looked at)
-__device__ __forceinline__ void muon_store(const MuonTensors& t, int b, int64_t at, const float (&old)[8], const float (&v)[8], int cnt) {
-    float w[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) w[i] = fmaf(-t.rate, v[i], t.keep != 0.0f ? t.keep * old[i] : 0.0f);
-    if (t.dt == WF_F32) {
-        float* p = static_cast<float*>(t.p[b]) + at;
-        if (cnt >= 8) __builtin_memcpy(p, w, 32);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i < cnt) p[i] = w[i];
-    } else if (t.dt == WF_BF16) {
-        Pack<WF_BF16> o;
-        o.put(w);
-        o.store(static_cast<uint16_t*>(t.p[b]) + at, cnt);
-    } else {
-        Pack<WF_F16> o;
-        o.put(w);
-        o.store(static_cast<uint16_t*>(t.p[b]) + at, cnt);
-    }
-}
-
-// 8 places of a parameter as they lie (float32: in two packs), and what they stand for
-__device__ __forceinline__ void muon_raw(const MuonTensors& t, int b, int64_t at, int cnt, Pack<WF_F16>& lo, Pack<WF_F16>& hi) {
-    if (t.dt == WF_F32) {
-        const float* p = static_cast<const float*>(t.p[b]) + at;
-        Pack<WF_F32> a, c;
-        a.load(p, cnt);
-        c.zero();
-        if (cnt > 4) c.load(p + 4, cnt - 4);
-        __builtin_memcpy(lo.w, a.w, 16);
-        __builtin_memcpy(hi.w, c.w, 16);
-    } else {
-        lo.load(static_cast<const uint16_t*>(t.p[b]) + at, cnt);
-    }
-}
-__device__ __forceinline__ void muon_values(const MuonTensors& t, const Pack<WF_F16>& lo, const Pack<WF_F16>& hi, float (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t h = i & 1 ? lo.w[i / 2] >> 16 : lo.w[i / 2] & 0xffffu;
-        v[i] = t.dt == WF_F32 ? __uint_as_float(i < 4 ? lo.w[i] : hi.w[i - 4]) : t.dt == WF_BF16 ? __uint_as_float(h << 16) : f16_bits_to_f32(h);
-    }
-}
-
 // A batch in float16, matrix b at x + b (rows ld), X s with s a power of two; symmetric matrices [side, sld], times s^2; rows' lengths ld, sld are
 // multiples of 8, zeros past the matrix.
 struct MuonShape {

@@ -327,6 +327,29 @@ __global__ __launch_bounds__(1024) void narrow_steps(const f64x4* __restrict__ p
     for (int i = threadIdx.x; i < M * M; i += 1024) out[(int64_t)b * M * M + i] = P[i / M * ROW + i % M];
 }
 
+// 8 places of a parameter from `at` on, the first cnt of them: keep old - rate v (keep 0: old is not looked at)
+__device__ __forceinline__ void muon_store(const MuonTensors& t, int b, int64_t at, const float (&old)[8], const float (&v)[8], int cnt) {
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = fmaf(-t.rate, v[i], t.keep != 0.0f ? t.keep * old[i] : 0.0f);
+    if (t.dt == WF_F32) {
+        float* p = static_cast<float*>(t.p[b]) + at;
+        if (cnt >= 8) __builtin_memcpy(p, w, 32);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < cnt) p[i] = w[i];
+    } else if (t.dt == WF_BF16) {
+        Pack<WF_BF16> o;
+        o.put(w);
+        o.store(static_cast<uint16_t*>(t.p[b]) + at, cnt);
+    } else {
+        Pack<WF_F16> o;
+        o.put(w);
+        o.store(static_cast<uint16_t*>(t.p[b]) + at, cnt);
+    }
+}
+
 // O = P u over a stretch, and the parameter's step: workgroup (stretch, matrix).
 template <int MT>
 __global__ __launch_bounds__(256, (MT <= 2 ? 4 : 2)) void narrow_apply(MuonTensors t, int m, int64_t n, int tall, const double* __restrict__ parts) {

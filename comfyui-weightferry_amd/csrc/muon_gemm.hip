@@ -198,69 +198,102 @@ __global__ __launch_bounds__(S::NT, (MuonLoop<S, false, BX>::WAVES)) void muon_u
         return;
     }
     constexpr int ROWS = Stage::ROWS, RUNS = ROWS * TC / 8 / 64, U = RUNS % 4 == 0 ? 4 : RUNS;
-    // U runs' loads in flight together
-    static_for<Stage::PHASES>([&](auto pc) {
-        constexpr int P = decltype(pc)::value;
-        const int mp = mw + P * ROWS;
-        if (mp >= rows) return;
-        auto at = [&](int it, int& m, int& n) {
-            const int p = it * 64 + lane;
-            m = mp + p / (TC / 8);
-            n = nw + 8 * (p % (TC / 8));
-            return m < rows && n < (q.next ? ld : cols);
-        };
-        Pack<WF_F16> x[U], r[U];                                   // of X and its remainder, or of the parameter (float32: both)
-        auto fetch = [&](int it) {
+    // The tile's runs of 8 outputs: what load(ahead, m, n) fetches for U of them goes out before the U before are finished by
+    // store(v, ahead, m, n), v the sums. width: the columns that are walked.
+    auto walk = [&](auto ahead, int width, auto&& load, auto&& store) {
+        using Ahead = decltype(ahead);
+        static_for<Stage::PHASES>([&](auto pc) {
+            constexpr int P = decltype(pc)::value;
+            const int mp = mw + P * ROWS;
+            if (mp >= rows) return;
+            Ahead next[U];
+            auto at = [&](int it, int& m, int& n) {
+                const int p = it * 64 + lane;
+                m = mp + p / (TC / 8);
+                n = nw + 8 * (p % (TC / 8));
+                return m < rows && n < width;
+            };
+            auto fetch = [&](int it) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                int m, n;
-                x[u].zero();
-                r[u].zero();
-                if (!at(it + u, m, n)) continue;
-                if (q.next) {
-                    x[u].load(q.x + b * x_step + (int64_t)m * ld + n, 8);
-                    r[u].load(q.lo + b * x_step + (int64_t)m * ld + n, 8);
-                } else if (t.keep != 0.0f) {
-                    muon_raw(t, b, (int64_t)m * cols + n, cols - n, x[u], r[u]);
+                for (int u = 0; u < U; u++) {
+                    int m, n;
+                    if (at(it + u, m, n)) load(next[u], m, n);
+                }
+            };
+            fetch(0);
+            Stage::template put<P>(st, acc, lane);
+#pragma unroll 1
+            for (int it = 0; it < RUNS; it += U) {
+                Ahead now[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) now[u] = next[u];
+                if (it + U < RUNS) fetch(it + U);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    int m, n;
+                    if (!at(it + u, m, n)) continue;
+                    float v[8];
+                    staged_run(v, st + ((it + u) * 64 + lane) * 8);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] *= q.alpha;
+                    store(v, now[u], m, n);
                 }
             }
-        };
-        fetch(0);
-        Stage::template put<P>(st, acc, lane);
-#pragma unroll 1
-        for (int it = 0; it < RUNS; it += U) {
-            Pack<WF_F16> xc[U], rc[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) xc[u] = x[u], rc[u] = r[u];
-            if (it + U < RUNS) fetch(it + U);
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                int m, n;
-                if (!at(it + u, m, n)) continue;
-                float v[8];
-                staged_run(v, st + ((it + u) * 64 + lane) * 8);
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] *= q.alpha;
+        });
+    };
+    if (q.next) {                                                  // a x from X and its remainder, the new remainder beside
+        struct Both { Pack<WF_F16> x, r; };
+        walk(
+            Both{}, ld,
+            [&](Both& f, int m, int n) {
+                f.x.load(q.x + b * x_step + (int64_t)m * ld + n, 8);
+                f.r.load(q.lo + b * x_step + (int64_t)m * ld + n, 8);
+            },
+            [&](float (&v)[8], const Both& f, int m, int n) {
                 const int64_t to = b * x_step + (int64_t)m * ld + n;
-                if (!q.next) {
-                    float old[8];
-                    muon_values(t, xc[u], rc[u], old);
-                    muon_store(t, b, (int64_t)m * cols + n, old, v, cols - n);
-                    continue;
-                }
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = fmaf(q.a, fmaf(rc[u].get(i), 1.0f / 2048.0f, xc[u].get(i)), v[i]);
+                for (int i = 0; i < 8; i++) v[i] = fmaf(q.a, fmaf(f.r.get(i), 1.0f / 2048.0f, f.x.get(i)), v[i]);
                 Pack<WF_F16> o;
                 o.put(v);
                 o.store(q.next + to, 8);
-                float w[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = (v[i] - o.get(i)) * 2048.0f;
-                o.put(w);
+                for (int i = 0; i < 8; i++) v[i] = (v[i] - o.get(i)) * 2048.0f;
+                o.put(v);
                 o.store(q.lo + to, 8);
-            }
-        }
-    });
+            });
+        return;
+    }
+    auto step = [&](auto dt) {                                     // the parameter's step
+        constexpr int D = decltype(dt)::value, VEC = Pack<D>::VEC;
+        struct Old { Pack<D> p[8 / VEC]; };
+        value_t<D>* const p = static_cast<value_t<D>*>(t.p[b]);
+        walk(
+            Old{}, cols,
+            [&](Old& f, int m, int n) {
+                if (t.keep == 0.0f) return;
+#pragma unroll
+                for (int h = 0; h < 8 / VEC; h++) {
+                    f.p[h].zero();
+                    if (h == 0 || cols - n > h * VEC) f.p[h].load(p + (int64_t)m * cols + n + h * VEC, cols - n - h * VEC);
+                }
+            },
+            [&](float (&v)[8], const Old& f, int m, int n) {
+#pragma unroll
+                for (int h = 0; h < 8 / VEC; h++) {
+                    if (h && cols - n <= h * VEC) break;
+                    float w[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; i++)
+                        w[i] = fmaf(-t.rate, v[h * VEC + i], t.keep != 0.0f ? t.keep * f.p[h].get(i) : 0.0f);
+                    Pack<D> o;
+                    o.put(w);
+                    o.store(p + (int64_t)m * cols + n + h * VEC, cols - n - h * VEC);
+                }
+            });
+    };
+    if (t.dt == WF_BF16) step(std::integral_constant<int, WF_BF16>{});
+    else if (t.dt == WF_F16) step(std::integral_constant<int, WF_F16>{});
+    else step(std::integral_constant<int, WF_F32>{});
 }
 
 // ------------------------------------------------------------------------------------------------- host side
