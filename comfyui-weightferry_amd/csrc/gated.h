@@ -4,7 +4,7 @@
 // They are kept in 24 bits, float32 without its last 8, in three planes of 16: the upper 16 bits of g, those of u, and both
 // lower 8. The gradients of both are products of both (dg = dy u act'(g), du = dy act(g)), so 16 bits each would put three more
 // roundings of bfloat16 into dx and dw beside the two that the matrix instructions and the outputs need: 3e-3 of their norm instead of
-// 2.4e-3, at 4 bytes a pair against 6.
+// 2.3e-3, at 4 bytes a pair against 6.
 #pragma once
 
 #include "dense.h"

@@ -279,6 +279,8 @@ struct MuonSteps {
     int steps;
     double a, b, c, eps;
 };
+// (a norm of float32 values is zero or above 1e-45: a smaller eps means the same, and 1 / eps^2 has to be finite)
+static MuonSteps muon_steps(int steps, const double* abc, double eps) { return {steps, abc[0], abc[1], abc[2], std::max(eps, 1e-60)}; }
 
 // From the sums to P / max(|u|, eps): a workgroup a matrix. out: [batch, 16 MT, 16 MT].
 template <int MT>
@@ -587,7 +589,7 @@ extern "C" int wf_muon(const int64_t* table, int64_t count, int64_t rows, int64_
     t.mu = (float)momentum;
     t.nu = (float)(1.0 - momentum);
     t.nesterov = nesterov;
-    return muon_run("wf_muon", table, count, rows, cols, t, {steps, coefficients[0], coefficients[1], coefficients[2], eps}, workspace,
+    return muon_run("wf_muon", table, count, rows, cols, t, muon_steps(steps, coefficients, eps), workspace,
                     workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
@@ -599,6 +601,6 @@ extern "C" int wf_orthogonalize(const int64_t* table, int64_t count, int64_t row
     MuonTensors t = {};
     t.dt = dt;
     t.rate = -1.0f;
-    return muon_run("wf_orthogonalize", table, count, rows, cols, t, {steps, coefficients[0], coefficients[1], coefficients[2], eps},
+    return muon_run("wf_orthogonalize", table, count, rows, cols, t, muon_steps(steps, coefficients, eps),
                     workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }

@@ -125,9 +125,10 @@ def _ready(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, 
     code = CODES.get(dt)
     if code is None or dev.type != "cuda":
         raise ValueError(f"parameters of type {dt} on {dev}: float32, bfloat16 or float16 on a GPU")
-    if _capturing():
-        raise RuntimeError("a step cannot be captured into a graph: its rates and addresses are the call's, and a replay would "
-                           "repeat them")
+    with _native.on_device(dev):
+        if _capturing():
+            raise RuntimeError("a step cannot be captured into a graph: its rates and addresses are the call's, and a replay would "
+                               "repeat them")
     if not plain(dev):
         raise ValueError("a step inside a functorch transform or a trace, which would not see it")
     # (questions of all tensors at once: with hundreds of adapters they are the step's host time, a microsecond a matrix)
@@ -160,6 +161,8 @@ def _ready(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, 
     changed = at[:many] + at[2 * many:] if len(order) == many else [at[i + k] for i in order for k in (0, 2 * many)]
     if len(set(changed)) != len(changed):
         raise ValueError("a parameter or a momentum is there twice: each is stepped on its own")
+    if dt == torch.float32 and not {at[i + many] for i in order}.isdisjoint(at[i + 2 * many] for i in order):
+        raise ValueError("a gradient is a momentum's memory, which the step changes before it has read the gradient for the last time")
     table = array.array("q", bytes(24 * len(order)))
     for k in range(3):
         column = at[k * many:(k + 1) * many]
@@ -186,7 +189,7 @@ def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, wei
     momentum m + (1 - momentum) g, orthogonalised as by ``orthogonalize``; p = (1 - lr weight_decay) p - lr s update, s =
     sqrt(max(1, rows / cols)) ("spectral") or 0.2 sqrt(max(rows, cols)) ("rms": updates as large as AdamW's). ``params`` and ``grads``:
     contiguous GPU matrices of one type (float32, bfloat16 or float16); ``momenta``: contiguous, float32, as many values
-    (``muon_momenta``); all on one device, no parameter or momentum twice.
+    (``muon_momenta``); all on one device, no parameter or momentum twice, none sharing its memory with another tensor.
     ValueError for anything else. Asynchronous on torch's current stream; RuntimeError while that is captured into a graph."""
     _ready(list(params), list(grads), list(momenta), lr, momentum, nesterov, weight_decay, steps, coefficients, eps, adjust)()
 

@@ -276,6 +276,31 @@ def test_refused_steps_change_nothing(native):
     fm.muon_step([], [], [])
 
 
+def test_zeros_below_any_eps(native):
+    # 1 / eps^2 is infinite from 1e-155 down, and 0 times that no number
+    for rows, cols in ((40, 90), (90, 40), (200, 90), (1, 1)):
+        zeros = torch.zeros(rows, cols, device="cuda")
+        for eps in (1e-100, 1e-200, 5e-324):
+            assert torch.equal(fm.orthogonalize(zeros, eps=eps), zeros)
+        p, m = torch.ones_like(zeros), torch.zeros_like(zeros)
+        fm.muon_step([p], [zeros], [m], lr=0.5, weight_decay=0.5, eps=1e-200)
+        assert torch.equal(p, torch.full_like(p, 0.75)) and torch.equal(m, zeros)
+
+
+def test_a_gradient_in_a_momentums_memory(native):
+    p = [torch.randn(70, 80, device="cuda"), torch.randn(8, 9, device="cuda"), torch.randn(0, 9, device="cuda")]
+    g = [torch.randn_like(t) for t in p]
+    m = fm.muon_momenta(p)
+    kept = [t.clone() for t in p]
+    for momenta in ([m[0], g[1], m[2]], [g[0], m[1], g[2]]):
+        with pytest.raises(ValueError):
+            fm.muon_step(p, g, momenta)
+    assert all(torch.equal(a, b) for a, b in zip(kept, p))
+    fm.muon_step(p, [g[0], g[1], p[2]], m)                          # (nothing shares no memory, and one gradient may serve two)
+    q = [torch.randn(70, 80, device="cuda") for _ in range(2)]
+    fm.muon_step(q, [g[0], g[0]], fm.muon_momenta(q))
+
+
 def test_the_largest_shorter_side(native):
     # 16384 x 16384: the powers of two that keep X and its products in float16's range are at their largest
     g = torch.Generator(device="cuda").manual_seed(9)
