@@ -8,7 +8,8 @@
 // from the gate's half and from the other in turn, so that a wave's accumulators hold g and u of the same outputs: the epilogue
 // is arithmetic on registers, and neither g nor u goes to memory unless the backward pass will want them (gated.h has the format). A
 // product with too few tiles runs as slices of K, whose float32 sums a second kernel adds before the epilogue; few rows of x take
-// the form of dense_rows.hip with a tile of each half a workgroup.
+// the form of dense_rows.hip with a tile of each half a workgroup. Operands whose rows are no aligned 16-byte runs are copied into rows
+// that are, or, where that would cost more, loaded as they lie (loose_ring.h).
 //
 // Backward: one element-wise kernel from dy and the kept g and u to [dg du], [M, 2 N], rounded to the operands' type because it is the
 // operand of the two products behind it, which are the 16-bit linear's own on a weight of 2 N rows.
@@ -20,18 +21,21 @@
 #include "deep_ring.h"
 #include "dense_call.h"
 #include "grids.h"
+#include "loose_ring.h"
 #include "tile_stage.h"
 
 namespace wf {
 
 // a, b: x and the weight's first half, along K; half: values from a row of the first half to the same of the second. Workgroup
-// (tile, slice); parts: [slices, M, 2 N] float32 partial sums, or NULL: one slice, and the outputs. DEEP: four stage buffers.
-template <int D, typename S, bool DEEP>
-__global__ __launch_bounds__(S::NT, (DEEP ? 1 : S::WAVES)) void gated_gemm(DenseOperand a, DenseOperand b, int64_t half, int M, int N, int K,
+// (tile, slice); parts: [slices, M, 2 N] float32 partial sums, or NULL: one slice, and the outputs.
+enum { RING_TWO, RING_DEEP, RING_LOOSE };                          // two stage buffers, four, rows that start anywhere
+template <int D, typename S, int RING>
+__global__ __launch_bounds__(S::NT, (RING == RING_TWO ? S::WAVES : 1)) void gated_gemm(DenseOperand a, DenseOperand b, int64_t half, int M, int N, int K,
                                                               int slice_stages, float* __restrict__ parts, GatedEpilogue e) {
     constexpr int WM = S::WM, WN = S::WN, TC = WN * 16, BO = S::BN / 2;    // outputs of a wave's row, of a tile's
     static_assert(WN % 2 == 0, "a fragment of each half");
-    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS], sb2[DEEP ? S::SLOTS : 1], sb3[DEEP ? S::SLOTS : 1];
+    constexpr int MORE = RING == RING_DEEP ? S::SLOTS : 1;
+    __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS], sb2[MORE], sb3[MORE];
     const int ntm = (M + S::BM - 1) / S::BM, ntn = (N + BO - 1) / BO;
     int tm, tn;
     tile_order(blockIdx.x, ntm * ntn, ntm, ntn, tm, tn);
@@ -39,9 +43,6 @@ __global__ __launch_bounds__(S::NT, (DEEP ? 1 : S::WAVES)) void gated_gemm(Dense
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int stages = (K + 63) / 64, s0 = blockIdx.y * slice_stages, nk = min(slice_stages, stages - s0);
-    const DenseTile ta = dense_tile<false>(a, m0), tg = dense_tile<false>(b, n0);
-    b.p += half;
-    const DensePair tb = {{tg.r, dense_tile<false>(b, n0).r}, tg.row, tg.k};
     const int mw = m0 + wave / S::VN * WM * 32, nw = n0 + wave % S::VN * TC;
     const int lr = lane & 31, lk = lane >> 5;
     // the sums start from the bias
@@ -55,14 +56,24 @@ __global__ __launch_bounds__(S::NT, (DEEP ? 1 : S::WAVES)) void gated_gemm(Dense
 #pragma unroll
             for (int x = 0; x < 16; x++) acc[i][j][x] = bn;
     }
-    using LA = DenseAlong<S::BM, S::NW, S::AW, WM>;
-    using LB = DenseAlongPair<S::BN, S::NW, S::BW, WN>;
     auto mma = [](const f32x16v& c, const wl_frag& x, const wl_frag& y) { return mma16<D>(c, x, y); };
-    if constexpr (DEEP) {
-        wl_frag* const sb[kDeep] = {sb0, sb1, sb2, sb3};
-        deep_loop<S, LA, LB>(ta, tb, s0, nk, wave, lane, sb, acc, mma);
+    if constexpr (RING == RING_LOOSE) {
+        const uint16_t* w = b.p + n0 * b.row;
+        const LooseTile ta = {a.p + m0 * a.row, (uint32_t)a.row, M - m0, K};
+        const LoosePair tb = {{w, w + half}, (uint32_t)b.row, N - n0, K};
+        loose_loop<S, LooseAlong<S::NW, S::AW>, LooseAlongPair<S::NW, S::BW>>(ta, tb, s0, nk, wave, lane, sb0, sb1, acc, mma);
     } else {
-        dense_loop<S, LA, LB>(ta, tb, s0, nk, wave, lane, sb0, sb1, acc, mma);
+        using LA = DenseAlong<S::BM, S::NW, S::AW, WM>;
+        using LB = DenseAlongPair<S::BN, S::NW, S::BW, WN>;
+        const DenseTile ta = dense_tile<false>(a, m0), tg = dense_tile<false>(b, n0);
+        b.p += half;
+        const DensePair tb = {{tg.r, dense_tile<false>(b, n0).r}, tg.row, tg.k};
+        if constexpr (RING == RING_DEEP) {
+            wl_frag* const sb[kDeep] = {sb0, sb1, sb2, sb3};
+            deep_loop<S, LA, LB>(ta, tb, s0, nk, wave, lane, sb, acc, mma);
+        } else {
+            dense_loop<S, LA, LB>(ta, tb, s0, nk, wave, lane, sb0, sb1, acc, mma);
+        }
     }
     if (parts) {                                                   // (32 lanes store 128 bytes of a row)
         float* o = parts + (int64_t)blockIdx.y * M * 2 * N;
@@ -202,17 +213,28 @@ __global__ __launch_bounds__(256) void gated_dact(const value_t<D>* __restrict__
 constexpr DenseTiling kGated[] = {{256, 256, 1, 6.1f, 1.09f, 1.09f}, {128, 256, 1, 3.0f, 0.70f, 0.70f},
                                   {128, 128, 2, 0.4f, 0.60f, 0.56f}, {128, 128, 1, 0.8f, 0.432f, 0.432f},
                                   {32, 256, 1, 1.3f, 0.426f, 0.426f}};
+// The same for rows that start anywhere: us with copies of both operands and the tilings above (or few rows) / as they lie, of 22 shapes:
+// 77 x 2607 x 1531 28 / 19.7, 300 x 1000 x 1025 22.9 / 14.6, 40 x 8191 x 2047 50 / 28, 1 x 13823 x 5119 138 / 67, 2000 x 2047 x 333 22.8 / 19.3;
+// but 128 x 5121 x 5119 74 / 76, 700 x 2047 x 2559 38.4 / 40.6: odd places halve the loads' rate, and long sums pay for that more than
+// once a copy. The way the model chooses among the two and their slices takes 3 % longer than the best on average.
+constexpr DenseTiling kLooseTiles[] = {{128, 128, 2, 2.5f, 0.863f, 0.979f}, {64, 128, 3, 1.3f, 0.556f, 0.67f}};
 
 template <int D>
-static void gated_tiling(const DenseOperand& a, const DenseOperand& b, int64_t half, int M, int N, int K, const DensePlan& p,
+static void gated_tiling(const DenseOperand& a, const DenseOperand& b, int64_t half, int M, int N, int K, const DensePlan& p, bool loose,
                          float* parts, const GatedEpilogue& e, hipStream_t s) {
-    auto go = [&](auto shape, auto deep) {
+    auto go = [&](auto shape, auto ring) {
         using S = decltype(shape);
         const int tiles = ((M + S::BM - 1) / S::BM) * ((N + S::BN / 2 - 1) / (S::BN / 2));
-        gated_gemm<D, S, decltype(deep)::value><<<dim3(tiles, p.slices), S::NT, 0, s>>>(a, b, half, M, N, K, p.slice_stages, parts, e);
+        gated_gemm<D, S, decltype(ring)::value><<<dim3(tiles, p.slices), S::NT, 0, s>>>(a, b, half, M, N, K, p.slice_stages, parts, e);
     };
-    const std::false_type two{};
-    const std::true_type four{};
+    const std::integral_constant<int, RING_TWO> two{};
+    const std::integral_constant<int, RING_DEEP> four{};
+    const std::integral_constant<int, RING_LOOSE> any{};
+    if (loose) {
+        if (p.tiling == 0) go(DenseShape<2, 2, 2, 2>{}, any);
+        else go(DenseShape<2, 2, 1, 2>{}, any);
+        return;
+    }
     switch (p.tiling) {
     case 0: go(DenseShape<2, 2, 4, 4>{}, two); break;
     case 1: go(DenseShape<2, 2, 2, 4>{}, two); break;
@@ -222,10 +244,10 @@ static void gated_tiling(const DenseOperand& a, const DenseOperand& b, int64_t h
     }
 }
 
-// How a call runs: few rows, or tiles in slices of K; where the copies of operands that cannot be loaded as they lie and the
+// How a call runs: few rows, or tiles in slices of K, of rows that start anywhere if loose; where the copies of operands that cannot be loaded as they lie and the
 // partial sums are in the workspace.
 struct GatedCall {
-    bool few;
+    bool few, loose;
     int slices;
     DensePlan tiles;
     int how_x, how_w;
@@ -242,8 +264,24 @@ static GatedCall gated_call(const DenseView& x, const DenseView& w, int64_t M, i
     c.parts_at = c.w_at + dense_copy_bytes(c.how_w, 2 * N, K);
     if (c.w_at) us += 3.0f + (float)c.w_at * 0.5e-6f;
     if (c.parts_at > c.w_at) us += 3.0f + (float)(c.parts_at - c.w_at) * 0.5e-6f;
+    auto rows = [](int how, const DenseView& v, int64_t R) {
+        return how == LIES_ALONG || (how == COPY_ALONG && (R == 1 || v.row <= (1 << 20)));
+    };
+    if (c.parts_at && K >= 8 && rows(c.how_x, x, M) && rows(c.how_w, w, 2 * N)) {
+        float any;
+        const DensePlan p = dense_plan_tiles(kLooseTiles, (int)(sizeof(kLooseTiles) / sizeof(kLooseTiles[0])), M, 2 * N, K,
+                                             EPI_ACT | (keep ? EPI_KEEP : 0), 7.0f, any);
+        if (any < us) {
+            us = any;
+            c.loose = true;
+            c.tiles = p;
+            c.slices = p.slices;
+            c.w_at = c.parts_at = 0;
+        }
+    }
     if (M <= 256 && x.col == 1 && w.col == 1 && dense_rows_time(M, 2 * N, K, ((x.row | w.row) & 1) != 0) < us) {
         c.few = true;
+        c.loose = false;
         c.slices = (N + 15) / 16 * ((M + 15) / 16) < 128 && K >= 4096 ? 4 : 1;
         c.w_at = c.parts_at = 0;
     }
@@ -296,11 +334,11 @@ extern "C" int wf_gated_dense_plan(const void* x, int64_t x_row, int64_t x_col, 
     plan[0] = plan[1] = plan[2] = plan[3] = plan[4] = 0;
     if (M == 0 || N == 0) return WF_OK;
     const GatedCall c = gated_call({x, x_row, x_col, false}, {w, w_row, w_col, false}, M, N, K, keep);
-    plan[0] = c.few ? 0 : 1;
+    plan[0] = c.few ? 0 : c.loose ? 2 : 1;
     plan[1] = c.few ? 0 : c.tiles.tiling;
     plan[2] = c.slices;
-    plan[3] = c.few ? LIES_ALONG : c.how_x;
-    plan[4] = c.few ? LIES_ALONG : c.how_w;
+    plan[3] = c.few || c.loose ? LIES_ALONG : c.how_x;
+    plan[4] = c.few || c.loose ? LIES_ALONG : c.how_w;
     *bytes = c.bytes;
     return WF_OK;
 }
@@ -332,10 +370,15 @@ extern "C" int wf_gated_dense(const void* x, int64_t x_row, int64_t x_col, const
                        (int)K, parts, e, s);
     } else {
         DenseOperand a, b;
-        dense_operands(xv, c.how_x, M, ws, wv, c.how_w, 2 * N, ws + c.w_at, K, a, b, s);
+        if (c.loose) {
+            a = {static_cast<const uint16_t*>(x), x_row, (int)K, (int)M, false};
+            b = {static_cast<const uint16_t*>(w), w_row, (int)K, (int)N, false};
+        } else {
+            dense_operands(xv, c.how_x, M, ws, wv, c.how_w, 2 * N, ws + c.w_at, K, a, b, s);
+        }
         b.rows = (int)N;
-        if (dt == WF_BF16) gated_tiling<WF_BF16>(a, b, N * b.row, (int)M, (int)N, (int)K, c.tiles, parts, e, s);
-        else gated_tiling<WF_F16>(a, b, N * b.row, (int)M, (int)N, (int)K, c.tiles, parts, e, s);
+        if (dt == WF_BF16) gated_tiling<WF_BF16>(a, b, N * b.row, (int)M, (int)N, (int)K, c.tiles, c.loose, parts, e, s);
+        else gated_tiling<WF_F16>(a, b, N * b.row, (int)M, (int)N, (int)K, c.tiles, c.loose, parts, e, s);
     }
     if (parts) {
         over_grids((M * ((N + 7) / 8) + 255) / 256, kGridMost, [&](int64_t wg, uint32_t n) {

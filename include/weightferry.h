@@ -256,7 +256,8 @@ int wf_dense_bwd(const void* x, int64_t x_row, const void* w, int64_t w_row, int
  * WF_F16), float32 accumulation, one rounding. w: [2 N, K], the gate's rows first; bias (may be NULL): [2 N] of type dt or
  * WF_F32; y: [M, N]; operands and act as in wf_dense. kept (may be NULL): 6 M N bytes, g and u in 24 bits for wf_gated_dense_bwd.
  * M <= 2^20, N <= 2^19, K <= 2^20. wf_gated_dense_plan: the workspace's bytes (256-byte aligned; it need not be cleared) and how
- * such a call runs, plan[5]: 0 few rows or 1 tiles, the tiling (0-4), slices of K, and how x and w get there as in wf_dense_plan. */
+ * such a call runs, plan[5]: 0 few rows, 1 tiles or 2 tiles of rows that start anywhere, the tiling (0-4; 0-1), slices of K, and how x
+ * and w get there as in wf_dense_plan. */
 int wf_gated_dense_plan(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt,
                         int64_t M, int64_t N, int64_t K, int keep, int* plan, int64_t* bytes);
 int wf_gated_dense(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_row, int64_t w_col, int dt, int64_t M,

@@ -80,7 +80,9 @@ SHAPES = [
     (5000, 333, 96), (536, 524, 4736), (803, 3008, 455), (3880, 1560, 576), (1096, 1903, 6264), (6080, 4, 400), (8224, 165, 2),
     (256, 2560, 5120), (1881, 3424, 736), (1419, 1655, 896), (1392, 1536, 5376), (904, 1135, 7552), (262, 6, 1152), (512, 16, 928),
     (2112, 1824, 648), (104, 1265, 3264), (3640, 1, 2934), (2225, 1295, 1744), (104, 1791, 2448), (8640, 1, 1152), (2113, 1824, 648),
-    (1984, 3200, 1302), (2048, 1040, 1814), (1420, 1656, 900), (1900, 3420, 737), (905, 1136, 7553), (1393, 1537, 5376), (263, 7, 1153), (513, 17, 928)]
+    (1984, 3200, 1302), (2048, 1040, 1814), (1420, 1656, 900), (1900, 3420, 737), (905, 1136, 7553), (1393, 1537, 5376), (263, 7, 1153), (513, 17, 928),
+    (7144, 1, 1992), (10104, 2, 1536), (4584, 5, 365), (1292, 528, 20), (622, 5320, 626), (3640, 2, 2935), (300, 200, 9), (301, 201, 65),
+    (330, 130, 8), (300, 200, 7), (260, 300, 127), (257, 65, 10)]
 
 
 @pytest.mark.parametrize("i", range(len(SHAPES)), ids=["x".join(map(str, s)) for s in SHAPES])
@@ -101,6 +103,20 @@ def test_gated_activations_with_float32_bias(native, act, dtype):
     t = make(96, 200, 160, getattr(torch, dtype), True, 11, torch.float32)
     _, grads = hold(t, act)
     assert grads["db"].dtype == torch.float32
+
+
+def test_gated_rows_that_start_anywhere(native):
+    # views at every place of a 16-byte run, row lengths of their own, the last row ending with its memory
+    for k in (8, 9, 15, 57, 64, 71, 128, 200, 449):
+        for place in range(0, 8, 1 if k < 64 else 3):
+            rows, n, x_row, w_row = 300 + place, 66 + k % 5, k + 3 * place + 1, k + place
+            t = make(rows, n, k, torch.float16, False, k)
+
+            def at(v, row, off):
+                whole = torch.full((off + (v.shape[0] - 1) * row + k,), float("nan"), dtype=v.dtype, device="cuda")
+                return torch.as_strided(whole, v.shape, (row, 1), off).copy_(v)
+            got = fd.gated_dense(at(t["x"], x_row, place), at(t["w"], w_row, 7 - place), None, "silu")
+            check(got, formula(t, "silu")["y"], f"k={k} place={place}")
 
 
 def test_gated_gradient_against_differences(native):
