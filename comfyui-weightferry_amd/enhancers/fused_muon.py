@@ -136,37 +136,42 @@ def _ready(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, 
     shapes, many = list(map(_shape, params)), len(params)
     if (set(map(_dtype, params + grads)) != {dt} or set(map(_dtype, momenta)) != {torch.float32}
             or set(map(_index, every)) != {dev.index} or not all(map(_contiguous, every))
-            or not _TYPES.issuperset(map(type, every)) or set(map(len, shapes)) != {2} or shapes != list(map(_shape, grads))
-            or list(map(_numel, params)) != list(map(_numel, momenta))):
+            or not _TYPES.issuperset(map(type, every)) or shapes != list(map(_shape, grads))):
         raise ValueError(_odd_one(params, grads, momenta, dt, dev))
     by_shape = {}
-    for i, shape in enumerate(shapes):
-        which = by_shape.get(shape)
+    for i, key in enumerate(zip(shapes, map(_numel, momenta))):
+        which = by_shape.get(key)
         if which is None:
-            by_shape[shape] = [i]
+            by_shape[key] = [i]
         else:
             which.append(i)
-    at, need, order, calls = list(map(_data_ptr, every)), 0, [], []
-    for (rows, cols), which in by_shape.items():
-        if rows and cols:
+    need, order, calls = 0, [], []
+    for (shape, values), which in by_shape.items():
+        if len(shape) != 2 or shape[0] * shape[1] != values:
+            raise ValueError(_odd_one(params, grads, momenta, dt, dev))
+        rows, cols = shape
+        if values:
             if not _fits(rows, cols):
                 raise ValueError(f"a matrix of {rows} x {cols}: the shorter side is at most {MAX_SHORT}, the longer {MAX_LONG}, "
                                  f"and there are fewer than {MAX_VALUES} values")
             # (contiguous, but not what its memory holds: only a single value can be both without a private call)
-            if rows * cols == 1 and any(t[i].is_neg() for t in (params, grads, momenta) for i in which):
+            if values == 1 and any(t[i].is_neg() for t in (params, grads, momenta) for i in which):
                 raise ValueError("a negative view: what it stands for is not in its memory")
             need = max(need, _bytes((len(which), rows, cols)))
             calls.append((24 * len(order), len(which), rows, cols, lr * _size(adjust, rows, cols)))
             order += which
-    changed = at[:many] + at[2 * many:] if len(order) == many else [at[i + k] for i in order for k in (0, 2 * many)]
-    if len(set(changed)) != len(changed):
+    at, table = list(map(_data_ptr, every)), array.array("q", bytes(24 * len(order)))
+    if len(order) > 1:
+        pick = operator.itemgetter(*order)
+        at_p, at_g, at_m = (pick(at[k * many:(k + 1) * many]) for k in range(3))
+    else:
+        at_p, at_g, at_m = ([at[i + k * many] for i in order] for k in range(3))
+    for k, column in enumerate((at_p, at_g, at_m)):
+        table[k::3] = array.array("q", column)
+    if len({*at_p, *at_m}) != 2 * len(order):
         raise ValueError("a parameter or a momentum is there twice: each is stepped on its own")
-    if dt == torch.float32 and not {at[i + many] for i in order}.isdisjoint(at[i + 2 * many] for i in order):
+    if dt == torch.float32 and not set(at_g).isdisjoint(at_m):
         raise ValueError("a gradient is a momentum's memory, which the step changes before it has read the gradient for the last time")
-    table = array.array("q", bytes(24 * len(order)))
-    for k in range(3):
-        column = at[k * many:(k + 1) * many]
-        table[k::3] = array.array("q", map(column.__getitem__, order))
 
     def launch():
         if not calls:
