@@ -148,7 +148,8 @@ def _launch_block(x2, h2, post_weight, gate, weight, bias, how, stats):
     """(r, or None without a branch, and y)"""
     rows, width = x2.shape
     dev = x2.device
-    y = torch.empty((rows, width), dtype=x2.dtype, device=dev)
+    # (the like of a contiguous tensor takes two thirds of the time)
+    y = torch.empty_like(x2) if x2.is_contiguous() else torch.empty((rows, width), dtype=x2.dtype, device=dev)
     r = None if h2 is None else torch.empty_like(y)
     if rows:
         q = _blocks(how)
