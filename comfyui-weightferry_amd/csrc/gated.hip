@@ -279,11 +279,18 @@ static GatedCall gated_call(const DenseView& x, const DenseView& w, int64_t M, i
             c.w_at = c.parts_at = 0;
         }
     }
-    if (M <= 256 && x.col == 1 && w.col == 1 && dense_rows_time(M, 2 * N, K, ((x.row | w.row) & 1) != 0) < us) {
-        c.few = true;
-        c.loose = false;
-        c.slices = (N + 15) / 16 * ((M + 15) / 16) < 128 && K >= 4096 ? 4 : 1;
-        c.w_at = c.parts_at = 0;
+    if (M <= 256 && x.col == 1 && w.col == 1) {
+        const int slices = (N + 15) / 16 * ((M + 15) / 16) < 128 && K >= 4096 ? 4 : 1;
+        float few = dense_rows_time(M, 2 * N, K, ((x.row | w.row) & 1) != 0);
+        // (loads at odd places, one after the other: us in this form / in tiles of such rows 20 x 600 x 4001 31.7 / 16.5, 1 x 600 x 4001
+        // 23.1 / 15.8, 8 x 1000 x 2047 20.9 / 15.9, 100 x 700 x 1025 21.8 / 14.3; 3 x 2607 x 1531 12.6 / 13.5)
+        if (c.loose) few = std::max(few * (M > 16 ? 1.25f : 1.0f), 4.0f + (4.5e-3f + 0.4e-3f * std::min<int64_t>(M, 8)) * (K / slices));
+        if (few < us) {
+            c.few = true;
+            c.loose = false;
+            c.slices = slices;
+            c.w_at = c.parts_at = 0;
+        }
     }
     c.bytes = c.parts_at + (c.slices > 1 ? (int64_t)c.slices * M * 2 * N * 4 : 0);
     return c;

@@ -82,7 +82,7 @@ SHAPES = [
     (2112, 1824, 648), (104, 1265, 3264), (3640, 1, 2934), (2225, 1295, 1744), (104, 1791, 2448), (8640, 1, 1152), (2113, 1824, 648),
     (1984, 3200, 1302), (2048, 1040, 1814), (1420, 1656, 900), (1900, 3420, 737), (905, 1136, 7553), (1393, 1537, 5376), (263, 7, 1153), (513, 17, 928),
     (7144, 1, 1992), (10104, 2, 1536), (4584, 5, 365), (1292, 528, 20), (622, 5320, 626), (3640, 2, 2935), (300, 200, 9), (301, 201, 65),
-    (330, 130, 8), (300, 200, 7), (260, 300, 127), (257, 65, 10)]
+    (330, 130, 8), (300, 200, 7), (260, 300, 127), (257, 65, 10), (1, 600, 4001), (8, 1000, 2047), (100, 700, 1025), (1, 9001, 2047)]
 
 
 @pytest.mark.parametrize("i", range(len(SHAPES)), ids=["x".join(map(str, s)) for s in SHAPES])
