@@ -511,7 +511,11 @@ static int muon_check(const char* who, int64_t count, int64_t rows, int64_t cols
         set_error("%s: the shorter side above 16384, the longer above 2^20 or 2^30 values", who);
         return WF_EUNSUPPORTED;
     }
-    // float16 holds what the steps pass through only while singular values stay small
+    // float16 holds what the steps pass through only while singular values stay small. (A maximum drops a NaN, so those are asked for.)
+    if (!std::isfinite(abc[0]) || !std::isfinite(abc[1]) || !std::isfinite(abc[2])) {
+        set_error("%s: coefficients %g, %g, %g", who, abc[0], abc[1], abc[2]);
+        return WF_EINVAL;
+    }
     double top = 1.0;
     for (int k = 0; k < steps; k++) {
         double next = 0.0, most = 0.0;
