@@ -134,14 +134,16 @@ def _block(*how):
     return ctypes.addressof(q), q
 
 
-def _ask_block(q, rows, width, sums):
-    need = ctypes.c_int64()
-    _native.call("wf_block_norm_bwd_workspace", q, rows, width, sums, ctypes.byref(need))
+_blocks = Sizes(_block)
+
+
+def _ask_block(how, rows, width, sums):
+    need, q = ctypes.c_int64(), _blocks(how)             # (q is held until the call is done: another thread may clear the cache)
+    _native.call("wf_block_norm_bwd_workspace", q[0], rows, width, sums, ctypes.byref(need))
     return need.value
 
 
-_blocks = Sizes(_block)
-_bytes_block = Sizes(lambda how, rows, width, sums: _ask_block(_blocks(how)[0], rows, width, sums))
+_bytes_block = Sizes(_ask_block)
 
 
 def _launch_block(x2, h2, post_weight, gate, weight, bias, how, stats):
