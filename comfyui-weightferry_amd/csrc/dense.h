@@ -109,6 +109,7 @@ struct DenseEpilogue {
     int act;
     int64_t rows_per_group, ldr;           // row m's gate is row m / rows_per_group of gate; resid's row stride
     void *y, *h;                           // [M, N]; h (may be NULL): the pre-activations
+    const float* alpha;                    // float16 alone, and beside it nothing else: the sums are multiplied by *alpha. Or NULL
 };
 
 // what a run at (m, n) of `cnt` values (8, or fewer at a row's end) needs from memory
@@ -134,6 +135,12 @@ template <int D, bool BIAS>
 __device__ __forceinline__ void epilogue_run(const DenseEpilogue& e, float (&v)[8], const EpilogueAhead<D>& a, int64_t m,
                                              int n, int N, int cnt) {
     float u[8];
+    if constexpr (BIAS && D == WF_F16)
+        if (e.alpha) {
+            const float alpha = *e.alpha;
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] *= alpha;
+        }
     if (BIAS && e.bias) {
         load_params<8>(u, e.bias, n, cnt, e.bias_dt);
 #pragma unroll

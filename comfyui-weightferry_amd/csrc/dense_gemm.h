@@ -37,7 +37,7 @@ __device__ __forceinline__ DenseTile dense_tile(const DenseOperand& o, int r0) {
 }
 
 // Workgroup (tile, slice). parts: [slices, M, N] float32 partial sums, or NULL: one slice, and the outputs. PLAIN: the
-// epilogue is at most a bias.
+// epilogue is at most a bias, or a factor.
 template <int D, bool AX, bool BX, bool PLAIN, typename S>
 __global__ __launch_bounds__(S::NT, S::WAVES) void dense_gemm(DenseOperand a, DenseOperand b, int M, int N, int K, int slice_stages,
                                                     float* __restrict__ parts, DenseEpilogue e) {
@@ -77,7 +77,12 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void dense_gemm(DenseOperand a, De
     };
     if constexpr (PLAIN) {
         if (!parts) {
-            store(e.y, [](float v) { return v; });
+            if constexpr (D == WF_F16) {
+                const float alpha = e.alpha ? *e.alpha : 1.0f;
+                store(e.y, [&](float v) { return v * alpha; });
+            } else {
+                store(e.y, [](float v) { return v; });
+            }
             return;
         }
     } else {

@@ -266,7 +266,8 @@ int wf_gated_dense(const void* x, int64_t x_row, int64_t x_col, const void* w, i
 
 /* Its backward pass for the gradient dy of y (rows dy_row values apart): dg = dy u act'(g), du = dy act(g), dh = [dg du] rounded to
  * dt, dx = dh w [M, K], dw = dh^T x [2 N, K], dbias the sums over rows of the unrounded dh [2 N]; any of the three may be NULL. Every
- * sum has a fixed order. */
+ * sum has a fixed order. WF_F16: where dh's largest finite magnitude is past 65504 or below 2^-8, dh is rounded times a power of two that
+ * brings it to 2^14, and the products are multiplied back. */
 int wf_gated_dense_bwd_workspace(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, int dt, int64_t M,
                                  int64_t N, int64_t K, int dx, int dw, int db, int64_t* bytes);
 int wf_gated_dense_bwd(const void* x, int64_t x_row, const void* w, int64_t w_row, int64_t w_col, const void* dy, int64_t dy_row,
