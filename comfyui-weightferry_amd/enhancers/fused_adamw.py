@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _native
-from .operands import CODES, plain
+from .operands import CODES, duals, plain
 
 BLOCK = 256
 _TYPES = frozenset((torch.Tensor, torch.nn.Parameter))
@@ -114,6 +114,8 @@ def _ready(params, grads, state, step, lr, betas, eps, weight_decay):
                            "replay would repeat them")
     if not plain(dev):
         raise ValueError("a step inside a functorch transform or a trace, which would not see it")
+    if duals(*params, *grads, *(t for t in state if t is not None)):
+        raise ValueError("a forward-mode tangent, which the step would leave behind")
     # (questions of all tensors at once: with hundreds of adapters they are the step's host time, 0.6 us a parameter; the numbers
     # of values are compared, not the shapes: that alone would be a third more)
     both, index, sizes = params + grads, dev.index, list(map(_numel, params))

@@ -11,7 +11,7 @@ import operator
 import torch
 
 from .. import _native
-from .operands import CODES, Sizes, plain, whole
+from .operands import CODES, Sizes, duals, plain, whole
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)     # steep at zero: small singular values grow by 3.4 a step; all end between 0.7 and 1.2
 _TYPES = frozenset((torch.Tensor, torch.nn.Parameter))
@@ -131,6 +131,8 @@ def _ready(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, 
                                "repeat them")
     if not plain(dev):
         raise ValueError("a step inside a functorch transform or a trace, which would not see it")
+    if duals(*params, *grads, *momenta):
+        raise ValueError("a forward-mode tangent, which the step would leave behind")
     # (questions of all tensors at once: with hundreds of adapters they are the step's host time, a microsecond a matrix)
     every = params + grads + momenta
     shapes, many = list(map(_shape, params)), len(params)

@@ -14,6 +14,16 @@ _jit_traces, _modes, _mode = torch._C._is_tracing, torch._C._len_torch_dispatch_
 _TRACERS = (torch._C._TorchDispatchModeKey.PROXY, torch._C._TorchDispatchModeKey.FAKE)
 
 
+def _dual(t):
+    return _wrapped(t) or t._is_zerotensor() or forward_ad.unpack_dual(t).tangent is not None
+
+
+def duals(*tensors):
+    """Whether forward mode is at work and one of ``tensors`` carries a tangent, which an operation in place on its memory alone
+    would leave behind."""
+    return forward_ad._current_level >= 0 and any(map(_dual, tensors))
+
+
 def plain(device, *tensors):
     """Whether each of ``tensors`` is None or an ordinary tensor on ``device``, outside functorch's transforms and traces."""
     if _level() is not None or _jit_traces():
@@ -26,7 +36,7 @@ def plain(device, *tensors):
             continue
         if type(t) not in _TYPES or t.device != device or t.is_neg():
             return False
-        if deep and (_wrapped(t) or t._is_zerotensor() or forward_ad.unpack_dual(t).tangent is not None):
+        if deep and _dual(t):
             return False
     return True
 
