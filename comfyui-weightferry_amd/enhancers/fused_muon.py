@@ -7,11 +7,12 @@ import array
 import ctypes
 import math
 import operator
+import warnings
 
 import torch
 
 from .. import _native
-from .operands import CODES, Sizes, duals, plain, whole
+from .operands import CODES, Sizes, duals, plain, wants_grad, whole
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)     # steep at zero: small singular values grow by 3.4 a step; all end between 0.7 and 1.2
 _TYPES = frozenset((torch.Tensor, torch.nn.Parameter))
@@ -57,7 +58,8 @@ def _polynomial(steps, coefficients, eps):
 
 def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     """``x`` [..., M, N] over its Frobenius norm (at least ``eps``), matrix by matrix, then ``steps`` times a X + (b A + c A A) X
-    with A = X X^T: each singular value v put through a v + b v^3 + c v^5. float16, bfloat16 or float32, any strides; no gradient. With a
+    with A = X X^T: each singular value v put through a v + b v^3 + c v^5. float16, bfloat16 or float32, any strides. No gradient is
+    recorded (a UserWarning says so where one would have been). With a
     shorter side up to 64 nothing is rounded before the result; above, the result is good to 1e-3 of its norm whatever its type (the
     products take float16). None when it is not the kernel's case (no plain GPU tensor, another type, a shorter side above 16384, a
     longer one above 2^20, 2^30 values); ValueError for coefficients that let singular values grow past 1.9."""
@@ -68,6 +70,8 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     rows, cols = x.shape[-2:]
     if code is None or dev.type != "cuda" or not plain(dev, x) or not _fits(rows, cols):
         return None
+    if wants_grad(x):
+        warnings.warn("orthogonalize records no gradient: its result is a constant to autograd", stacklevel=2)
     x = whole(x.detach())
     out = torch.empty_like(x)
     if not x.numel():
