@@ -81,6 +81,7 @@ EXPORTS = {
     "wf_adamw": (_int, [_p, _i64, _int, _int, _p, _p, _p, _p, _i64, _i64] + [ctypes.c_double] * 5 + [_p]),
     "wf_adamw_values": (_int, [_p, _p, _p, _p, _i64, _p, _p, _p]),
     "wf_muon_workspace": (_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "wf_muon_plan": (_int, [_i64, _i64, _i64, ctypes.POINTER(_int)]),
     "wf_muon": (_int, [_p, _i64, _i64, _i64, _int, ctypes.c_double, _int, ctypes.c_double, ctypes.c_double, _int, _p,
                        ctypes.c_double, _p, _i64, _p]),
     "wf_orthogonalize": (_int, [_p, _i64, _i64, _i64, _int, _int, _p, ctypes.c_double, _p, _i64, _p]),

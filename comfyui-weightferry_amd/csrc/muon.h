@@ -41,6 +41,10 @@ struct MuonUpdate {
     float alpha, a;
 };
 
+// how a batch's products run: the tiling of a symmetric product (square: of A, else of X) and its slices of the sum, of the update
+void muon_symmetric_form(const MuonShape& s, bool square, int& tiling, int& slices);
+int muon_update_tiling(const MuonShape& s);
+
 int64_t muon_symmetric_bytes(const MuonShape& s, bool square);      // of float32 partial sums
 void muon_symmetric(const MuonShape& s, const MuonSymmetric& q, float* parts, hipStream_t st);
 void muon_update(const MuonShape& s, const MuonUpdate& q, const MuonTensors& t, hipStream_t st);

@@ -577,6 +577,23 @@ extern "C" int wf_muon_workspace(int64_t count, int64_t rows, int64_t cols, int6
     return WF_OK;
 }
 
+extern "C" int wf_muon_plan(int64_t count, int64_t rows, int64_t cols, int* plan) {
+    using namespace wf;
+    const double abc[3] = {1.0, 0.0, 0.0};
+    if (!plan) { set_error("wf_muon_plan: null pointer"); return WF_EINVAL; }
+    if (const int rc = muon_check("wf_muon_plan", count, rows, cols, WF_F32, 1, abc)) return rc;
+    for (int i = 0; i < 7; i++) plan[i] = 0;
+    if (!count || !rows || !cols) return WF_OK;
+    const MuonPlan p = muon_plan(rows, cols, count);
+    plan[0] = p.batch;
+    plan[1] = p.mt;
+    if (p.narrow) return WF_OK;
+    muon_symmetric_form(p.s, false, plan[2], plan[3]);
+    muon_symmetric_form(p.s, true, plan[4], plan[5]);
+    plan[6] = muon_update_tiling(p.s);
+    return WF_OK;
+}
+
 extern "C" int wf_muon(const int64_t* table, int64_t count, int64_t rows, int64_t cols, int dt, double momentum, int nesterov,
                        double keep, double rate, int steps, const double* coefficients, double eps, void* workspace,
                        int64_t workspace_bytes, void* stream) {

@@ -339,6 +339,12 @@ static MuonSlices muon_symmetric_plan(const MuonShape& s, int64_t K) {
 }
 static int muon_symmetric_k(const MuonShape& s, bool square) { return square ? s.sld : s.tall ? s.rows : s.ld; }
 
+void muon_symmetric_form(const MuonShape& s, bool square, int& tiling, int& slices) {
+    const MuonSlices p = muon_symmetric_plan(s, muon_symmetric_k(s, square));
+    tiling = p.tiling;
+    slices = p.slices;
+}
+
 int64_t muon_symmetric_bytes(const MuonShape& s, bool square) {
     const MuonSlices p = muon_symmetric_plan(s, muon_symmetric_k(s, square));
     const int64_t bm = kSymmetric[p.tiling].bm;
@@ -376,7 +382,7 @@ void muon_symmetric(const MuonShape& s, const MuonSymmetric& q, float* parts, hi
 constexpr MuonTile kUpdate[] = {{256, 320, 1, 12.3f, 1.70f, 1.70f}, {256, 192, 1, 13.3f, 1.12f, 1.12f},
                                 {128, 128, 2, 5.5f, 0.57f, 0.50f}, {64, 64, 2, 2.7f, 0.20f, 0.19f}};
 
-void muon_update(const MuonShape& s, const MuonUpdate& q, const MuonTensors& t, hipStream_t st) {
+int muon_update_tiling(const MuonShape& s) {
     int tiling = 0;
     float least = 1e30f;
     for (int i = 0; i < 4; i++) {
@@ -385,6 +391,11 @@ void muon_update(const MuonShape& s, const MuonUpdate& q, const MuonTensors& t, 
         const float c = muon_time(z, wgs, (s.side + 63) / 64);
         if (c < least) least = c, tiling = i;
     }
+    return tiling;
+}
+
+void muon_update(const MuonShape& s, const MuonUpdate& q, const MuonTensors& t, hipStream_t st) {
+    const int tiling = muon_update_tiling(s);
     const int64_t x_step = (int64_t)s.rows * s.ld, q_step = (int64_t)s.side * s.sld;
     const DenseOperand q_along = {q.q, s.sld, s.sld, s.side, false};
     auto go = [&](auto bx, auto shape) {

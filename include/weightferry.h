@@ -294,8 +294,11 @@ int wf_adamw_values(const int8_t* exp_avg, const uint8_t* exp_avg_sq, const floa
  * (float32) may be 0: u = g. coefficients: a, b, c; WF_EINVAL for ones that take singular values from [0, 1] past 1.9. The shorter side
  * <= 16384, the longer <= 2^20, (rows + 256) (cols + 8) < 2^30. No matrix may be there twice. With a shorter side up to 64 everything
  * is float32 or more; above, the products' operands are float16 and X is good to 1e-3 of its norm. wf_orthogonalize: out = X, table:
- * addresses of out, g and 0. The workspace (256-byte aligned) need not be cleared. */
+ * addresses of out, g and 0. The workspace (256-byte aligned) need not be cleared. wf_muon_plan: how such a call runs, plan[7]: matrices a
+ * launch (what is left behind the last whole batch runs as a call of that many), 16-row tiles of the shorter side where everything runs on the
+ * Gram matrix (1-4; then nothing follows), or 0; the tiling (0-2) and slices of the sum of X X^T, of its square, the update's tiling (0-3). */
 int wf_muon_workspace(int64_t count, int64_t rows, int64_t cols, int64_t* bytes);
+int wf_muon_plan(int64_t count, int64_t rows, int64_t cols, int* plan);
 int wf_muon(const int64_t* table, int64_t count, int64_t rows, int64_t cols, int dt, double momentum, int nesterov, double keep,
             double rate, int steps, const double* coefficients, double eps, void* workspace, int64_t workspace_bytes, void* stream);
 int wf_orthogonalize(const int64_t* table, int64_t count, int64_t rows, int64_t cols, int dt, int steps, const double* coefficients,
