@@ -10,8 +10,10 @@
 //
 // Shorter side above 64: float16 tiles (muon_gemm.hip). Everything there is bounded (sigma <= 2, which the host checks), so float16's 11 bits
 // serve where bfloat16's 8 would: the direction is off by 1e-3 of its norm against 1e-2, and in gradients whose singular values
-// fall off fast, where X is carried with the remainder of its rounding until the last two steps, by 1e-3 against 5e-2. Powers of
-// two keep the small entries of X and A in float16's normal range.
+// fall off fast, where X is carried with the remainder of its rounding until the last two steps, by 1e-3 against 5e-2. The five steps
+// multiply a singular value's relative error by up to 10, and each adds roundings: the fewer singular values hold a matrix, the less they
+// average, up to 4e-3 where a few directions do, 1.5e-2 for two or three entries alone. That is so for float32 matrices too: float32
+// matrix instructions have a sixteenth of the rate. Powers of two keep the small entries of X and A in float16's normal range.
 //
 // Up to 64: the steps run on the Gram matrix, in float64. G = u u^T is summed from the float32 u, then P = the product of the steps'
 // polynomials of G / |u|^2, each a 64 x 64 matrix product in one workgroup's LDS, then O = P u / |u|. That is two reads of u and three

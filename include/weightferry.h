@@ -293,8 +293,9 @@ int wf_adamw_values(const int8_t* exp_avg, const uint8_t* exp_avg_sq, const floa
  * keep p - rate X, in place (p and m). table: host memory, read before the call returns: addresses of p, g and m of each matrix; m
  * (float32) may be 0: u = g. coefficients: a, b, c; WF_EINVAL for ones that take singular values from [0, 1] past 1.9. The shorter side
  * <= 16384, the longer <= 2^20, (rows + 256) (cols + 8) < 2^30. No matrix may be there twice. With a shorter side up to 64 everything
- * is float32 or more; above, the products' operands are float16 and X is good to 1e-3 of its norm. wf_orthogonalize: out = X, table:
- * addresses of out, g and 0. The workspace (256-byte aligned) need not be cleared. wf_muon_plan: how such a call runs, plan[7]: matrices a
+ * is float32 or more; above, the products' operands are float16, for float32 matrices too, and X is off by about 1e-3 of its norm for flat and
+ * falling spectra, by up to 4e-3 where few directions hold nearly all of a matrix, 1.5e-2 where two or three entries do (singular values on
+ * the polynomial's steep parts). wf_orthogonalize: out = X, table: addresses of out, g and 0. The workspace (256-byte aligned) need not be cleared. wf_muon_plan: how such a call runs, plan[7]: matrices a
  * launch (what is left behind the last whole batch runs as a call of that many), 16-row tiles of the shorter side where everything runs on the
  * Gram matrix (1-4; then nothing follows), or 0; the tiling (0-2) and slices of the sum of X X^T, of its square, the update's tiling (0-3). */
 int wf_muon_workspace(int64_t count, int64_t rows, int64_t cols, int64_t* bytes);
