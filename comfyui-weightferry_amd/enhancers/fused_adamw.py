@@ -114,11 +114,11 @@ def _ready(params, grads, state, step, lr, betas, eps, weight_decay):
                            "replay would repeat them")
     if not plain(dev):
         raise ValueError("a step inside a functorch transform or a trace, which would not see it")
-    if duals(*params, *grads, *(t for t in state if t is not None)):
-        raise ValueError("a forward-mode tangent, which the step would leave behind")
     # (questions of all tensors at once: with hundreds of adapters they are the step's host time, 0.6 us a parameter; the numbers
     # of values are compared, not the shapes: that alone would be a third more)
     both, index, sizes = params + grads, dev.index, list(map(_numel, params))
+    if duals(both) or duals(t for t in state if t is not None):
+        raise ValueError("a forward-mode tangent, which the step would leave behind")
     if (set(map(_dtype, both)) != {dt} or set(map(_index, both)) != {index} or not all(map(_contiguous, both))
             or sizes != list(map(_numel, grads)) or not _TYPES.issuperset(map(type, both))):
         raise ValueError(_odd_one(params, grads, dt, dev))

@@ -136,10 +136,10 @@ def _ready(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, 
                                "repeat them")
     if not plain(dev):
         raise ValueError("a step inside a functorch transform or a trace, which would not see it")
-    if duals(*params, *grads, *momenta):
-        raise ValueError("a forward-mode tangent, which the step would leave behind")
     # (questions of all tensors at once: with hundreds of adapters they are the step's host time, a microsecond a matrix)
     every = params + grads + momenta
+    if duals(every):
+        raise ValueError("a forward-mode tangent, which the step would leave behind")
     shapes, many = list(map(_shape, params)), len(params)
     if (set(map(_dtype, params + grads)) != {dt} or set(map(_dtype, momenta)) != {torch.float32}
             or set(map(_index, every)) != {dev.index} or not all(map(_contiguous, every))

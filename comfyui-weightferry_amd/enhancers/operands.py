@@ -18,8 +18,8 @@ def _dual(t):
     return _wrapped(t) or t._is_zerotensor() or forward_ad.unpack_dual(t).tangent is not None
 
 
-def duals(*tensors):
-    """Whether forward mode is at work and one of ``tensors`` carries a tangent, which an operation in place on its memory alone
+def duals(tensors):
+    """Whether forward mode is at work and one of ``tensors`` (an iterable) carries a tangent, which an operation in place on its memory alone
     would leave behind."""
     return forward_ad._current_level >= 0 and any(map(_dual, tensors))
 
