@@ -6,8 +6,6 @@
 
 namespace wf {
 
-inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-
 // a tiling in the time model of dense.hip: its outputs, workgroups a CU, us of a workgroup and of each 64 values of K
 struct DenseTiling {
     int bm, bn, per_cu;

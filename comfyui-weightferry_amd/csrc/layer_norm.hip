@@ -254,13 +254,13 @@ constexpr int kLnMaxWidth = 32768;
 // 3000 x 8192 float32 (16 waves) with one a CU 32.8, with three 35.6. 16384 x 5120 takes 64 us, 5.2 TB/s. Rows of one pack a
 // lane use half the registers: 30000 x 256 in three workgroups of 8 waves a CU 13.0, in three of 5 14.4.
 static RowShape ln_fwd_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt) {
-    return K <= 64 * (dt == WF_F32 ? 4 : 8) ? row_shape(M, K, rows_per_group, dt, 8, 24, 3)
-                                            : row_shape(M, K, rows_per_group, dt, 5, 16, 8);
+    return K <= 64 * (dt == WF_F32 ? 4 : 8) ? row_shape(M, K, rows_per_group, dt, 2, 8, 24, 3)
+                                            : row_shape(M, K, rows_per_group, dt, 2, 5, 16, 8);
 }
 // Backward: one workgroup of up to 16 waves a CU, since every workgroup writes a row of partial sums: 4096 x 5120 takes
 // 35.7 us with 256, 37.9 with 512 of half the teams, 42.4 with 512 whole ones. 16384 x 5120: 98 us, 5.2 TB/s.
 static RowShape ln_bwd_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt) {
-    return row_shape(M, K, rows_per_group, dt, 16, 16, 1);
+    return row_shape(M, K, rows_per_group, dt, 2, 16, 16, 1);
 }
 
 // f with a lane's packs as a constant: the next of 1, 2, 3, 4, 6, 8 (a row of 32768 values over 16 waves has 4, or 8 of

@@ -284,7 +284,8 @@ struct MuonSteps {
 // (a norm of float32 values is zero or above 1e-45: a smaller eps means the same, and 1 / eps^2 has to be finite)
 static MuonSteps muon_steps(int steps, const double* abc, double eps) { return {steps, abc[0], abc[1], abc[2], std::max(eps, 1e-60)}; }
 
-// From the sums to P / max(|u|, eps): a workgroup a matrix. out: [batch, 16 MT, 16 MT].
+// From the sums to P / max(|u|, eps): a workgroup a matrix, which adds its stretches in turn: 16 us at 8 of them (32 rows), 49 at 54 (64 rows),
+// but 1080 at 4096, the longest side there is, where orthogonalising 64 x 2^20 takes 1550. out: [batch, 16 MT, 16 MT].
 template <int MT>
 __global__ __launch_bounds__(1024) void narrow_steps(const f64x4* __restrict__ parts, int stretches, MuonSteps s, double* __restrict__ out) {
     constexpr int TILES = MT * (MT + 1) / 2, M = 16 * MT, ROW = M + 2;      // (two rows' lanes then lie in different banks)
@@ -411,8 +412,6 @@ __global__ __launch_bounds__(256, (MT <= 2 ? 4 : 2)) void narrow_apply(MuonTenso
 }
 
 // ------------------------------------------------------------------------------------------------- host side
-static int64_t up_to(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-
 // How matrices of a shape are stepped: `batch` at a time, and where what they need is in the workspace.
 struct MuonPlan {
     bool narrow;
@@ -430,19 +429,19 @@ static MuonPlan muon_plan(int64_t rows, int64_t cols, int64_t count) {
         p.batch = (int)std::min<int64_t>(count, kMuonBatch);
         p.mt = (int)(side + 15) / 16;
         p.stretches = (int)((n + kStretch - 1) / kStretch);
-        p.sums_at = up_to((int64_t)p.batch * p.stretches * p.mt * (p.mt + 1) / 2 * 64 * 32, 256);
+        p.sums_at = up((int64_t)p.batch * p.stretches * p.mt * (p.mt + 1) / 2 * 64 * 32, 256);
         p.bytes = p.sums_at + (int64_t)p.batch * 256 * p.mt * p.mt * 8;
         return p;
     }
     // as many matrices at a time as fill the chip a few times over: more would only take more memory
     const int64_t tiles = ((rows + 127) / 128) * ((cols + 127) / 128);
     p.batch = (int)std::min<int64_t>(std::min<int64_t>(count, kMuonBatch), std::max<int64_t>(1, 4096 / tiles));
-    p.chunk = up_to(std::max<int64_t>(8192, (size + 1023) / 1024), 8);
+    p.chunk = up(std::max<int64_t>(8192, (size + 1023) / 1024), 8);
     p.parts = (size + p.chunk - 1) / p.chunk;
     p.scale = std::exp2(std::floor(0.5 * std::log2((double)side)) - 1.0);
-    p.s = {(int)rows, (int)cols, (int)up_to(cols, 8), (int)side, (int)up_to(side, 8), p.batch, rows > cols};
-    const int64_t x = up_to((int64_t)p.batch * rows * p.s.ld * 2, 256), a = up_to((int64_t)p.batch * side * p.s.sld * 2, 256);
-    p.x_at = up_to((int64_t)p.batch * p.parts * 8, 256);
+    p.s = {(int)rows, (int)cols, (int)up(cols, 8), (int)side, (int)up(side, 8), p.batch, rows > cols};
+    const int64_t x = up((int64_t)p.batch * rows * p.s.ld * 2, 256), a = up((int64_t)p.batch * side * p.s.sld * 2, 256);
+    p.x_at = up((int64_t)p.batch * p.parts * 8, 256);
     p.y_at = p.x_at + x;
     p.lo_at = p.y_at + x;
     p.a_at = p.lo_at + x;

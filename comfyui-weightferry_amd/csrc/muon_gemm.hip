@@ -168,8 +168,9 @@ __global__ __launch_bounds__(S::NT, (MuonLoop<S, X, X>::WAVES)) void muon_sym(De
 
 // Workgroup: a tile of a matrix's outputs [rows, cols]; BX: b lies across K.
 template <bool BX, typename S>
-__global__ __launch_bounds__(S::NT, (MuonLoop<S, false, BX>::WAVES)) void muon_upd(DenseOperand a, int64_t a_step, DenseOperand bo, int64_t b_step, MuonUpdate q,
-                                                            int64_t x_step, int rows, int cols, int ld, int K, MuonTensors t) {
+__global__ __launch_bounds__(S::NT, (MuonLoop<S, false, BX>::WAVES)) void muon_upd(DenseOperand a, int64_t a_step, DenseOperand bo,
+                                                                                   int64_t b_step, MuonUpdate q, int64_t x_step,
+                                                                                   int rows, int cols, int ld, int K, MuonTensors t) {
     constexpr int WM = S::WM, WN = S::WN, TC = WN * 32;
     using Loop = MuonLoop<S, false, BX>;
     __shared__ wl_frag sb0[S::SLOTS], sb1[S::SLOTS], sb2[Loop::MORE], sb3[Loop::MORE];

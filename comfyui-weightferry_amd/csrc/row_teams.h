@@ -31,12 +31,15 @@ __device__ __forceinline__ float2 team_sum2(float a, float b, int W, float* red,
 struct RowShape {
     int waves, packs, teams, parts;      // a row's waves, a lane's packs, a workgroup's teams, workgroups a group of rows
 };
-// Two packs a lane, then more waves (up to 16); teams up to team_waves waves a workgroup, fewer where that would leave CUs
+// packs of a lane, if a row had one wave
+inline int64_t row_packs(int64_t K, int dt) { return (K * value_bytes(dt) + 1023) / 1024; }
+// lane_packs packs a lane, then more waves (up to 16); teams up to team_waves waves a workgroup, fewer where that would leave CUs
 // idle; workgroups over all groups: as many a CU as make cu_waves waves of it, at most per_cu.
-inline RowShape row_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt, int team_waves, int cu_waves, int per_cu) {
-    const int64_t lane = 64 * (dt == WF_F32 ? 4 : 8), packs = (K + lane - 1) / lane;   // of a lane, if the row had one wave
+inline RowShape row_shape(int64_t M, int64_t K, int64_t rows_per_group, int dt, int lane_packs, int team_waves, int cu_waves,
+                          int per_cu) {
+    const int64_t packs = row_packs(K, dt);
     RowShape s;
-    s.waves = (int)std::min<int64_t>(16, (packs + 1) / 2);
+    s.waves = (int)std::min<int64_t>(16, (packs + lane_packs - 1) / lane_packs);
     s.packs = (int)((packs + s.waves - 1) / s.waves);
     s.teams = (int)std::max<int64_t>(1, std::min<int64_t>(team_waves / s.waves, M / 256));
     const int64_t wgs = 256 * std::max(1, std::min(per_cu, cu_waves / (s.waves * s.teams)));

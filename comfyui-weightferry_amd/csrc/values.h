@@ -11,6 +11,7 @@ template <int D> struct ValueType { typedef uint16_t T; };
 template <> struct ValueType<WF_F32> { typedef float T; };
 template <int D> using value_t = typename ValueType<D>::T;
 
+inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 inline int value_bytes(int dt) { return dt == WF_F32 ? 4 : 2; }
 inline bool known_dtype(int dt) { return dt == WF_F16 || dt == WF_BF16 || dt == WF_F32; }
 
